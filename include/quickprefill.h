@@ -55,7 +55,7 @@ int qp_create(qp_ctx** out, int device);
 int qp_dev_switch(const char* name, int value);
 void qp_destroy(qp_ctx* ctx);
 const char* qp_last_error(void);
-const char* qp_version(void);          /* "quickprefill-mi355x 0.7 (gfx950)": 0.3 prune_mode became a per-call argument; 0.4 qp_prefill_segment; 0.5 qp_linear_plan_choice; 0.6 qp_frame_ring_*; 0.7 qp_linear_plan_choice returns a status, qp_frame_ring_acquire_for, qp_patchify */
+const char* qp_version(void);          /* "quickprefill-mi355x 0.8 (gfx950)": 0.3 prune_mode became a per-call argument; 0.4 qp_prefill_segment; 0.5 qp_linear_plan_choice; 0.6 qp_frame_ring_*; 0.7 qp_linear_plan_choice returns a status, qp_frame_ring_acquire_for, qp_patchify; 0.8 qp_batch_*, qp_verify_drafts */
 int qp_device_cus(const qp_ctx* ctx);
 
 /* Host helper of the overlap producer (no device work): memcpy `bytes` from src to dst (e.g. decoded uint8 frames into a pinned
@@ -274,6 +274,55 @@ int qp_decode_attn_fused(qp_ctx* ctx, const void* qkv, const void* cos, const vo
 /* state[i] += 1 for i < n_values (end of the step; the state blocks of all layers are one array: layers may hold
  * different numbers of rows under the decaying keep ratios, utils.py:231-251). */
 int qp_decode_advance(qp_ctx* ctx, int64_t* state, int64_t n_values, void* stream);
+
+/* ---- a batch of sequences over one prefilled video -----------------------------------------------------------------------------
+ * Beams, sampled answers, several questions, drafted tokens (the reference hands `num_beams`, `prompt_lookup_num_tokens`, ... to HF
+ * generate, lvu/models/qwen25_lvu.py:744-761): `batch` sequences share the video's K/V rows of a layer ([0, prefix_len) of the arena,
+ * frozen meanwhile), and every sequence keeps the rows of its own tokens in pages.
+ *   pages        K and V bf16, page p at k_pages + p * page_stride (elements): [n_kv_heads][page_size][128]; any page_size >= 1
+ *   page_table   int32 [batch][max_pages] (device): key row j of sequence b is slot j % page_size of page page_table[b][j / page_size].
+ *                Sequences may name the same page for reading; a page that rows are stored into belongs to ONE sequence.
+ *   seq_len      int32 [batch] (device): rows stored before this step.  The caller adds what it keeps after the step (n_new for a decode
+ *                step, accepted + 1 after qp_verify_drafts: rows behind seq_len are overwritten by the next step).
+ *   n_new        int32 [batch] (device) or NULL = t_max for all: tokens of this step, clamped to [0, t_max].  Row (b, t) with
+ *                t >= n_new[b] is not read, not stored, and its outputs are left as they were.
+ * Lengths and tables are read on the device: a captured step replays with new ones.  A page number outside [0, n_pages), a row behind
+ * max_pages * page_size or a negative seq_len is never followed: such a row is not stored, and not attended.
+ * batch * t_max <= 65536; the context's device need not be the current one, `stream` must be the context device's.                    */
+/* Rotates the step's queries and keys and stores keys and values into the pages.  qkv bf16 [batch][t_max][(n_q + 2 n_kv) * 128]; cos /
+ * sin bf16 [batch][t_max][64] (qp_mrope_table over batch * t_max positions); q_out bf16 [batch][t_max][n_q][128], not overlapping qkv.
+ * Rotate-half as in qp_rope_append, in fp32 with ONE rounding to bf16 (qp_rope_append rounds after each step). */
+int qp_batch_rope_append(qp_ctx* ctx, const void* qkv, const void* cos, const void* sin, int batch, int t_max, const int32_t* seq_len,
+                         const int32_t* n_new, int n_q_heads, int n_kv_heads, int head_dim, void* q_out, void* k_pages, void* v_pages,
+                         int64_t page_stride, int n_pages, int page_size, const int32_t* page_table, int max_pages, void* stream);
+/* Query (b, t) attends the prefix rows [0, prefix_len) and its sequence's rows j <= seq_len[b] + t (the step's rows must have been
+ * appended).  The prefix is read once for the whole batch.  GQA native, any n_q / n_kv ratio.  q, out bf16 [batch][t_max][n_q][128] (out
+ * may be q).  A row that sees no key is zero; what a masked row holds (infinities, NaN) does not reach the result.  prefix tensors may
+ * be NULL when prefix_len is 0.  workspace: qp_batch_attn_workspace_bytes with suffix_capacity = max_pages * page_size; a caller with
+ * two of these calls in flight at once (two streams, two captured graphs) gives each its own. */
+size_t qp_batch_attn_workspace_bytes(const qp_ctx* ctx, int batch, int t_max, int64_t prefix_len, int64_t suffix_capacity, int n_q_heads,
+                                     int n_kv_heads);
+int qp_batch_attn(qp_ctx* ctx, const void* q, const void* k_prefix, const void* v_prefix, int64_t prefix_head_stride, int64_t prefix_len,
+                  const void* k_pages, const void* v_pages, int64_t page_stride, int n_pages, int page_size, const int32_t* page_table,
+                  int max_pages, const int32_t* seq_len, const int32_t* n_new, int batch, int t_max, int n_q_heads, int n_kv_heads,
+                  int head_dim, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
+/* How many of the drafted tokens stand against the model's distribution, and the token that follows them (speculative sampling, with
+ * the caller's random numbers; with t_max = 0 plain sampling of a batch).  logits [batch][t_max + 1][vocab] bf16, or fp32 with logits_f32
+ * (strides in elements, rows contiguous, any alignment): row t is the distribution that drafts[b][t] (int64 [batch][t_max]) is held against,
+ * row n_draft[b] the one behind the last draft.  n_draft int32 [batch] (device; NULL = t_max; -1 = an idle place of the batch).
+ * p_t = softmax(logits / temperature); draft t stands while uniforms[b][t] * q_t(draft) < p_t(draft), q = draft_probs fp32
+ * [batch][t_max][vocab], NULL = 1 at the draft (lookup drafts).  At the first refusal the next token is drawn from max(p - q, 0) (from p
+ * where that is all zero), otherwise from the row behind the last draft: the lowest token whose running sum exceeds
+ * uniforms[b][t_max] * total.  uniforms fp32 [batch][t_max + 1] in [0, 1).  temperature 0: greedy, draft t stands while it is the argmax
+ * (lowest index); uniforms and draft_probs are not read.  -infinity and NaN logits are never chosen; infinite ones share the row.
+ * Out: n_accepted int32 [batch]; tokens int64 [batch][t_max + 1] = the accepted drafts, the next token, -1 ... (all -1, 0 accepted where
+ * idle; -1 as next token where a row offers nothing; a draft outside the vocabulary is refused).
+ * vocab <= 4194304, t_max <= 255, batch <= 65535. */
+size_t qp_verify_drafts_workspace_bytes(int batch, int t_max, int64_t vocab);
+int qp_verify_drafts(qp_ctx* ctx, const void* logits, int logits_f32, int64_t logits_seq_stride, int64_t logits_row_stride, const int64_t* drafts,
+                     const int32_t* n_draft, const float* draft_probs, int64_t probs_seq_stride, int64_t probs_row_stride, const float* uniforms,
+                     int batch, int t_max, int64_t vocab, float temperature, int32_t* n_accepted, int64_t* tokens, void* workspace,
+                     size_t workspace_bytes, void* stream);
 
 /* ---- vision front end (transformers Qwen2VisionTransformerPretrainedModel [3P]) ---------------
  * The ViT tower itself runs on PyTorch-ROCm (quickvideo_amd/vit.py); these three entry points replace its non-GEMM ops.

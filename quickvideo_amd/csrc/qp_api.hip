@@ -48,7 +48,7 @@ static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t
 extern "C" {
 
 const char* qp_last_error(void) { return g_err; }
-const char* qp_version(void) { return "quickprefill-mi355x 0.7 (gfx950)"; }
+const char* qp_version(void) { return "quickprefill-mi355x 0.8 (gfx950)"; }
 
 int qp_dev_switch(const char* name, int value) {
   QP_REQUIRE(name != nullptr, QP_ERR_INVALID, "qp_dev_switch: name is NULL");
@@ -690,6 +690,120 @@ int qp_decode_advance(qp_ctx* ctx, int64_t* state, int64_t n_values, void* strea
   QP_REQUIRE(ctx && state, QP_ERR_INVALID, "qp_decode_advance: NULL argument");
   QP_REQUIRE(n_values > 0 && n_values <= (1 << 20), QP_ERR_INVALID, "qp_decode_advance: n_values=%lld", (long long)n_values);
   return qp_launch_decode_advance(state, (int)n_values, (hipStream_t)stream);
+}
+
+// ---- batch of sequences over one prefilled video ----------------------------------------------------------------------------------
+// the operators of this section may be called with another device current than the context's
+namespace {
+struct DeviceScope {
+  int back = -1;
+  explicit DeviceScope(int device) {
+    int cur = device;
+    if (hipGetDevice(&cur) == hipSuccess && cur != device && hipSetDevice(device) == hipSuccess) back = cur;
+  }
+  ~DeviceScope() { if (back >= 0) (void)hipSetDevice(back); }
+};
+
+int check_pages(const char* who, int64_t page_stride, int n_pages, int page_size, int max_pages, int n_kv_heads, const void* k_pages, const void* v_pages) {
+  QP_REQUIRE(n_pages >= 1 && page_size >= 1 && max_pages >= 1, QP_ERR_INVALID, "%s: n_pages=%d, page_size=%d, max_pages=%d must be >= 1", who, n_pages,
+             page_size, max_pages);
+  QP_REQUIRE((int64_t)max_pages * page_size <= INT32_MAX, QP_ERR_UNSUPPORTED, "%s: max_pages * page_size = %lld rows per sequence (at most 2^31 - 1)", who,
+             (long long)max_pages * page_size);
+  QP_REQUIRE(page_stride >= (int64_t)n_kv_heads * page_size * 128 && page_stride % 8 == 0, QP_ERR_INVALID,
+             "%s: page_stride=%lld elements (at least n_kv_heads * page_size * 128, a multiple of 8)", who, (long long)page_stride);
+  QP_REQUIRE(aligned16(k_pages) && aligned16(v_pages), QP_ERR_INVALID, "%s: pages must be 16-byte aligned", who);
+  return QP_OK;
+}
+int check_batch(const char* who, int batch, int t_max, int n_q_heads, int n_kv_heads, int head_dim) {
+  QP_REQUIRE(head_dim == 128, QP_ERR_UNSUPPORTED, "%s: head_dim=%d (only 128)", who, head_dim);
+  QP_REQUIRE(batch >= 1 && t_max >= 1, QP_ERR_INVALID, "%s: batch=%d, t_max=%d must be >= 1", who, batch, t_max);
+  QP_REQUIRE((int64_t)batch * t_max <= 65536, QP_ERR_UNSUPPORTED, "%s: batch * t_max = %lld rows (at most 65536 a call)", who, (long long)batch * t_max);
+  QP_REQUIRE(n_q_heads > 0 && n_kv_heads > 0 && n_q_heads % n_kv_heads == 0, QP_ERR_INVALID, "%s: n_q_heads=%d not a multiple of n_kv_heads=%d", who,
+             n_q_heads, n_kv_heads);
+  QP_REQUIRE(n_q_heads <= 1024, QP_ERR_UNSUPPORTED, "%s: n_q_heads=%d (at most 1024)", who, n_q_heads);
+  return QP_OK;
+}
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const char *x = (const char*)a, *y = (const char*)b;
+  return x < y + nb && y < x + na;
+}
+}  // namespace
+
+int qp_batch_rope_append(qp_ctx* ctx, const void* qkv, const void* cos, const void* sin, int batch, int t_max, const int32_t* seq_len,
+                         const int32_t* n_new, int n_q_heads, int n_kv_heads, int head_dim, void* q_out, void* k_pages, void* v_pages,
+                         int64_t page_stride, int n_pages, int page_size, const int32_t* page_table, int max_pages, void* stream) {
+  const char* who = "qp_batch_rope_append";
+  QP_REQUIRE(ctx && qkv && cos && sin && seq_len && q_out && k_pages && v_pages && page_table, QP_ERR_INVALID, "%s: NULL argument", who);
+  int rc = check_batch(who, batch, t_max, n_q_heads, n_kv_heads, head_dim);
+  if (rc) return rc;
+  if ((rc = check_pages(who, page_stride, n_pages, page_size, max_pages, n_kv_heads, k_pages, v_pages))) return rc;
+  QP_REQUIRE(aligned16(qkv) && aligned16(cos) && aligned16(sin) && aligned16(q_out), QP_ERR_INVALID, "%s: alignment", who);
+  const size_t rows = (size_t)batch * t_max;
+  QP_REQUIRE(!overlap(qkv, rows * (n_q_heads + 2 * n_kv_heads) * 256, q_out, rows * n_q_heads * 256), QP_ERR_INVALID, "%s: q_out overlaps qkv", who);
+  DeviceScope dev(ctx->device);
+  return qp_launch_batch_rope_append(qkv, cos, sin, batch, t_max, seq_len, n_new, n_q_heads, n_kv_heads, q_out, k_pages, v_pages, page_stride, n_pages,
+                                     page_size, page_table, max_pages, (hipStream_t)stream);
+}
+
+size_t qp_batch_attn_workspace_bytes(const qp_ctx* ctx, int batch, int t_max, int64_t prefix_len, int64_t suffix_capacity, int n_q_heads, int n_kv_heads) {
+  if (!ctx || batch < 1 || t_max < 1 || prefix_len < 0 || suffix_capacity < 1 || n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads ||
+      (int64_t)batch * t_max > 65536 || n_q_heads > 1024)
+    return 0;
+  return qp_batch_attn_workspace_bytes_impl(ctx, batch, t_max, prefix_len, suffix_capacity, n_q_heads, n_kv_heads);
+}
+
+int qp_batch_attn(qp_ctx* ctx, const void* q, const void* k_prefix, const void* v_prefix, int64_t prefix_head_stride, int64_t prefix_len,
+                  const void* k_pages, const void* v_pages, int64_t page_stride, int n_pages, int page_size, const int32_t* page_table, int max_pages,
+                  const int32_t* seq_len, const int32_t* n_new, int batch, int t_max, int n_q_heads, int n_kv_heads, int head_dim, float scale, void* out,
+                  void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "qp_batch_attn";
+  QP_REQUIRE(ctx && q && k_pages && v_pages && page_table && seq_len && out && workspace, QP_ERR_INVALID, "%s: NULL argument", who);
+  int rc = check_batch(who, batch, t_max, n_q_heads, n_kv_heads, head_dim);
+  if (rc) return rc;
+  if ((rc = check_pages(who, page_stride, n_pages, page_size, max_pages, n_kv_heads, k_pages, v_pages))) return rc;
+  QP_REQUIRE(prefix_len >= 0, QP_ERR_INVALID, "%s: prefix_len=%lld", who, (long long)prefix_len);
+  QP_REQUIRE(prefix_len == 0 || (k_prefix && v_prefix), QP_ERR_INVALID, "%s: prefix_len=%lld without prefix tensors", who, (long long)prefix_len);
+  QP_REQUIRE(prefix_len == 0 || (prefix_head_stride % 8 == 0 && prefix_head_stride / 128 >= prefix_len), QP_ERR_INVALID,
+             "%s: prefix_head_stride=%lld elements for %lld rows (a multiple of 8)", who, (long long)prefix_head_stride, (long long)prefix_len);
+  QP_REQUIRE(prefix_len <= INT32_MAX, QP_ERR_UNSUPPORTED, "%s: prefix_len=%lld (at most 2^31 - 1)", who, (long long)prefix_len);
+  QP_REQUIRE(scale > 0.f && scale <= 3.0e38f, QP_ERR_INVALID, "%s: scale=%g must be positive and finite", who, (double)scale);
+  QP_REQUIRE(aligned16(q) && aligned16(k_prefix) && aligned16(v_prefix) && aligned16(out) && aligned16(workspace), QP_ERR_INVALID, "%s: alignment", who);
+  const size_t need = qp_batch_attn_workspace_bytes_impl(ctx, batch, t_max, prefix_len, (int64_t)max_pages * page_size, n_q_heads, n_kv_heads);
+  if (workspace_bytes < need) return qp_fail(QP_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", who, workspace_bytes, need);
+  DeviceScope dev(ctx->device);
+  return qp_launch_batch_attn(ctx, q, k_prefix, v_prefix, prefix_head_stride, prefix_len, k_pages, v_pages, page_stride, n_pages, page_size, page_table,
+                              max_pages, seq_len, n_new, batch, t_max, n_q_heads, n_kv_heads, scale, out, workspace, (hipStream_t)stream);
+}
+
+size_t qp_verify_drafts_workspace_bytes(int batch, int t_max, int64_t vocab) {
+  if (batch < 1 || batch > 65535 || t_max < 0 || t_max > qp_verify_max_drafts() || vocab < 1 || vocab > qp_verify_max_vocab()) return 0;
+  return qp_verify_workspace_bytes_impl(batch, t_max, vocab);
+}
+
+int qp_verify_drafts(qp_ctx* ctx, const void* logits, int logits_f32, int64_t logits_seq_stride, int64_t logits_row_stride, const int64_t* drafts,
+                     const int32_t* n_draft, const float* draft_probs, int64_t probs_seq_stride, int64_t probs_row_stride, const float* uniforms,
+                     int batch, int t_max, int64_t vocab, float temperature, int32_t* n_accepted, int64_t* tokens, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  const char* who = "qp_verify_drafts";
+  QP_REQUIRE(ctx && logits && n_accepted && tokens && workspace, QP_ERR_INVALID, "%s: NULL argument", who);
+  QP_REQUIRE(batch >= 1 && batch <= 65535, QP_ERR_INVALID, "%s: batch=%d (1 ... 65535)", who, batch);
+  QP_REQUIRE(t_max >= 0 && t_max <= qp_verify_max_drafts(), QP_ERR_UNSUPPORTED, "%s: t_max=%d drafts (0 ... %d)", who, t_max, qp_verify_max_drafts());
+  QP_REQUIRE(t_max == 0 || drafts, QP_ERR_INVALID, "%s: drafts is NULL", who);
+  QP_REQUIRE(vocab >= 1 && vocab <= qp_verify_max_vocab(), QP_ERR_UNSUPPORTED, "%s: vocab=%lld (1 ... %lld)", who, (long long)vocab,
+             (long long)qp_verify_max_vocab());
+  QP_REQUIRE(temperature >= 0.f && temperature <= 3.0e38f, QP_ERR_INVALID, "%s: temperature=%g must be >= 0 and finite", who, (double)temperature);
+  QP_REQUIRE(temperature == 0.f || uniforms, QP_ERR_INVALID, "%s: temperature=%g needs the random numbers", who, (double)temperature);
+  QP_REQUIRE((t_max == 0 || logits_row_stride >= vocab) && (batch == 1 || logits_seq_stride >= vocab), QP_ERR_INVALID,
+             "%s: logits strides %lld / %lld below vocab=%lld", who, (long long)logits_seq_stride, (long long)logits_row_stride, (long long)vocab);
+  QP_REQUIRE(!draft_probs || ((t_max <= 1 || probs_row_stride >= vocab) && (batch == 1 || t_max == 0 || probs_seq_stride >= vocab)), QP_ERR_INVALID,
+             "%s: draft_probs strides %lld / %lld below vocab=%lld", who, (long long)probs_seq_stride, (long long)probs_row_stride, (long long)vocab);
+  QP_REQUIRE(((uintptr_t)logits & (logits_f32 ? 3u : 1u)) == 0 && ((uintptr_t)draft_probs & 3u) == 0 && ((uintptr_t)workspace & 7u) == 0, QP_ERR_INVALID,
+             "%s: alignment", who);
+  const size_t need = qp_verify_workspace_bytes_impl(batch, t_max, vocab);
+  if (workspace_bytes < need) return qp_fail(QP_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", who, workspace_bytes, need);
+  DeviceScope dev(ctx->device);
+  return qp_launch_verify_drafts(logits, logits_f32, logits_seq_stride, logits_row_stride, drafts, n_draft, draft_probs, probs_seq_stride,
+                                 probs_row_stride, uniforms, batch, t_max, vocab, temperature, n_accepted, tokens, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"

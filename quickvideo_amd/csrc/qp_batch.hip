@@ -1,0 +1,479 @@
+// Decoding a BATCH of sequences over one prefilled video (beams, sampled answers, several questions, drafted tokens).  All sequences
+// share the video's keys (the layer's arena, contiguous, frozen); what a sequence adds - its question, its generated tokens - lives in
+// pages of its own: pages [n_pages][n_kv][page_size][128], page_table int32 [batch][max_pages], key row j of sequence b = slot j % page_size
+// of page page_table[b][j / page_size].  seq_len[b] = rows stored before this step, n_new[b] <= t_max = rows of this step; both are read on
+// the device, so a captured step replays with new lengths.  A page number outside [0, n_pages) is never followed.
+//
+//   batch_rope_append_kernel   rotates the step's q and k rows and stores k / v into the pages
+//   batch_attn_kernel          attention of (batch x t_max) query rows over (shared prefix, own pages): partial results per key range
+//   batch_combine_kernel       joins the partial results of a row
+#include "qp_attn.h"
+
+namespace {
+
+using qpattn::lds_read_b128;
+using qpattn::lds_read_tr16;
+using qpattn::s16x8_t;
+using qpattn::xhalf_max;
+using qpattn::xhalf_sum;
+
+struct Pages {
+  const int* table;               // [batch][max_pages]
+  const int* seq_len;             // [batch]
+  const int* n_new;               // [batch] or NULL (= t_max for all)
+  int max_pages, n_pages, page_size;
+  int64_t page_stride16;          // uint4 between consecutive pages
+};
+
+__device__ __forceinline__ int rows_new(const Pages& p, int b, int t_max) {
+  if (!p.n_new) return t_max;
+  const int n = p.n_new[b];
+  return n < 0 ? 0 : (n > t_max ? t_max : n);
+}
+// uint4 offset of key row j of sequence b, kv head h; -1 when the row has no page
+__device__ __forceinline__ int64_t page_row16(const Pages& p, int b, int h, int64_t j) {
+  if (j < 0 || j >= (int64_t)p.max_pages * p.page_size) return -1;
+  const unsigned pi = (unsigned)j / (unsigned)p.page_size, slot = (unsigned)j - pi * (unsigned)p.page_size;
+  const int page = p.table[(int64_t)b * p.max_pages + pi];
+  if ((unsigned)page >= (unsigned)p.n_pages) return -1;
+  return (int64_t)page * p.page_stride16 + ((int64_t)h * p.page_size + slot) * 16;
+}
+
+// y[d] = x[d] cos[d] - x[d + 64] sin[d],  y[d + 64] = x[d + 64] cos[d] + x[d] sin[d],  d < 64.
+// 16 lanes per head row (16 B each), the partner half comes from lane ^ 8.  A product of two bf16 is exact in fp32, so each output is
+// two exact products, one fp32 sum and ONE rounding to bf16 (qp_rope_append rounds after every step because the reference's bf16 tensors
+// do; a page's keys are never compared bit for bit with the reference's, and the nearer value costs nothing).
+// Bytes bound: every row of qkv is read once and written once.
+__global__ __launch_bounds__(256) void batch_rope_append_kernel(const uint4* __restrict__ qkv, const uint4* __restrict__ cos_t,
+                                                                const uint4* __restrict__ sin_t, Pages pg, int t_max, int hq, int hkv,
+                                                                int head_blocks, uint4* __restrict__ q_out, uint4* __restrict__ k_pages,
+                                                                uint4* __restrict__ v_pages) {
+  const int c = threadIdx.x & 15;
+  const int64_t row = blockIdx.x / head_blocks;                // b * t_max + t (uniform)
+  const int hr = (int)(blockIdx.x % head_blocks) * 16 + (threadIdx.x >> 4);
+  const int b = (int)(row / t_max), t = (int)(row % t_max);
+  if (t >= rows_new(pg, b, t_max)) return;
+  const int heads = hq + 2 * hkv;
+  if (hr >= heads) return;                                     // whole 16-lane groups
+  const uint4 x = qkv[(row * heads + hr) * 16 + c];
+  const int64_t j = (int64_t)pg.seq_len[b] + t;
+  if (hr >= hq + hkv) {
+    const int64_t at = page_row16(pg, b, hr - hq - hkv, j);
+    if (at >= 0) v_pages[at + c] = x;
+    return;
+  }
+  const uint4 ct = cos_t[row * 8 + (c & 7)], st = sin_t[row * 8 + (c & 7)];
+  uint4 p;
+  p.x = __shfl_xor((int)x.x, 8, 16); p.y = __shfl_xor((int)x.y, 8, 16);
+  p.z = __shfl_xor((int)x.z, 8, 16); p.w = __shfl_xor((int)x.w, 8, 16);
+  const float sign = (c < 8) ? -1.f : 1.f;
+  const unsigned xw[4] = {x.x, x.y, x.z, x.w}, pw[4] = {p.x, p.y, p.z, p.w}, cw[4] = {ct.x, ct.y, ct.z, ct.w}, sw[4] = {st.x, st.y, st.z, st.w};
+  unsigned o[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float lo = __uint_as_float(xw[w] << 16) * __uint_as_float(cw[w] << 16) + (sign * __uint_as_float(pw[w] << 16)) * __uint_as_float(sw[w] << 16);
+    const float hi = __uint_as_float(xw[w] & 0xffff0000u) * __uint_as_float(cw[w] & 0xffff0000u) +
+                     (sign * __uint_as_float(pw[w] & 0xffff0000u)) * __uint_as_float(sw[w] & 0xffff0000u);
+    o[w] = (unsigned)f32_to_bf16_bits(lo) | ((unsigned)f32_to_bf16_bits(hi) << 16);
+  }
+  const uint4 y = make_uint4(o[0], o[1], o[2], o[3]);
+  if (hr < hq) {
+    q_out[(row * hq + hr) * 16 + c] = y;
+  } else {
+    const int64_t at = page_row16(pg, b, hr - hq, j);
+    if (at >= 0) k_pages[at + c] = y;
+  }
+}
+
+// ---- attention ------------------------------------------------------------------------------------------------------------------------
+// Query rows of kv head h: r = (b * t_max + t) * G + g, g < G = hq / hkv, R = batch * t_max * G of them.  All R rows attend every prefix key, so
+// the prefix is ONE R-row problem per kv head and is read once for the batch; the pages of a sequence are attended by its own t_max * G rows,
+// row (t, g) seeing keys j <= seq_len + t.  Both kinds of work are cut into key ranges; every range leaves (max, sum, o[128]) per row, in
+// 32 bits, and batch_combine_kernel joins them:  out = sum_p 2^((m_p - M) c) o_p / sum_p 2^((m_p - M) c) l_p,  c = scale * log2(e).
+struct BatchAttnParams {
+  const uint4* q; uint16_t* out;
+  const uint4* k_pre; const uint4* v_pre; int64_t pre_hs16; int64_t P;
+  const uint4* k_pages; const uint4* v_pages;
+  Pages pg;
+  int t_max, hq, hkv, G; float c;
+  int64_t R;
+  int ns, nrb;                    // prefix: key ranges, row blocks (per kv head)
+  int ns2, nrb2;                  // pages: key ranges, row blocks (per sequence and kv head)
+  int64_t prefix_wgs;             // hkv * nrb * ns
+  float* part_o; float2* part_ml; // [hkv][ns + ns2][R] rows of 128 floats / (max, sum)
+};
+
+constexpr int kTile = 64;         // keys per tile
+
+// bf16 words whose exponent is all ones (infinities, NaN) set to zero; *any = there was one
+__device__ __forceinline__ unsigned finite_word(unsigned w, bool* any) {
+  if ((w & 0x7f80u) == 0x7f80u) { *any = true; w &= 0xffff0000u; }
+  if ((w & 0x7f800000u) == 0x7f800000u) { *any = true; w &= 0x0000ffffu; }
+  return w;
+}
+
+// A workgroup of WR x WK waves takes a block of 32 * WR rows over one key range, kTile keys at a time: the tile goes through registers into LDS
+// (K row-major with XOR-swizzled 16-B slots; V as [key / 4][d / 32][key % 4][32] for the transposing LDS reads), the next tile's loads are in
+// flight while this one is computed.  Wave (wr, wk) owns rows [32 wr, 32 wr + 32) and, for WK = 2, half of the tile's keys:
+// S^T = K.Q^T (rows are the columns of v_mfma_f32_32x32x16_bf16: a lane owns one row), online softmax, O^T += V^T.P, P rounded to bf16 for
+// the product (as in the prefill and decode kernels: its error averages out below the output's own rounding), everything else fp32.
+template <int WR, int WK, bool kPaged>
+__device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int kvh, int b, int64_t row0, int64_t row_end, int64_t k0, int64_t k1,
+                                                 int part, unsigned char* lds, float* lds_ml, unsigned long long* key_bits) {
+  constexpr int NT = 64 * WR * WK, PT = kTile * 16 / NT, KB = 2 / WK;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, l31 = lane & 31;
+  const int wr = wave % WR, wk = wave / WR;
+  const int64_t r = row0 + wr * 32 + l31;
+  const bool row_live = r < row_end;
+  const bool wave_live = row0 + wr * 32 < row_end;
+  unsigned char* kl = lds;
+  unsigned char* vl = lds + kTile * 256;
+  bf16x8_t qf[8];
+  int64_t limit = INT64_MAX;                                   // last visible key of this lane's row
+  int64_t seen_by_all = INT64_MAX;                             // keys below this are visible to every row of the sequence
+  {
+    const int64_t rr = row_live ? r : row0;
+    const int64_t bt = rr / p.G;
+    const int g = (int)(rr - bt * p.G);
+    const uint4* src = p.q + ((bt * p.hq) + (int64_t)kvh * p.G + g) * 16;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (row_live) x = src[kk * 2 + hi];
+      qf[kk] = __builtin_bit_cast(bf16x8_t, x);
+    }
+    if (kPaged) {
+      seen_by_all = (int64_t)p.pg.seq_len[b] + 1;
+      limit = (int64_t)p.pg.seq_len[b] + (bt - (int64_t)b * p.t_max);
+    }
+  }
+  const uint4* kbase = kPaged ? p.k_pages : p.k_pre + (int64_t)kvh * p.pre_hs16;
+  const uint4* vbase = kPaged ? p.v_pages : p.v_pre + (int64_t)kvh * p.pre_hs16;
+  const int slot16 = tid & 15, srow = tid >> 4;                // this thread stages rows srow + i * (NT / 16), 16-B slot slot16
+  uint4 kx[PT], vx[PT];
+  unsigned holes = 0;                                          // bit i: staged row i has no page
+  auto load = [&](int64_t t0) {
+    holes = 0;
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      const int64_t key = t0 + srow + i * (NT / 16);
+      kx[i] = vx[i] = make_uint4(0, 0, 0, 0);                  // rows past the end are zero: their probability is 0 and 0 * 0 stays 0
+      if (key < k1) {
+        int64_t at = key * 16;
+        if (kPaged) {
+          at = page_row16(p.pg, b, kvh, key);
+          if (at < 0) { holes |= 1u << i; continue; }
+        }
+        kx[i] = kbase[at + slot16]; vx[i] = vbase[at + slot16];
+      }
+    }
+  };
+  int koff[8];
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) koff[kk] = l31 * 256 + (((kk * 2 + hi) ^ (l31 & 15)) << 4);
+  const int voff = (((lane & 15) >> 2) << 6) + (((lane >> 4) & 1) << 5) + ((lane & 3) << 3) + (hi << 10);
+  f32x16_t o[4];
+#pragma unroll
+  for (int db = 0; db < 4; ++db) o[db] = (f32x16_t){0};
+  float m_run = -1e30f, l_run = 0.f;
+  if (kPaged && tid < 4) key_bits[tid] = 0;                    // [parity][0: rows without a page, 1: masked rows with a non-finite value]
+  int par = 0;
+  if (k0 < k1) load(k0);
+  for (int64_t t0 = k0; t0 < k1; t0 += kTile, par ^= 1) {
+    __syncthreads();                                           // everyone has read the previous tile
+    const bool masked = kPaged && t0 + kTile > seen_by_all;    // some row of the sequence does not see some key of this tile
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+      const int row = srow + i * (NT / 16);
+      if (kPaged) {
+        if ((holes >> i) & 1 && slot16 == 0) atomicOr(&key_bits[par * 2], 1ull << row);
+        if (masked && t0 + row >= seen_by_all) {               // 0 * infinity is NaN: a masked row's values must be finite in the product
+          bool any = false;
+          vx[i].x = finite_word(vx[i].x, &any); vx[i].y = finite_word(vx[i].y, &any);
+          vx[i].z = finite_word(vx[i].z, &any); vx[i].w = finite_word(vx[i].w, &any);
+          if (any) atomicOr(&key_bits[par * 2 + 1], 1ull << row);
+        }
+      }
+      *reinterpret_cast<uint4*>(kl + row * 256 + ((slot16 ^ (row & 15)) << 4)) = kx[i];
+      *reinterpret_cast<uint4*>(vl + (((row >> 2) * 4 + (slot16 >> 2)) << 8) + ((row & 3) << 6) + ((slot16 & 3) << 4)) = vx[i];
+    }
+    __syncthreads();
+    unsigned long long hole_bits = 0, odd_bits = 0;
+    if (kPaged) {
+      hole_bits = key_bits[par * 2]; odd_bits = key_bits[par * 2 + 1];
+      if (tid < 2) key_bits[(par ^ 1) * 2 + tid] = 0;          // last read before the barrier above, next written behind the next one
+    }
+    if (t0 + kTile < k1) load(t0 + kTile);
+    if (!wave_live) continue;
+    f32x16_t s[KB];
+#pragma unroll
+    for (int k = 0; k < KB; ++k) {
+      const int kb = WK == 2 ? wk : k;
+      s[k] = (f32x16_t){0};
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)
+        s[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_read_b128(kl, kb * 32 * 256 + koff[kk]), qf[kk], s[k], 0, 0, 0);
+    }
+    if (t0 + kTile > k1 || masked || hole_bits) {
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        const int kb = WK == 2 ? wk : k;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int row = kb * 32 + (e & 3) + 8 * (e >> 2) + 4 * hi;
+          const int64_t key = t0 + row;
+          s[k][e] = (key < k1 && key <= limit && !((hole_bits >> row) & 1)) ? s[k][e] : -INFINITY;
+        }
+      }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[k][e]);
+    mx = xhalf_max(mx);
+    if (!__all((mx - m_run) * p.c <= 8.0f)) {                  // the reference moves only when a row outgrows it by 2^8
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * p.c);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
+    }
+    const float mc = m_run * p.c;
+    float rs = 0.f;
+#pragma unroll
+    for (int k = 0; k < KB; ++k) {
+      const int kb = WK == 2 ? wk : k;
+      bf16x8_t pf[2];
+#pragma unroll
+      for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][cc * 8 + e], p.c, -mc));
+          rs += pe;
+          pf[cc][e] = (__bf16)pe;
+        }
+#pragma unroll
+      for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+        for (int db = 0; db < 4; ++db) {
+          const int off = voff + (((kb * 8 + cc * 4) * 4 + db) << 8);
+          const s16x4_t v0 = lds_read_tr16(vl, off);
+          const s16x4_t v1 = lds_read_tr16(vl, off + (2 * 4 << 8));
+          const s16x8_t av = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), pf[cc], o[db], 0, 0, 0);
+        }
+      if (kPaged && odd_bits) {                                // rare: give the rows that DO see such a key its infinities / NaN back
+#pragma unroll 1
+        for (int row = 0; row < 32; ++row) {
+          const int trow = kb * 32 + row;
+          if (!((odd_bits >> trow) & 1)) continue;
+          const int64_t key = t0 + trow;
+          const int64_t at = page_row16(p.pg, b, kvh, key);
+          if (at < 0) continue;
+          const uint16_t* vrow = reinterpret_cast<const uint16_t*>(vbase + at);
+          const int e_of = (row & 3) + 4 * (row >> 3), h_of = (row >> 2) & 1;
+          float pv = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pv = e == e_of ? (float)pf[e >> 3][e & 7] : pv;
+          pv = __shfl(pv, l31 + 32 * h_of, 64);
+          if (key <= limit) {
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const uint16_t w = vrow[db * 32 + 8 * (e >> 2) + 4 * hi + (e & 3)];
+                if ((w & 0x7f80u) == 0x7f80u) o[db][e] += pv * bf16_bits_to_f32(w);
+              }
+          }
+        }
+      }
+    }
+    l_run += xhalf_sum(rs);
+  }
+  if (WK == 2) {                                               // join the two key halves of a row (the tile's LDS is free)
+    __syncthreads();
+    float* obuf = reinterpret_cast<float*>(lds);               // [WR][32 rows][128]
+    if (wk == 1) {
+      if (hi == 0) { lds_ml[(wr * 32 + l31) * 2] = m_run; lds_ml[(wr * 32 + l31) * 2 + 1] = l_run; }
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4)
+          *reinterpret_cast<float4*>(obuf + (wr * 32 + l31) * 128 + db * 32 + 8 * q4 + 4 * hi) =
+              make_float4(o[db][q4 * 4 + 0], o[db][q4 * 4 + 1], o[db][q4 * 4 + 2], o[db][q4 * 4 + 3]);
+    }
+    __syncthreads();
+    if (wk == 1) return;
+    const float m1 = lds_ml[(wr * 32 + l31) * 2], l1 = lds_ml[(wr * 32 + l31) * 2 + 1];
+    const float m = fmaxf(m_run, m1);
+    const float a0 = __builtin_amdgcn_exp2f((m_run - m) * p.c), a1 = __builtin_amdgcn_exp2f((m1 - m) * p.c);
+    m_run = m;
+    l_run = l_run * a0 + l1 * a1;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[db][e] = o[db][e] * a0 + obuf[(wr * 32 + l31) * 128 + db * 32 + 8 * (e >> 2) + 4 * hi + (e & 3)] * a1;
+  }
+  if (!row_live) return;
+  const int64_t slot = ((int64_t)kvh * (p.ns + p.ns2) + part) * p.R + r;
+  if (hi == 0) p.part_ml[slot] = make_float2(m_run, l_run);
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4)
+      *reinterpret_cast<float4*>(p.part_o + slot * 128 + db * 32 + 8 * q4 + 4 * hi) =
+          make_float4(o[db][q4 * 4 + 0], o[db][q4 * 4 + 1], o[db][q4 * 4 + 2], o[db][q4 * 4 + 3]);
+}
+
+template <int WR, int WK>
+__global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnParams p) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kTile * 256];
+  __shared__ float lds_ml[WR * 64];
+  __shared__ unsigned long long key_bits[4];
+  int64_t w = blockIdx.x;
+  if (w < p.prefix_wgs) {
+    const int rb = (int)(w % p.nrb), split = (int)((w / p.nrb) % p.ns), kvh = (int)(w / ((int64_t)p.nrb * p.ns));
+    int64_t chunk = (p.P + p.ns - 1) / p.ns;
+    chunk = (chunk + kTile - 1) / kTile * kTile;
+    const int64_t k0 = (int64_t)split * chunk, k1 = k0 + chunk < p.P ? k0 + chunk : p.P;
+    batch_attn_range<WR, WK, false>(p, kvh, 0, (int64_t)rb * 32 * WR, p.R, k0, k1, split, lds, lds_ml, key_bits);
+    return;
+  }
+  w -= p.prefix_wgs;
+  const int rb = (int)(w % p.nrb2), split = (int)((w / p.nrb2) % p.ns2);
+  const int64_t hb = w / ((int64_t)p.nrb2 * p.ns2);
+  const int kvh = (int)(hb % p.hkv), b = (int)(hb / p.hkv);
+  const int n_new = rows_new(p.pg, b, p.t_max);
+  if (n_new == 0) return;                                      // nothing of this sequence is written
+  int64_t len = (int64_t)p.pg.seq_len[b] + n_new;
+  if (len > (int64_t)p.pg.max_pages * p.pg.page_size) len = (int64_t)p.pg.max_pages * p.pg.page_size;
+  if (len < 0) len = 0;
+  int64_t chunk = (len + p.ns2 - 1) / p.ns2;
+  chunk = (chunk + kTile - 1) / kTile * kTile;
+  const int64_t k0 = (int64_t)split * chunk, k1 = k0 + chunk < len ? k0 + chunk : len;
+  const int64_t seq_row0 = (int64_t)b * p.t_max * p.G, row0 = seq_row0 + (int64_t)rb * 32 * WR, row_end = seq_row0 + (int64_t)n_new * p.G;
+  if (row0 >= row_end) return;
+  batch_attn_range<WR, WK, true>(p, kvh, b, row0, row_end, k0, k1, p.ns + split, lds, lds_ml, key_bits);
+}
+
+// one workgroup per row: 8 groups of 32 lanes walk the partial results (16 B per lane), then join through LDS
+__global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
+  __shared__ float4 lds_o[8][32];
+  __shared__ float red[8];
+  const int kvh = blockIdx.x % p.hkv;
+  const int64_t r = blockIdx.x / p.hkv, bt = r / p.G;
+  const int g = (int)(r - bt * p.G), b = (int)(bt / p.t_max), t = (int)(bt % p.t_max);
+  if (t >= rows_new(p.pg, b, p.t_max)) return;                 // rows behind a sequence's last token stay as they are
+  const int np = p.ns + p.ns2, tid = threadIdx.x, lane32 = tid & 31, grp = tid >> 5;
+  const float2* ml = p.part_ml + (int64_t)kvh * np * p.R + r;
+  const float* po = p.part_o + ((int64_t)kvh * np * p.R + r) * 128;
+  float M = -1e30f;
+  for (int i = tid; i < np; i += 256) M = fmaxf(M, ml[(int64_t)i * p.R].x);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+  if ((tid & 63) == 0) red[tid >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  __syncthreads();
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  for (int i = grp; i < np; i += 8) {
+    const float2 x = ml[(int64_t)i * p.R];
+    if (x.y == 0.f) continue;                                  // an empty range left no o behind
+    const float a = __builtin_amdgcn_exp2f((x.x - M) * p.c);
+    const float4 v = *reinterpret_cast<const float4*>(po + (int64_t)i * p.R * 128 + lane32 * 4);
+    l = __builtin_fmaf(x.y, a, l);
+    acc.x = __builtin_fmaf(v.x, a, acc.x); acc.y = __builtin_fmaf(v.y, a, acc.y);
+    acc.z = __builtin_fmaf(v.z, a, acc.z); acc.w = __builtin_fmaf(v.w, a, acc.w);
+  }
+  lds_o[grp][lane32] = acc;
+  if (lane32 == 0) red[grp] = l;
+  __syncthreads();
+  if (grp) return;
+  l = ((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]));
+#pragma unroll
+  for (int k = 1; k < 8; ++k) {
+    const float4 v = lds_o[k][lane32];
+    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+  }
+  uint2 y = make_uint2(0, 0);                                  // a row that sees no key is zero
+  if (l != 0.f) {
+    const float inv = 1.0f / l;
+    y.x = (unsigned)f32_to_bf16_bits(acc.x * inv) | ((unsigned)f32_to_bf16_bits(acc.y * inv) << 16);
+    y.y = (unsigned)f32_to_bf16_bits(acc.z * inv) | ((unsigned)f32_to_bf16_bits(acc.w * inv) << 16);
+  }
+  *reinterpret_cast<uint2*>(p.out + ((bt * p.hq) + (int64_t)kvh * p.G + g) * 128 + lane32 * 4) = y;
+}
+
+struct Plan { int ns, nrb, ns2, nrb2; int64_t R; };
+
+Plan make_plan(const qp_ctx* ctx, int batch, int t_max, int64_t P, int64_t suffix_cap, int hq, int hkv) {
+  Plan pl;
+  const int G = hq / hkv, rows = 32;
+  pl.R = (int64_t)batch * t_max * G;
+  pl.nrb = (int)((pl.R + rows - 1) / rows);
+  pl.nrb2 = (int)(((int64_t)t_max * G + rows - 1) / rows);
+  const int64_t want = 4LL * ctx->cus;
+  int64_t ns = (want + (int64_t)hkv * pl.nrb - 1) / ((int64_t)hkv * pl.nrb);
+  const int64_t most = (P + 127) / 128;
+  pl.ns = (int)(ns < most ? ns : most);
+  int64_t ns2 = want / ((int64_t)hkv * batch * pl.nrb2);
+  const int64_t most2 = (suffix_cap + 255) / 256;
+  if (ns2 > most2) ns2 = most2;
+  pl.ns2 = (int)(ns2 < 1 ? 1 : (ns2 > 64 ? 64 : ns2));
+  return pl;
+}
+
+size_t ml_bytes(const Plan& pl, int hkv) { return ((size_t)hkv * (pl.ns + pl.ns2) * pl.R * sizeof(float2) + 15) & ~(size_t)15; }
+
+Pages pages_of(const int32_t* table, const int32_t* seq_len, const int32_t* n_new, int max_pages, int n_pages, int page_size, int64_t page_stride) {
+  Pages pg;
+  pg.table = table; pg.seq_len = seq_len; pg.n_new = n_new;
+  pg.max_pages = max_pages; pg.n_pages = n_pages; pg.page_size = page_size; pg.page_stride16 = page_stride / 8;
+  return pg;
+}
+
+}  // namespace
+
+int qp_launch_batch_rope_append(const void* qkv, const void* cos, const void* sin, int batch, int t_max, const int32_t* seq_len, const int32_t* n_new,
+                                int hq, int hkv, void* q_out, void* k_pages, void* v_pages, int64_t page_stride, int n_pages, int page_size,
+                                const int32_t* table, int max_pages, hipStream_t s) {
+  const int head_blocks = (hq + 2 * hkv + 15) / 16;
+  const int64_t grid = (int64_t)batch * t_max * head_blocks;
+  batch_rope_append_kernel<<<(unsigned)grid, 256, 0, s>>>((const uint4*)qkv, (const uint4*)cos, (const uint4*)sin,
+                                                          pages_of(table, seq_len, n_new, max_pages, n_pages, page_size, page_stride), t_max, hq, hkv,
+                                                          head_blocks, (uint4*)q_out, (uint4*)k_pages, (uint4*)v_pages);
+  return qp_check_launch("batch_rope_append");
+}
+
+size_t qp_batch_attn_workspace_bytes_impl(const qp_ctx* ctx, int batch, int t_max, int64_t P, int64_t suffix_cap, int hq, int hkv) {
+  const Plan pl = make_plan(ctx, batch, t_max, P, suffix_cap, hq, hkv);
+  return ml_bytes(pl, hkv) + (size_t)hkv * (pl.ns + pl.ns2) * pl.R * 128 * sizeof(float);
+}
+
+int qp_launch_batch_attn(const qp_ctx* ctx, const void* q, const void* k_prefix, const void* v_prefix, int64_t prefix_head_stride, int64_t P,
+                         const void* k_pages, const void* v_pages, int64_t page_stride, int n_pages, int page_size, const int32_t* table, int max_pages,
+                         const int32_t* seq_len, const int32_t* n_new, int batch, int t_max, int hq, int hkv, float scale, void* out, void* workspace,
+                         hipStream_t s) {
+  const Plan pl = make_plan(ctx, batch, t_max, P, (int64_t)max_pages * page_size, hq, hkv);
+  BatchAttnParams p;
+  p.q = (const uint4*)q; p.out = (uint16_t*)out;
+  p.k_pre = (const uint4*)k_prefix; p.v_pre = (const uint4*)v_prefix; p.pre_hs16 = prefix_head_stride / 8; p.P = P;
+  p.k_pages = (const uint4*)k_pages; p.v_pages = (const uint4*)v_pages;
+  p.pg = pages_of(table, seq_len, n_new, max_pages, n_pages, page_size, page_stride);
+  p.t_max = t_max; p.hq = hq; p.hkv = hkv; p.G = hq / hkv; p.c = scale * 1.4426950408889634f;
+  p.R = pl.R; p.ns = pl.ns; p.nrb = pl.nrb; p.ns2 = pl.ns2; p.nrb2 = pl.nrb2;
+  p.prefix_wgs = (int64_t)hkv * pl.nrb * pl.ns;
+  p.part_ml = (float2*)workspace;
+  p.part_o = (float*)((char*)workspace + ml_bytes(pl, hkv));
+  const int64_t grid = p.prefix_wgs + (int64_t)hkv * batch * pl.nrb2 * pl.ns2;
+  batch_attn_kernel<1, 2><<<(unsigned)grid, 128, 0, s>>>(p);
+  int rc = qp_check_launch("batch_attn");
+  if (rc) return rc;
+  batch_combine_kernel<<<(unsigned)(pl.R * hkv), 256, 0, s>>>(p);
+  return qp_check_launch("batch_attn(combine)");
+}

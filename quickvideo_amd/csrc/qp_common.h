@@ -133,6 +133,20 @@ int qp_launch_decode_attn_fused(const qp_ctx* ctx, const void* qkv, const void* 
                                 int64_t head_stride, const int64_t* state, int hq, int hkv, float scale, void* out, void* workspace,
                                 hipStream_t s);
 int qp_launch_decode_advance(int64_t* state, int n, hipStream_t s);
+int qp_launch_batch_rope_append(const void* qkv, const void* cos, const void* sin, int batch, int t_max, const int32_t* seq_len, const int32_t* n_new,
+                                int hq, int hkv, void* q_out, void* k_pages, void* v_pages, int64_t page_stride, int n_pages, int page_size,
+                                const int32_t* table, int max_pages, hipStream_t s);
+size_t qp_batch_attn_workspace_bytes_impl(const qp_ctx* ctx, int batch, int t_max, int64_t P, int64_t suffix_cap, int hq, int hkv);
+int qp_launch_batch_attn(const qp_ctx* ctx, const void* q, const void* k_prefix, const void* v_prefix, int64_t prefix_head_stride, int64_t P,
+                         const void* k_pages, const void* v_pages, int64_t page_stride, int n_pages, int page_size, const int32_t* table, int max_pages,
+                         const int32_t* seq_len, const int32_t* n_new, int batch, int t_max, int hq, int hkv, float scale, void* out, void* workspace,
+                         hipStream_t s);
+int64_t qp_verify_max_vocab();
+int qp_verify_max_drafts();
+size_t qp_verify_workspace_bytes_impl(int batch, int t_max, int64_t vocab);
+int qp_launch_verify_drafts(const void* logits, int logits_f32, int64_t seq_stride, int64_t row_stride, const int64_t* drafts, const int32_t* n_draft,
+                            const float* probs, int64_t probs_seq_stride, int64_t probs_row_stride, const float* uniforms, int batch, int t_max,
+                            int64_t vocab, float temperature, int32_t* n_accepted, int64_t* tokens, void* workspace, hipStream_t s);
 int qp_launch_tail_keys(const void* rows, int64_t head_stride, int64_t row0, int64_t n, int hkv, uint16_t* norm_keys, int largest,
                         int* sync_words, int n_sync_words, hipStream_t s);
 int qp_prune_tail_inplace_capacity(int cus);

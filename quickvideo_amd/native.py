@@ -95,6 +95,12 @@ SIGNATURES = {
     "qp_decode_attn": (_i32, [_vp, _vp, _vp, _vp, _i64, _vp, _i32, _i32, _i32, _f32, _vp, _vp, _sz, _vp]),
     "qp_decode_attn_fused": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _f32, _vp, _vp, _sz, _vp]),
     "qp_decode_advance": (_i32, [_vp, _vp, _i64, _vp]),
+    "qp_batch_rope_append": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _i32, _vp]),
+    "qp_batch_attn_workspace_bytes": (_sz, [_vp, _i32, _i32, _i64, _i64, _i32, _i32]),
+    "qp_batch_attn": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _vp,
+                             _sz, _vp]),
+    "qp_verify_drafts_workspace_bytes": (_sz, [_i32, _i32, _i64]),
+    "qp_verify_drafts": (_i32, [_vp, _vp, _i32, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i32, _i32, _i64, _f32, _vp, _vp, _vp, _sz, _vp]),
     "qp_vit_rope": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp]),
     "qp_vit_attn": (_i32, [_vp, _vp, _i64, _i64, _i32, _i32, _f32, _vp, _vp]),
     "qp_vit_attn_varlen": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _i32, _f32, _vp, _vp]),
@@ -408,6 +414,109 @@ class QuickPrefillOps:
 
     def decode_advance(self, state):
         self._check(self.lib.qp_decode_advance(self.ctx, state.data_ptr(), state.numel(), self._stream()))
+
+    # -- a batch of sequences over one prefilled video (include/quickprefill.h; batch.py drives them)
+    def _on_device(self, t) -> bool:
+        return t.is_cuda and t.get_device() == (self.device.index or 0)
+
+    def _batch_check(self, name, t, dtype, shape=None, contiguous=True):
+        """The kernels take raw pointers: what torch knows about a tensor is checked here."""
+        if t.dtype != dtype:
+            raise ValueError(f"libquickprefill: {name} is {t.dtype}, {dtype} is needed")
+        if shape is not None and t.shape != shape:
+            raise ValueError(f"libquickprefill: {name} has shape {tuple(t.shape)}, {tuple(shape)} is needed")
+        if contiguous and not t.is_contiguous():
+            raise ValueError(f"libquickprefill: {name} must be contiguous")
+        if not self._on_device(t):
+            raise ValueError(f"libquickprefill: {name} is on {t.device}, the operators are on {self.device}")
+
+    def _batch_pages(self, k_pages, v_pages, table, seq_len, n_new, batch, n_kv, head_dim):
+        n_pages, ps = k_pages.shape[0], k_pages.shape[2]
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            self._batch_check(name, t, torch.bfloat16, (n_pages, n_kv, ps, head_dim), contiguous=False)
+            if not t[0].is_contiguous() or t.stride(0) != k_pages.stride(0):
+                raise ValueError(f"libquickprefill: {name}: a page must be contiguous, and both kinds equally far apart")
+        self._batch_check("page_table", table, torch.int32, (batch, table.shape[1]))
+        self._batch_check("seq_len", seq_len, torch.int32, (batch,))
+        if n_new is not None:
+            self._batch_check("n_new", n_new, torch.int32, (batch,))
+        return k_pages.stride(0), n_pages, ps
+
+    def _stream_here(self):
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def batch_rope_append(self, qkv, cos, sin, seq_len, n_new, table, k_pages, v_pages, n_q, n_kv, head_dim, q_out):
+        """qkv [B, T, (n_q + 2 n_kv) * D] -> q_out [B, T, n_q, D] rotated; rotated keys and values into the sequences' pages
+        [n_pages, n_kv, page_size, D] at rows seq_len[b] ...  cos / sin: bf16 [B, T, D/2] (or the [B * T, D/2] mrope_table returns).
+        seq_len int32 [B], n_new int32 [B] or None (T each), table int32 [B, max_pages]."""
+        B, T = qkv.shape[:2]
+        stride, n_pages, ps = self._batch_pages(k_pages, v_pages, table, seq_len, n_new, B, n_kv, head_dim)
+        self._batch_check("qkv", qkv, torch.bfloat16, (B, T, (n_q + 2 * n_kv) * head_dim))
+        self._batch_check("q_out", q_out, torch.bfloat16, (B, T, n_q, head_dim))
+        for name, t in (("cos", cos), ("sin", sin)):
+            self._batch_check(name, t, torch.bfloat16)
+            if t.numel() != B * T * head_dim // 2:
+                raise ValueError(f"libquickprefill: {name} has {t.numel()} values, {B} x {T} x {head_dim // 2} are needed")
+        self._check(self.lib.qp_batch_rope_append(self.ctx, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), B, T, seq_len.data_ptr(), _ptr(n_new), n_q, n_kv,
+                                                  head_dim, q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), stride, n_pages, ps, table.data_ptr(),
+                                                  table.shape[1], self._stream_here()))
+
+    def batch_attn_workspace(self, batch, t_max, prefix_len, suffix_capacity, n_q, n_kv):
+        """Scratch of batch_attn calls up to this size; one per stream (or captured graph) that may run at the same time."""
+        nbytes = int(self.lib.qp_batch_attn_workspace_bytes(self.ctx, batch, t_max, prefix_len, suffix_capacity, n_q, n_kv))
+        if nbytes == 0:
+            raise ValueError(f"libquickprefill: no batch of {batch} x {t_max} rows over {prefix_len} + {suffix_capacity} keys with {n_q} / {n_kv} heads")
+        return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+
+    def batch_attn(self, q, k_prefix, v_prefix, prefix_head_stride, prefix_len, k_pages, v_pages, table, seq_len, n_new, n_q, n_kv, head_dim, scale, out,
+                   workspace):
+        """q, out [B, T, n_q, D]: attention of every row over the shared prefix rows [0, prefix_len) (k_prefix / v_prefix as in prefill_attn, None
+        without a prefix) and its sequence's pages up to and including its own row."""
+        B, T = q.shape[:2]
+        stride, n_pages, ps = self._batch_pages(k_pages, v_pages, table, seq_len, n_new, B, n_kv, head_dim)
+        self._batch_check("q", q, torch.bfloat16, (B, T, n_q, head_dim))
+        self._batch_check("out", out, torch.bfloat16, (B, T, n_q, head_dim))
+        if prefix_len > 0:
+            for name, t in (("k_prefix", k_prefix), ("v_prefix", v_prefix)):
+                self._batch_check(name, t, torch.bfloat16, contiguous=False)
+                if (n_kv - 1) * prefix_head_stride + prefix_len * head_dim > t.untyped_storage().nbytes() // 2 - t.storage_offset():
+                    raise ValueError(f"libquickprefill: {name} holds fewer than {prefix_len} rows of {n_kv} heads {prefix_head_stride} elements apart")
+        self._batch_check("workspace", workspace, workspace.dtype)
+        self._check(self.lib.qp_batch_attn(self.ctx, q.data_ptr(), _ptr(k_prefix), _ptr(v_prefix), prefix_head_stride, prefix_len, k_pages.data_ptr(),
+                                           v_pages.data_ptr(), stride, n_pages, ps, table.data_ptr(), table.shape[1], seq_len.data_ptr(), _ptr(n_new), B, T,
+                                           n_q, n_kv, head_dim, float(scale), out.data_ptr(), workspace.data_ptr(),
+                                           workspace.numel() * workspace.element_size(), self._stream_here()))
+
+    def verify_drafts_workspace(self, batch, t_max, vocab):
+        nbytes = int(self.lib.qp_verify_drafts_workspace_bytes(batch, t_max, vocab))
+        if nbytes == 0:
+            raise ValueError(f"libquickprefill: no verification of {batch} x {t_max} drafts over {vocab} tokens")
+        return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+
+    def verify_drafts(self, logits, drafts, n_draft, draft_probs, uniforms, temperature, n_accepted, tokens, workspace):
+        """logits [B, T + 1, V] (bf16 or fp32, rows contiguous), drafts int64 [B, T], n_draft int32 [B] or None, draft_probs fp32 [B, T, V] or None,
+        uniforms fp32 [B, T + 1] (None when temperature is 0) -> n_accepted int32 [B], tokens int64 [B, T + 1]."""
+        B, T, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+        if logits.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"libquickprefill: logits are {logits.dtype}, torch.bfloat16 or torch.float32 is needed")
+        for name, t, shape in (("logits", logits, (B, T + 1, V)), ("draft_probs", draft_probs, (B, T, V))):
+            if t is not None:
+                self._batch_check(name, t, logits.dtype if t is logits else torch.float32, shape, contiguous=False)
+                if t.numel() and t.shape[2] > 1 and t.stride(2) != 1:
+                    raise ValueError(f"libquickprefill: {name}: rows must be contiguous")
+        self._batch_check("drafts", drafts, torch.int64, (B, T))
+        if n_draft is not None:
+            self._batch_check("n_draft", n_draft, torch.int32, (B,))
+        if uniforms is not None:
+            self._batch_check("uniforms", uniforms, torch.float32, (B, T + 1))
+        self._batch_check("n_accepted", n_accepted, torch.int32, (B,))
+        self._batch_check("tokens", tokens, torch.int64, (B, T + 1))
+        self._batch_check("workspace", workspace, workspace.dtype)
+        ps, pr = (draft_probs.stride(0), draft_probs.stride(1)) if draft_probs is not None else (0, 0)
+        self._check(self.lib.qp_verify_drafts(self.ctx, logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), logits.stride(1),
+                                              _ptr(drafts) if T else None, _ptr(n_draft), _ptr(draft_probs) if T else None, ps, pr, _ptr(uniforms), B, T, V,
+                                              float(temperature), n_accepted.data_ptr(), tokens.data_ptr(), workspace.data_ptr(),
+                                              workspace.numel() * workspace.element_size(), self._stream_here()))
 
     # -- vision front end
     def vit_rope(self, qkv, cos, sin, heads, head_dim):

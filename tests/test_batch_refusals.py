@@ -1,0 +1,148 @@
+"""What the batch operators (qp_batch_rope_append, qp_batch_attn, qp_verify_drafts) refuse, checked without a GPU: the C entry points
+validate before anything is launched, the Python face before it looks for a stream.  Pointers here are never followed."""
+import ctypes
+
+import pytest
+import torch
+
+from quickvideo_amd import native
+
+A = 1 << 20                      # an aligned address that nothing reads
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return native.load_library()
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    class Ctx(ctypes.Structure):  # struct qp_ctx {device, cus, lds_per_cu, lt}
+        _fields_ = [("device", ctypes.c_int), ("cus", ctypes.c_int), ("lds", ctypes.c_int), ("lt", ctypes.c_void_p)]
+    c = Ctx(0, 256, 65536, None)
+    return ctypes.addressof(c), c
+
+
+APPEND = dict(qkv=A, cos=A, sin=A, batch=2, t_max=3, seq_len=A, n_new=None, n_q=28, n_kv=4, head_dim=128, q_out=A + (1 << 24), k_pages=A, v_pages=A,
+              page_stride=4 * 16 * 128, n_pages=9, page_size=16, table=A, max_pages=4)
+ATTN = dict(q=A, k_prefix=A, v_prefix=A, stride=200 * 128, prefix_len=200, k_pages=A, v_pages=A, page_stride=4 * 16 * 128, n_pages=9, page_size=16, table=A,
+            max_pages=4, seq_len=A, n_new=None, batch=2, t_max=3, n_q=28, n_kv=4, head_dim=128, scale=0.1, out=A, ws=A, ws_bytes=1 << 30)
+VERIFY = dict(logits=A, f32=1, seq_stride=5000, row_stride=1000, drafts=A, n_draft=None, probs=None, pss=0, prs=0, u=A, batch=2, t_max=4, vocab=1000,
+              temperature=1.0, accepted=A, tokens=A, ws=A, ws_bytes=1 << 24)
+
+
+def call(fn, ctx, base, **change):
+    args = dict(base)
+    args.update(change)
+    return fn(ctx[0], *args.values(), None)
+
+
+@pytest.mark.parametrize("change,status,word", [
+    (dict(qkv=None), -1, "NULL"), (dict(seq_len=None), -1, "NULL"), (dict(table=None), -1, "NULL"), (dict(q_out=None), -1, "NULL"),
+    (dict(head_dim=64), -2, "head_dim"), (dict(batch=0), -1, "batch"), (dict(t_max=0), -1, "t_max"), (dict(batch=1 << 9, t_max=1 << 9), -2, "65536"),
+    (dict(n_q=30), -1, "multiple"), (dict(n_kv=0), -1, "multiple"), (dict(n_q=2048, n_kv=1), -2, "1024"), (dict(n_pages=0), -1, "n_pages"),
+    (dict(page_size=0), -1, "page_size"), (dict(max_pages=0), -1, "max_pages"), (dict(page_size=1 << 16, max_pages=1 << 16, page_stride=1 << 40), -2, "2^31"),
+    (dict(page_stride=4 * 16 * 128 - 8), -1, "page_stride"), (dict(page_stride=4 * 16 * 128 + 4), -1, "page_stride"), (dict(k_pages=A + 8), -1, "aligned"),
+    (dict(qkv=A + 2), -1, "alignment"), (dict(cos=A + 4), -1, "alignment"), (dict(q_out=A + 4096), -1, "overlaps"),
+])
+def test_append_refuses(lib, ctx, change, status, word):
+    assert call(lib.qp_batch_rope_append, ctx, APPEND, **change) == status
+    assert word in lib.qp_last_error().decode()
+
+
+def test_no_context(lib):
+    for fn, base in ((lib.qp_batch_rope_append, APPEND), (lib.qp_batch_attn, ATTN), (lib.qp_verify_drafts, VERIFY)):
+        assert fn(None, *base.values(), None) == -1 and "NULL" in lib.qp_last_error().decode()
+
+
+@pytest.mark.parametrize("change,status,word", [
+    (dict(q=None), -1, "NULL"), (dict(ws=None), -1, "NULL"), (dict(k_prefix=None), -1, "without prefix"), (dict(v_prefix=None), -1, "without prefix"),
+    (dict(head_dim=80), -2, "head_dim"), (dict(prefix_len=-1), -1, "prefix_len"), (dict(stride=199 * 128), -1, "prefix_head_stride"),
+    (dict(stride=200 * 128 + 4), -1, "prefix_head_stride"), (dict(prefix_len=1 << 31, stride=1 << 40), -2, "2^31"), (dict(scale=0.0), -1, "scale"),
+    (dict(scale=-1.0), -1, "scale"), (dict(scale=float("nan")), -1, "scale"), (dict(scale=float("inf")), -1, "scale"), (dict(out=A + 8), -1, "alignment"),
+    (dict(k_prefix=A + 2), -1, "alignment"), (dict(ws_bytes=1000), -4, "workspace"), (dict(batch=70000, t_max=1), -2, "65536"), (dict(n_q=27), -1, "multiple"),
+    (dict(page_size=17), -1, "page_stride"),
+])
+def test_attn_refuses(lib, ctx, change, status, word):
+    assert call(lib.qp_batch_attn, ctx, ATTN, **change) == status
+    assert word in lib.qp_last_error().decode()
+
+
+@pytest.mark.parametrize("change,status,word", [
+    (dict(logits=None), -1, "NULL"), (dict(accepted=None), -1, "NULL"), (dict(tokens=None), -1, "NULL"), (dict(drafts=None), -1, "drafts"),
+    (dict(u=None), -1, "random"), (dict(batch=0), -1, "batch"), (dict(batch=65536), -1, "batch"), (dict(t_max=-1), -2, "t_max"), (dict(t_max=256), -2, "t_max"),
+    (dict(vocab=0), -2, "vocab"), (dict(vocab=4194305, row_stride=1 << 30, seq_stride=1 << 30), -2, "vocab"), (dict(temperature=-0.5), -1, "temperature"),
+    (dict(temperature=float("nan")), -1, "temperature"), (dict(temperature=float("inf")), -1, "temperature"), (dict(row_stride=999), -1, "strides"),
+    (dict(seq_stride=999), -1, "strides"), (dict(probs=A, pss=4000, prs=999), -1, "draft_probs"), (dict(probs=A, pss=999, prs=1000), -1, "draft_probs"),
+    (dict(logits=A + 2), -1, "alignment"), (dict(logits=A + 1, f32=0), -1, "alignment"), (dict(probs=A + 2, pss=4000, prs=1000), -1, "alignment"),
+    (dict(ws=A + 4), -1, "alignment"), (dict(ws_bytes=100), -4, "workspace"),
+])
+def test_verify_refuses(lib, ctx, change, status, word):
+    assert call(lib.qp_verify_drafts, ctx, VERIFY, **change) == status
+    assert word in lib.qp_last_error().decode()
+
+
+def test_workspace_sizes(lib, ctx):
+    good = lib.qp_batch_attn_workspace_bytes(ctx[0], 4, 1, 11535, 256, 28, 4)
+    assert good > 0
+    for bad in ((0, 1, 10, 16, 28, 4), (4, 0, 10, 16, 28, 4), (4, 1, -1, 16, 28, 4), (4, 1, 10, 0, 28, 4), (4, 1, 10, 16, 27, 4), (70000, 1, 10, 16, 28, 4)):
+        assert lib.qp_batch_attn_workspace_bytes(ctx[0], *bad) == 0
+    assert lib.qp_batch_attn_workspace_bytes(None, 4, 1, 10, 16, 28, 4) == 0
+    assert lib.qp_verify_drafts_workspace_bytes(3, 4, 152064) > lib.qp_verify_drafts_workspace_bytes(3, 0, 1) > 0
+    for bad in ((0, 4, 10), (1, -1, 10), (1, 256, 10), (1, 4, 0), (65536, 0, 10), (1, 0, 4194305)):
+        assert lib.qp_verify_drafts_workspace_bytes(*bad) == 0
+
+
+@pytest.fixture
+def ops(ctx):
+    o = object.__new__(native.QuickPrefillOps)          # no GPU: everything below is refused before a pointer or a stream is taken
+    o.lib, o.ctx, o.device = native.load_library(), None, torch.device("cuda", 0)
+    return o
+
+
+def batch_tensors(B=2, T=3, hq=4, hkv=2, ps=4, pages=6, width=3):
+    bf = torch.bfloat16
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32)                                                           # noqa: E731
+    return dict(qkv=torch.zeros(B, T, (hq + 2 * hkv) * 128, dtype=bf), cos=torch.zeros(B, T, 64, dtype=bf), sin=torch.zeros(B, T, 64, dtype=bf), seq_len=i32(B),
+                n_new=i32(B), table=i32(B, width), k_pages=torch.zeros(pages, hkv, ps, 128, dtype=bf), v_pages=torch.zeros(pages, hkv, ps, 128, dtype=bf),
+                n_q=hq, n_kv=hkv, head_dim=128, q_out=torch.zeros(B, T, hq, 128, dtype=bf))
+
+
+@pytest.mark.parametrize("name,make,word", [
+    ("qkv", lambda t: t.float(), "float32"), ("qkv", lambda t: t[:, :, :-1], "shape"), ("cos", lambda t: t[:, :2], "contiguous"), ("q_out", lambda t: t[:, :, :3], "shape"),
+    ("seq_len", lambda t: t.long(), "int64"), ("n_new", lambda t: t[:1], "shape"), ("table", lambda t: t.float(), "float32"), ("table", lambda t: t.t(), "shape"),
+    ("k_pages", lambda t: t.half(), "float16"), ("v_pages", lambda t: t[:, :, :2], "shape"), ("v_pages", lambda t: t.transpose(1, 2).contiguous().transpose(1, 2), "page"),
+    ("v_pages", lambda t: torch.cat([t, t], 1)[:, :2], "page"), ("qkv", lambda t: t, "is on cpu"),
+])
+def test_python_append_refuses(ops, name, make, word):
+    kw = batch_tensors()
+    kw[name] = make(kw[name])
+    if word != "is on cpu":
+        ops._on_device = lambda t: True
+    with pytest.raises(ValueError, match=word):
+        ops.batch_rope_append(*kw.values())
+
+
+@pytest.mark.parametrize("name,make,word", [
+    ("logits", lambda t: t.double(), "float64"), ("logits", lambda t: t.transpose(1, 2).contiguous().transpose(1, 2), "rows must be contiguous"),
+    ("drafts", lambda t: t.int(), "int32"), ("drafts", lambda t: t[:, :1], "shape"), ("probs", lambda t: t.double(), "float64"), ("probs", lambda t: t[:, :, :5], "shape"),
+    ("u", lambda t: t[:, :1], "shape"), ("accepted", lambda t: t.long(), "int64"), ("tokens", lambda t: t[:, :2].contiguous(), "shape"), ("logits", lambda t: t, "is on cpu"),
+])
+def test_python_verify_refuses(ops, name, make, word):
+    B, T, V = 2, 2, 7
+    kw = dict(logits=torch.zeros(B, T + 1, V), drafts=torch.zeros(B, T, dtype=torch.int64), n_draft=None, probs=torch.zeros(B, T, V), u=torch.zeros(B, T + 1),
+              temperature=1.0, accepted=torch.zeros(B, dtype=torch.int32), tokens=torch.zeros(B, T + 1, dtype=torch.int64), ws=torch.zeros(4096, dtype=torch.uint8))
+    kw[name] = make(kw[name])
+    if word != "is on cpu":
+        ops._on_device = lambda t: True
+    with pytest.raises(ValueError, match=word):
+        ops.verify_drafts(*kw.values())
+
+
+def test_python_workspaces_refuse(ops, ctx):
+    ops.ctx = ctx[0]
+    with pytest.raises(ValueError, match="no batch"):
+        ops.batch_attn_workspace(0, 1, 10, 16, 28, 4)
+    with pytest.raises(ValueError, match="no verification"):
+        ops.verify_drafts_workspace(1, 256, 1000)
+    ops.ctx = None
