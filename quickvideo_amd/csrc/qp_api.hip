@@ -707,7 +707,7 @@ struct DeviceScope {
 int check_pages(const char* who, int64_t page_stride, int n_pages, int page_size, int max_pages, int n_kv_heads, const void* k_pages, const void* v_pages) {
   QP_REQUIRE(n_pages >= 1 && page_size >= 1 && max_pages >= 1, QP_ERR_INVALID, "%s: n_pages=%d, page_size=%d, max_pages=%d must be >= 1", who, n_pages,
              page_size, max_pages);
-  QP_REQUIRE((int64_t)max_pages * page_size <= INT32_MAX, QP_ERR_UNSUPPORTED, "%s: max_pages * page_size = %lld rows per sequence (at most 2^31 - 1)", who,
+  QP_REQUIRE((int64_t)max_pages * page_size <= (1 << 30), QP_ERR_UNSUPPORTED, "%s: max_pages * page_size = %lld rows per sequence (at most 2^30)", who,
              (long long)max_pages * page_size);
   QP_REQUIRE(page_stride >= (int64_t)n_kv_heads * page_size * 128 && page_stride % 8 == 0, QP_ERR_INVALID,
              "%s: page_stride=%lld elements (at least n_kv_heads * page_size * 128, a multiple of 8)", who, (long long)page_stride);
@@ -765,7 +765,7 @@ int qp_batch_attn(qp_ctx* ctx, const void* q, const void* k_prefix, const void* 
   QP_REQUIRE(prefix_len == 0 || (k_prefix && v_prefix), QP_ERR_INVALID, "%s: prefix_len=%lld without prefix tensors", who, (long long)prefix_len);
   QP_REQUIRE(prefix_len == 0 || (prefix_head_stride % 8 == 0 && prefix_head_stride / 128 >= prefix_len), QP_ERR_INVALID,
              "%s: prefix_head_stride=%lld elements for %lld rows (a multiple of 8)", who, (long long)prefix_head_stride, (long long)prefix_len);
-  QP_REQUIRE(prefix_len <= INT32_MAX, QP_ERR_UNSUPPORTED, "%s: prefix_len=%lld (at most 2^31 - 1)", who, (long long)prefix_len);
+  QP_REQUIRE(prefix_len <= (1 << 30), QP_ERR_UNSUPPORTED, "%s: prefix_len=%lld (at most 2^30)", who, (long long)prefix_len);
   QP_REQUIRE(scale > 0.f && scale <= 3.0e38f, QP_ERR_INVALID, "%s: scale=%g must be positive and finite", who, (double)scale);
   QP_REQUIRE(aligned16(q) && aligned16(k_prefix) && aligned16(v_prefix) && aligned16(out) && aligned16(workspace), QP_ERR_INVALID, "%s: alignment", who);
   const size_t need = qp_batch_attn_workspace_bytes_impl(ctx, batch, t_max, prefix_len, (int64_t)max_pages * page_size, n_q_heads, n_kv_heads);

@@ -31,8 +31,8 @@ __device__ __forceinline__ int rows_new(const Pages& p, int b, int t_max) {
   return n < 0 ? 0 : (n > t_max ? t_max : n);
 }
 // uint4 offset of key row j of sequence b, kv head h; -1 when the row has no page
-__device__ __forceinline__ int64_t page_row16(const Pages& p, int b, int h, int64_t j) {
-  if (j < 0 || j >= (int64_t)p.max_pages * p.page_size) return -1;
+__device__ __forceinline__ int64_t page_row16(const Pages& p, int b, int h, int j) {
+  if ((unsigned)j >= (unsigned)p.max_pages * (unsigned)p.page_size) return -1;
   const unsigned pi = (unsigned)j / (unsigned)p.page_size, slot = (unsigned)j - pi * (unsigned)p.page_size;
   const int page = p.table[(int64_t)b * p.max_pages + pi];
   if ((unsigned)page >= (unsigned)p.n_pages) return -1;
@@ -56,7 +56,8 @@ __global__ __launch_bounds__(256) void batch_rope_append_kernel(const uint4* __r
   const int heads = hq + 2 * hkv;
   if (hr >= heads) return;                                     // whole 16-lane groups
   const uint4 x = qkv[(row * heads + hr) * 16 + c];
-  const int64_t j = (int64_t)pg.seq_len[b] + t;
+  const int64_t row_to = (int64_t)pg.seq_len[b] + t;
+  const int j = row_to > INT32_MAX ? -1 : (int)row_to;
   if (hr >= hq + hkv) {
     const int64_t at = page_row16(pg, b, hr - hq - hkv, j);
     if (at >= 0) v_pages[at + c] = x;
@@ -99,27 +100,69 @@ struct BatchAttnParams {
   int64_t R;
   int ns, nrb;                    // prefix: key ranges, row blocks (per kv head)
   int ns2, nrb2;                  // pages: key ranges, row blocks (per sequence and kv head)
-  int64_t prefix_wgs;             // hkv * nrb * ns
+  unsigned page_wgs;              // batch * hkv * nrb2 * ns2
   float* part_o; float2* part_ml; // [hkv][ns + ns2][R] rows of 128 floats / (max, sum)
 };
 
 constexpr int kTile = 64;         // keys per tile
+constexpr int kMaxKeys = 1 << 30; // of the prefix, and of a sequence's table: key numbers and their sums fit in 32 bits
 
-// bf16 words whose exponent is all ones (infinities, NaN) set to zero; *any = there was one
-__device__ __forceinline__ unsigned finite_word(unsigned w, bool* any) {
-  if ((w & 0x7f80u) == 0x7f80u) { *any = true; w &= 0xffff0000u; }
-  if ((w & 0x7f800000u) == 0x7f800000u) { *any = true; w &= 0x0000ffffu; }
-  return w;
+// does one of the eight bf16 have an exponent of all ones (infinity, NaN)?
+__device__ __forceinline__ bool has_odd(uint4 x) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  auto mag = [](unsigned w) { return __builtin_bit_cast(u16x2, w & 0x7fff7fffu); };
+  const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(mag(x.x), mag(x.y)), __builtin_elementwise_max(mag(x.z), mag(x.w)));
+  return m.x >= 0x7f80 || m.y >= 0x7f80;
+}
+__device__ __forceinline__ void make_finite(uint4& x) {       // such numbers to zero
+  unsigned* w = reinterpret_cast<unsigned*>(&x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if ((w[i] & 0x7f80u) == 0x7f80u) w[i] &= 0xffff0000u;
+    if ((w[i] & 0x7f800000u) == 0x7f800000u) w[i] &= 0x0000ffffu;
+  }
+}
+
+// The rare end of a range: every value that is not finite is added, times its probability, to the rows that see it, where their partial results
+// lie (one thread per row: it wrote none of them itself, the barrier before the call orders the writes).
+template <bool kPaged>
+__device__ __forceinline__ void add_odd_values(const BatchAttnParams& p, int kvh, int b, int64_t row0, int64_t row_end, int k0, int k1, int64_t slot0) {
+  for (int key = k0; key < k1; ++key) {
+    const int64_t at = kPaged ? page_row16(p.pg, b, kvh, key) : (int64_t)kvh * p.pre_hs16 + (int64_t)key * 16;
+    if (at < 0) continue;
+    const uint4* vrow = (kPaged ? p.v_pages : p.v_pre) + at;
+    bool odd = false;
+    for (int i = 0; i < 16; ++i) odd |= has_odd(vrow[i]);
+    if (!odd) continue;                                        // (the same for all threads)
+    const uint16_t* krow = reinterpret_cast<const uint16_t*>((kPaged ? p.k_pages : p.k_pre) + at);
+    for (int64_t r = row0 + threadIdx.x; r < row_end; r += blockDim.x) {
+      const int64_t bt = r / p.G;
+      if (kPaged && key > (int64_t)p.pg.seq_len[b] + (bt - (int64_t)b * p.t_max)) continue;
+      const uint16_t* qrow = reinterpret_cast<const uint16_t*>(p.q) + ((bt * p.hq) + (int64_t)kvh * p.G + (r - bt * p.G)) * 128;
+      float s = 0.f;
+      for (int d = 0; d < 128; ++d) s = __builtin_fmaf(bf16_bits_to_f32(qrow[d]), bf16_bits_to_f32(krow[d]), s);
+      const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c, -p.part_ml[slot0 + r].x * p.c));
+      for (int d = 0; d < 128; ++d) {
+        const uint16_t w = reinterpret_cast<const uint16_t*>(vrow)[d];
+        if ((w & 0x7f80u) == 0x7f80u) p.part_o[(slot0 + r) * 128 + d] += pe * bf16_bits_to_f32(w);
+      }
+    }
+  }
 }
 
 // A workgroup of WR x WK waves takes a block of 32 * WR rows over one key range, kTile keys at a time: the tile goes through registers into LDS
 // (K row-major with XOR-swizzled 16-B slots; V as [key / 4][d / 32][key % 4][32] for the transposing LDS reads), the next tile's loads are in
 // flight while this one is computed.  Wave (wr, wk) owns rows [32 wr, 32 wr + 32) and, for WK = 2, half of the tile's keys:
-// S^T = K.Q^T (rows are the columns of v_mfma_f32_32x32x16_bf16: a lane owns one row), online softmax, O^T += V^T.P, P rounded to bf16 for
-// the product (as in the prefill and decode kernels: its error averages out below the output's own rounding), everything else fp32.
+// S^T = K.Q^T (rows are the columns of v_mfma_f32_32x32x16_bf16: a lane owns one row), online softmax, O^T += V^T.P, all sums in fp32.
+// A value that is not finite would spoil rows that do not see it (0 * infinity is NaN) and the sum of the two products below, so it goes into
+// LDS as zero; a range that holds one ends with add_odd_values.
+// P goes into the product as TWO bf16 numbers, bf16(p) and bf16(p - bf16(p)): 2^-17 of p is lost instead of 2^-9.  Rounded once, as the prefill and
+// decode kernels do it, the result's error against 64 bits is 0.0021 - 0.0027 of it, with two terms 0.0017, which is its own rounding; the second
+// product reuses the V fragments, and a step that waits for the prefix's bytes has the matrix pipe free.
 template <int WR, int WK, bool kPaged>
-__device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int kvh, int b, int64_t row0, int64_t row_end, int64_t k0, int64_t k1,
-                                                 int part, unsigned char* lds, float* lds_ml, unsigned long long* key_bits) {
+__device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int kvh, int b, int64_t row0, int64_t row_end, int k0, int k1,
+                                                 int part, unsigned char* lds, float* lds_ml, unsigned long long* hole_keys, int* odd_seen) {
+  constexpr bool kAhead = !kPaged || WR > 1;                   // (with 64 registers a thread in flight the paged form of the narrow one would spill)
   constexpr int NT = 64 * WR * WK, PT = kTile * 16 / NT, KB = 2 / WK;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, l31 = lane & 31;
   const int wr = wave % WR, wk = wave / WR;
@@ -129,8 +172,8 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
   unsigned char* kl = lds;
   unsigned char* vl = lds + kTile * 256;
   bf16x8_t qf[8];
-  int64_t limit = INT64_MAX;                                   // last visible key of this lane's row
-  int64_t seen_by_all = INT64_MAX;                             // keys below this are visible to every row of the sequence
+  int limit = INT32_MAX;                                       // last visible key of this lane's row
+  int seen_by_all = INT32_MAX;                                 // keys below this are visible to every row of the sequence
   {
     const int64_t rr = row_live ? r : row0;
     const int64_t bt = rr / p.G;
@@ -143,8 +186,9 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
       qf[kk] = __builtin_bit_cast(bf16x8_t, x);
     }
     if (kPaged) {
-      seen_by_all = (int64_t)p.pg.seq_len[b] + 1;
-      limit = (int64_t)p.pg.seq_len[b] + (bt - (int64_t)b * p.t_max);
+      const int stored = min(p.pg.seq_len[b], kMaxKeys);      // (a table has no more rows)
+      seen_by_all = stored + 1;
+      limit = stored + (int)(bt - (int64_t)b * p.t_max);
     }
   }
   const uint4* kbase = kPaged ? p.k_pages : p.k_pre + (int64_t)kvh * p.pre_hs16;
@@ -152,19 +196,32 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
   const int slot16 = tid & 15, srow = tid >> 4;                // this thread stages rows srow + i * (NT / 16), 16-B slot slot16
   uint4 kx[PT], vx[PT];
   unsigned holes = 0;                                          // bit i: staged row i has no page
-  auto load = [&](int64_t t0) {
-    holes = 0;
+  auto load = [&](int t0) {                                // rows past the end are zero: their probability is 0, and 0 * 0 stays 0
+    if (!kPaged) {
+      const uint4* kt = kbase + (int64_t)t0 * 16;              // a tile of the prefix is 16 KB in a row
+      const uint4* vt = vbase + (int64_t)t0 * 16;
+      if (t0 + kTile <= k1) {
 #pragma unroll
-    for (int i = 0; i < PT; ++i) {
-      const int64_t key = t0 + srow + i * (NT / 16);
-      kx[i] = vx[i] = make_uint4(0, 0, 0, 0);                  // rows past the end are zero: their probability is 0 and 0 * 0 stays 0
-      if (key < k1) {
-        int64_t at = key * 16;
-        if (kPaged) {
-          at = page_row16(p.pg, b, kvh, key);
-          if (at < 0) { holes |= 1u << i; continue; }
+        for (int i = 0; i < PT; ++i) { kx[i] = kt[tid + i * NT]; vx[i] = vt[tid + i * NT]; }
+      } else {
+        const int rows = k1 - t0;
+#pragma unroll
+        for (int i = 0; i < PT; ++i) {
+          kx[i] = vx[i] = make_uint4(0, 0, 0, 0);
+          if (srow + i * (NT / 16) < rows) { kx[i] = kt[tid + i * NT]; vx[i] = vt[tid + i * NT]; }
         }
-        kx[i] = kbase[at + slot16]; vx[i] = vbase[at + slot16];
+      }
+    } else {
+      holes = 0;
+#pragma unroll
+      for (int i = 0; i < PT; ++i) {
+        const int key = t0 + srow + i * (NT / 16);
+        kx[i] = vx[i] = make_uint4(0, 0, 0, 0);
+        if (key < k1) {
+          const int64_t at = page_row16(p.pg, b, kvh, key);
+          if (at < 0) { holes |= 1u << i; continue; }
+          kx[i] = kbase[at + slot16]; vx[i] = vbase[at + slot16];
+        }
       }
     }
   };
@@ -176,34 +233,26 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
 #pragma unroll
   for (int db = 0; db < 4; ++db) o[db] = (f32x16_t){0};
   float m_run = -1e30f, l_run = 0.f;
-  if (kPaged && tid < 4) key_bits[tid] = 0;                    // [parity][0: rows without a page, 1: masked rows with a non-finite value]
+  if (tid < 2) hole_keys[tid] = 0;                             // by parity of the tile: its rows without a page
+  if (tid == 0) *odd_seen = 0;                                 // set when the range holds a value that is not finite
   int par = 0;
-  if (k0 < k1) load(k0);
-  for (int64_t t0 = k0; t0 < k1; t0 += kTile, par ^= 1) {
+  if (kAhead && k0 < k1) load(k0);
+  for (int t0 = k0; t0 < k1; t0 += kTile, par ^= 1) {
+    if (!kAhead) load(t0);
     __syncthreads();                                           // everyone has read the previous tile
     const bool masked = kPaged && t0 + kTile > seen_by_all;    // some row of the sequence does not see some key of this tile
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
       const int row = srow + i * (NT / 16);
-      if (kPaged) {
-        if ((holes >> i) & 1 && slot16 == 0) atomicOr(&key_bits[par * 2], 1ull << row);
-        if (masked && t0 + row >= seen_by_all) {               // 0 * infinity is NaN: a masked row's values must be finite in the product
-          bool any = false;
-          vx[i].x = finite_word(vx[i].x, &any); vx[i].y = finite_word(vx[i].y, &any);
-          vx[i].z = finite_word(vx[i].z, &any); vx[i].w = finite_word(vx[i].w, &any);
-          if (any) atomicOr(&key_bits[par * 2 + 1], 1ull << row);
-        }
-      }
+      if (kPaged && ((holes >> i) & 1) && slot16 == 0) atomicOr(&hole_keys[par], 1ull << row);
+      if (has_odd(vx[i])) { make_finite(vx[i]); *odd_seen = 1; }
       *reinterpret_cast<uint4*>(kl + row * 256 + ((slot16 ^ (row & 15)) << 4)) = kx[i];
       *reinterpret_cast<uint4*>(vl + (((row >> 2) * 4 + (slot16 >> 2)) << 8) + ((row & 3) << 6) + ((slot16 & 3) << 4)) = vx[i];
     }
     __syncthreads();
-    unsigned long long hole_bits = 0, odd_bits = 0;
-    if (kPaged) {
-      hole_bits = key_bits[par * 2]; odd_bits = key_bits[par * 2 + 1];
-      if (tid < 2) key_bits[(par ^ 1) * 2 + tid] = 0;          // last read before the barrier above, next written behind the next one
-    }
-    if (t0 + kTile < k1) load(t0 + kTile);
+    const unsigned long long hole_bits = kPaged ? hole_keys[par] : 0;
+    if (kPaged && tid == 0) hole_keys[par ^ 1] = 0;            // last read before the barrier above, next written behind the next one
+    if (kAhead && t0 + kTile < k1) load(t0 + kTile);
     if (!wave_live) continue;
     f32x16_t s[KB];
 #pragma unroll
@@ -214,15 +263,18 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
       for (int kk = 0; kk < 8; ++kk)
         s[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_read_b128(kl, kb * 32 * 256 + koff[kk]), qf[kk], s[k], 0, 0, 0);
     }
+    __builtin_amdgcn_sched_barrier(0);                         // (keeps hipcc from holding K, V and the next tile in registers at once)
     if (t0 + kTile > k1 || masked || hole_bits) {
+      const int last = (limit < k1 ? limit : k1 - 1) - t0 - 4 * hi;              // last visible row of the tile, seen from this lane's rows
+      const unsigned long long here = ~hole_bits >> (4 * hi);
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
         const int kb = WK == 2 ? wk : k;
+        const unsigned have = (unsigned)(here >> (kb * 32));
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int row = kb * 32 + (e & 3) + 8 * (e >> 2) + 4 * hi;
-          const int64_t key = t0 + row;
-          s[k][e] = (key < k1 && key <= limit && !((hole_bits >> row) & 1)) ? s[k][e] : -INFINITY;
+          const int row = (e & 3) + 8 * (e >> 2);
+          s[k][e] = kb * 32 + row <= last && ((have >> row) & 1) ? s[k][e] : -INFINITY;
         }
       }
     }
@@ -247,7 +299,7 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
 #pragma unroll
     for (int k = 0; k < KB; ++k) {
       const int kb = WK == 2 ? wk : k;
-      bf16x8_t pf[2];
+      bf16x8_t pf[2], pr[2];
 #pragma unroll
       for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
@@ -255,7 +307,9 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
           const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][cc * 8 + e], p.c, -mc));
           rs += pe;
           pf[cc][e] = (__bf16)pe;
+          pr[cc][e] = (__bf16)(pe - (float)pf[cc][e]);
         }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
@@ -265,32 +319,8 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
           const s16x4_t v1 = lds_read_tr16(vl, off + (2 * 4 << 8));
           const s16x8_t av = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
           o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), pf[cc], o[db], 0, 0, 0);
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), pr[cc], o[db], 0, 0, 0);
         }
-      if (kPaged && odd_bits) {                                // rare: give the rows that DO see such a key its infinities / NaN back
-#pragma unroll 1
-        for (int row = 0; row < 32; ++row) {
-          const int trow = kb * 32 + row;
-          if (!((odd_bits >> trow) & 1)) continue;
-          const int64_t key = t0 + trow;
-          const int64_t at = page_row16(p.pg, b, kvh, key);
-          if (at < 0) continue;
-          const uint16_t* vrow = reinterpret_cast<const uint16_t*>(vbase + at);
-          const int e_of = (row & 3) + 4 * (row >> 3), h_of = (row >> 2) & 1;
-          float pv = 0.f;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) pv = e == e_of ? (float)pf[e >> 3][e & 7] : pv;
-          pv = __shfl(pv, l31 + 32 * h_of, 64);
-          if (key <= limit) {
-#pragma unroll
-            for (int db = 0; db < 4; ++db)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const uint16_t w = vrow[db * 32 + 8 * (e >> 2) + 4 * hi + (e & 3)];
-                if ((w & 0x7f80u) == 0x7f80u) o[db][e] += pv * bf16_bits_to_f32(w);
-              }
-          }
-        }
-      }
     }
     l_run += xhalf_sum(rs);
   }
@@ -307,7 +337,7 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
               make_float4(o[db][q4 * 4 + 0], o[db][q4 * 4 + 1], o[db][q4 * 4 + 2], o[db][q4 * 4 + 3]);
     }
     __syncthreads();
-    if (wk == 1) return;
+    if (wk == 0) {
     const float m1 = lds_ml[(wr * 32 + l31) * 2], l1 = lds_ml[(wr * 32 + l31) * 2 + 1];
     const float m = fmaxf(m_run, m1);
     const float a0 = __builtin_amdgcn_exp2f((m_run - m) * p.c), a1 = __builtin_amdgcn_exp2f((m1 - m) * p.c);
@@ -317,47 +347,64 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
     for (int db = 0; db < 4; ++db)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[db][e] = o[db][e] * a0 + obuf[(wr * 32 + l31) * 128 + db * 32 + 8 * (e >> 2) + 4 * hi + (e & 3)] * a1;
+    }
   }
-  if (!row_live) return;
-  const int64_t slot = ((int64_t)kvh * (p.ns + p.ns2) + part) * p.R + r;
-  if (hi == 0) p.part_ml[slot] = make_float2(m_run, l_run);
+  const int64_t slot0 = ((int64_t)kvh * (p.ns + p.ns2) + part) * p.R;
+  if (row_live && wk == 0) {
+    if (hi == 0) p.part_ml[slot0 + r] = make_float2(m_run, l_run);
 #pragma unroll
-  for (int db = 0; db < 4; ++db)
+    for (int db = 0; db < 4; ++db)
 #pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4)
-      *reinterpret_cast<float4*>(p.part_o + slot * 128 + db * 32 + 8 * q4 + 4 * hi) =
-          make_float4(o[db][q4 * 4 + 0], o[db][q4 * 4 + 1], o[db][q4 * 4 + 2], o[db][q4 * 4 + 3]);
+      for (int q4 = 0; q4 < 4; ++q4)
+        *reinterpret_cast<float4*>(p.part_o + (slot0 + r) * 128 + db * 32 + 8 * q4 + 4 * hi) =
+            make_float4(o[db][q4 * 4 + 0], o[db][q4 * 4 + 1], o[db][q4 * 4 + 2], o[db][q4 * 4 + 3]);
+  }
+  if (k0 < k1 && *odd_seen) {                                  // (read behind the loop's barriers)
+    __threadfence_block();
+    __syncthreads();
+    add_odd_values<kPaged>(p, kvh, b, row0, row0 + 32 * WR < row_end ? row0 + 32 * WR : row_end, k0, k1, slot0);
+  }
 }
 
+// range `split` of n keys cut into `ns` ranges of whole tiles (the last ones may be empty: k0 >= k1)
+__device__ __forceinline__ void key_range(int n, int ns, int split, int& k0, int& k1) {
+  const int tiles = (n + kTile - 1) / kTile, per = (tiles + ns - 1) / ns;
+  const int64_t at = (int64_t)split * per * kTile, to = at + (int64_t)per * kTile;
+  k0 = (int)(at < n ? at : n);
+  k1 = (int)(to < n ? to : n);
+}
+
+// Grid: first the workgroups of the pages (short), then those of the prefix.  The row blocks that read the same keys are 8 workgroups apart, so that
+// they run on the same XCD (workgroups go to the 8 XCDs in turn) and share its L2.
 template <int WR, int WK>
 __global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnParams p) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kTile * 256];
   __shared__ float lds_ml[WR * 64];
-  __shared__ unsigned long long key_bits[4];
-  int64_t w = blockIdx.x;
-  if (w < p.prefix_wgs) {
-    const int rb = (int)(w % p.nrb), split = (int)((w / p.nrb) % p.ns), kvh = (int)(w / ((int64_t)p.nrb * p.ns));
-    int64_t chunk = (p.P + p.ns - 1) / p.ns;
-    chunk = (chunk + kTile - 1) / kTile * kTile;
-    const int64_t k0 = (int64_t)split * chunk, k1 = k0 + chunk < p.P ? k0 + chunk : p.P;
-    batch_attn_range<WR, WK, false>(p, kvh, 0, (int64_t)rb * 32 * WR, p.R, k0, k1, split, lds, lds_ml, key_bits);
+  __shared__ unsigned long long hole_keys[2];
+  __shared__ int odd_seen;
+  if (blockIdx.x >= p.page_wgs) {
+    const unsigned w = blockIdx.x - p.page_wgs, turn = 8u * p.nrb;
+    const int item = (int)(w / turn) * 8 + (int)(w % 8), rb = (int)(w % turn) / 8;
+    if (item >= p.hkv * p.ns) return;
+    const int kvh = item / p.ns, split = item - kvh * p.ns;
+    int k0, k1;
+    key_range((int)p.P, p.ns, split, k0, k1);
+    batch_attn_range<WR, WK, false>(p, kvh, 0, (int64_t)rb * 32 * WR, p.R, k0, k1, split, lds, lds_ml, hole_keys, &odd_seen);
     return;
   }
-  w -= p.prefix_wgs;
-  const int rb = (int)(w % p.nrb2), split = (int)((w / p.nrb2) % p.ns2);
-  const int64_t hb = w / ((int64_t)p.nrb2 * p.ns2);
-  const int kvh = (int)(hb % p.hkv), b = (int)(hb / p.hkv);
+  const int w = (int)blockIdx.x;
+  const int rb = w % p.nrb2, split = (w / p.nrb2) % p.ns2, hb = w / (p.nrb2 * p.ns2);
+  const int kvh = hb % p.hkv, b = hb / p.hkv;
   const int n_new = rows_new(p.pg, b, p.t_max);
   if (n_new == 0) return;                                      // nothing of this sequence is written
   int64_t len = (int64_t)p.pg.seq_len[b] + n_new;
   if (len > (int64_t)p.pg.max_pages * p.pg.page_size) len = (int64_t)p.pg.max_pages * p.pg.page_size;
   if (len < 0) len = 0;
-  int64_t chunk = (len + p.ns2 - 1) / p.ns2;
-  chunk = (chunk + kTile - 1) / kTile * kTile;
-  const int64_t k0 = (int64_t)split * chunk, k1 = k0 + chunk < len ? k0 + chunk : len;
+  int k0, k1;
+  key_range((int)len, p.ns2, split, k0, k1);
   const int64_t seq_row0 = (int64_t)b * p.t_max * p.G, row0 = seq_row0 + (int64_t)rb * 32 * WR, row_end = seq_row0 + (int64_t)n_new * p.G;
   if (row0 >= row_end) return;
-  batch_attn_range<WR, WK, true>(p, kvh, b, row0, row_end, k0, k1, p.ns + split, lds, lds_ml, key_bits);
+  batch_attn_range<WR, WK, true>(p, kvh, b, row0, row_end, k0, k1, p.ns + split, lds, lds_ml, hole_keys, &odd_seen);
 }
 
 // one workgroup per row: 8 groups of 32 lanes walk the partial results (16 B per lane), then join through LDS
@@ -409,22 +456,27 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
   *reinterpret_cast<uint2*>(p.out + ((bt * p.hq) + (int64_t)kvh * p.G + g) * 128 + lane32 * 4) = y;
 }
 
-struct Plan { int ns, nrb, ns2, nrb2; int64_t R; };
+struct Plan { int wr, ns, nrb, ns2, nrb2; int64_t R; };
 
+// Row blocks as wide as the batch's rows (up to 256), key ranges so many that every CU is busy once.
 Plan make_plan(const qp_ctx* ctx, int batch, int t_max, int64_t P, int64_t suffix_cap, int hq, int hkv) {
   Plan pl;
-  const int G = hq / hkv, rows = 32;
+  const int G = hq / hkv;
   pl.R = (int64_t)batch * t_max * G;
+  pl.wr = pl.R <= 32 ? 1 : (pl.R <= 64 ? 2 : (pl.R <= 128 ? 4 : 8));
+  const int rows = 32 * pl.wr, per_cu = pl.wr == 1 ? 4 : (pl.wr == 8 ? 1 : 2);     // resident workgroups (registers: two waves per SIMD)
   pl.nrb = (int)((pl.R + rows - 1) / rows);
   pl.nrb2 = (int)(((int64_t)t_max * G + rows - 1) / rows);
-  const int64_t want = 4LL * ctx->cus;
-  int64_t ns = (want + (int64_t)hkv * pl.nrb - 1) / ((int64_t)hkv * pl.nrb);
-  const int64_t most = (P + 127) / 128;
-  pl.ns = (int)(ns < most ? ns : most);
-  int64_t ns2 = want / ((int64_t)hkv * batch * pl.nrb2);
+  const int64_t slots = (int64_t)per_cu * ctx->cus, seqs = (int64_t)hkv * batch * pl.nrb2;
+  int64_t ns2 = slots / (4 * seqs);
   const int64_t most2 = (suffix_cap + 255) / 256;
   if (ns2 > most2) ns2 = most2;
   pl.ns2 = (int)(ns2 < 1 ? 1 : (ns2 > 64 ? 64 : ns2));
+  const int64_t page_wgs = seqs * pl.ns2, left = page_wgs * 2 < slots ? slots - page_wgs : slots;
+  int64_t ns = left / ((int64_t)hkv * pl.nrb);
+  const int64_t most = (P + 2 * kTile - 1) / (2 * kTile);
+  if (ns < 1) ns = 1;
+  pl.ns = (int)(ns < most ? ns : most);
   return pl;
 }
 
@@ -467,11 +519,16 @@ int qp_launch_batch_attn(const qp_ctx* ctx, const void* q, const void* k_prefix,
   p.pg = pages_of(table, seq_len, n_new, max_pages, n_pages, page_size, page_stride);
   p.t_max = t_max; p.hq = hq; p.hkv = hkv; p.G = hq / hkv; p.c = scale * 1.4426950408889634f;
   p.R = pl.R; p.ns = pl.ns; p.nrb = pl.nrb; p.ns2 = pl.ns2; p.nrb2 = pl.nrb2;
-  p.prefix_wgs = (int64_t)hkv * pl.nrb * pl.ns;
+  p.page_wgs = (unsigned)((int64_t)hkv * batch * pl.nrb2 * pl.ns2);
   p.part_ml = (float2*)workspace;
   p.part_o = (float*)((char*)workspace + ml_bytes(pl, hkv));
-  const int64_t grid = p.prefix_wgs + (int64_t)hkv * batch * pl.nrb2 * pl.ns2;
-  batch_attn_kernel<1, 2><<<(unsigned)grid, 128, 0, s>>>(p);
+  const unsigned grid = p.page_wgs + (unsigned)(((int64_t)hkv * pl.ns + 7) / 8 * 8 * pl.nrb);
+  switch (pl.wr) {
+    case 1: batch_attn_kernel<1, 2><<<grid, 128, 0, s>>>(p); break;
+    case 2: batch_attn_kernel<2, 2><<<grid, 256, 0, s>>>(p); break;
+    case 4: batch_attn_kernel<4, 1><<<grid, 256, 0, s>>>(p); break;
+    default: batch_attn_kernel<8, 1><<<grid, 512, 0, s>>>(p); break;
+  }
   int rc = qp_check_launch("batch_attn");
   if (rc) return rc;
   batch_combine_kernel<<<(unsigned)(pl.R * hkv), 256, 0, s>>>(p);

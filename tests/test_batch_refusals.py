@@ -41,7 +41,7 @@ def call(fn, ctx, base, **change):
     (dict(qkv=None), -1, "NULL"), (dict(seq_len=None), -1, "NULL"), (dict(table=None), -1, "NULL"), (dict(q_out=None), -1, "NULL"),
     (dict(head_dim=64), -2, "head_dim"), (dict(batch=0), -1, "batch"), (dict(t_max=0), -1, "t_max"), (dict(batch=1 << 9, t_max=1 << 9), -2, "65536"),
     (dict(n_q=30), -1, "multiple"), (dict(n_kv=0), -1, "multiple"), (dict(n_q=2048, n_kv=1), -2, "1024"), (dict(n_pages=0), -1, "n_pages"),
-    (dict(page_size=0), -1, "page_size"), (dict(max_pages=0), -1, "max_pages"), (dict(page_size=1 << 16, max_pages=1 << 16, page_stride=1 << 40), -2, "2^31"),
+    (dict(page_size=0), -1, "page_size"), (dict(max_pages=0), -1, "max_pages"), (dict(page_size=1 << 16, max_pages=1 << 16, page_stride=1 << 40), -2, "2^30"),
     (dict(page_stride=4 * 16 * 128 - 8), -1, "page_stride"), (dict(page_stride=4 * 16 * 128 + 4), -1, "page_stride"), (dict(k_pages=A + 8), -1, "aligned"),
     (dict(qkv=A + 2), -1, "alignment"), (dict(cos=A + 4), -1, "alignment"), (dict(q_out=A + 4096), -1, "overlaps"),
 ])
@@ -58,7 +58,7 @@ def test_no_context(lib):
 @pytest.mark.parametrize("change,status,word", [
     (dict(q=None), -1, "NULL"), (dict(ws=None), -1, "NULL"), (dict(k_prefix=None), -1, "without prefix"), (dict(v_prefix=None), -1, "without prefix"),
     (dict(head_dim=80), -2, "head_dim"), (dict(prefix_len=-1), -1, "prefix_len"), (dict(stride=199 * 128), -1, "prefix_head_stride"),
-    (dict(stride=200 * 128 + 4), -1, "prefix_head_stride"), (dict(prefix_len=1 << 31, stride=1 << 40), -2, "2^31"), (dict(scale=0.0), -1, "scale"),
+    (dict(stride=200 * 128 + 4), -1, "prefix_head_stride"), (dict(prefix_len=(1 << 30) + 1, stride=1 << 40), -2, "2^30"), (dict(scale=0.0), -1, "scale"),
     (dict(scale=-1.0), -1, "scale"), (dict(scale=float("nan")), -1, "scale"), (dict(scale=float("inf")), -1, "scale"), (dict(out=A + 8), -1, "alignment"),
     (dict(k_prefix=A + 2), -1, "alignment"), (dict(ws_bytes=1000), -4, "workspace"), (dict(batch=70000, t_max=1), -2, "65536"), (dict(n_q=27), -1, "multiple"),
     (dict(page_size=17), -1, "page_stride"),
@@ -96,7 +96,7 @@ def test_workspace_sizes(lib, ctx):
 @pytest.fixture
 def ops(ctx):
     o = object.__new__(native.QuickPrefillOps)          # no GPU: everything below is refused before a pointer or a stream is taken
-    o.lib, o.ctx, o.device = native.load_library(), None, torch.device("cuda", 0)
+    o.lib, o.ctx, o.device, o._dev = native.load_library(), None, torch.device("cuda", 0), -1          # -1: where torch says CPU tensors are
     return o
 
 
@@ -109,7 +109,7 @@ def batch_tensors(B=2, T=3, hq=4, hkv=2, ps=4, pages=6, width=3):
 
 
 @pytest.mark.parametrize("name,make,word", [
-    ("qkv", lambda t: t.float(), "float32"), ("qkv", lambda t: t[:, :, :-1], "shape"), ("cos", lambda t: t[:, :2], "contiguous"), ("q_out", lambda t: t[:, :, :3], "shape"),
+    ("qkv", lambda t: t.float(), "float32"), ("qkv", lambda t: t[:, :, :-1], "shape"), ("cos", lambda t: t[:, :2], "shape"), ("sin", lambda t: t.transpose(1, 2).contiguous().transpose(1, 2), "contiguous"), ("q_out", lambda t: t[:, :, :3], "shape"),
     ("seq_len", lambda t: t.long(), "int64"), ("n_new", lambda t: t[:1], "shape"), ("table", lambda t: t.float(), "float32"), ("table", lambda t: t.t(), "shape"),
     ("k_pages", lambda t: t.half(), "float16"), ("v_pages", lambda t: t[:, :, :2], "shape"), ("v_pages", lambda t: t.transpose(1, 2).contiguous().transpose(1, 2), "page"),
     ("v_pages", lambda t: torch.cat([t, t], 1)[:, :2], "page"), ("qkv", lambda t: t, "is on cpu"),
@@ -117,8 +117,8 @@ def batch_tensors(B=2, T=3, hq=4, hkv=2, ps=4, pages=6, width=3):
 def test_python_append_refuses(ops, name, make, word):
     kw = batch_tensors()
     kw[name] = make(kw[name])
-    if word != "is on cpu":
-        ops._on_device = lambda t: True
+    if word == "is on cpu":
+        ops._dev = 0
     with pytest.raises(ValueError, match=word):
         ops.batch_rope_append(*kw.values())
 
@@ -133,8 +133,8 @@ def test_python_verify_refuses(ops, name, make, word):
     kw = dict(logits=torch.zeros(B, T + 1, V), drafts=torch.zeros(B, T, dtype=torch.int64), n_draft=None, probs=torch.zeros(B, T, V), u=torch.zeros(B, T + 1),
               temperature=1.0, accepted=torch.zeros(B, dtype=torch.int32), tokens=torch.zeros(B, T + 1, dtype=torch.int64), ws=torch.zeros(4096, dtype=torch.uint8))
     kw[name] = make(kw[name])
-    if word != "is on cpu":
-        ops._on_device = lambda t: True
+    if word == "is on cpu":
+        ops._dev = 0
     with pytest.raises(ValueError, match=word):
         ops.verify_drafts(*kw.values())
 
