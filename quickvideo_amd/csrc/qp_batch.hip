@@ -104,16 +104,16 @@ struct BatchAttnParams {
   float* part_o; float2* part_ml; // [hkv][ns + ns2][R] rows of 128 floats / (max, sum)
 };
 
-constexpr int kTile = 64;         // keys per tile
+constexpr float kTiny = 1e-38f;   // least weight of a key or range that is seen: an infinite value shows however small its probability
 constexpr int kMaxKeys = 1 << 30; // of the prefix, and of a sequence's table: key numbers and their sums fit in 32 bits
 
-// does one of the eight bf16 have an exponent of all ones (infinity, NaN)?
-__device__ __forceinline__ bool has_odd(uint4 x) {
-  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
-  auto mag = [](unsigned w) { return __builtin_bit_cast(u16x2, w & 0x7fff7fffu); };
-  const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(mag(x.x), mag(x.y)), __builtin_elementwise_max(mag(x.z), mag(x.w)));
-  return m.x >= 0x7f80 || m.y >= 0x7f80;
+// largest of eight bf16 as 15-bit patterns (even and odd places apart); is_odd: an exponent of all ones among them (infinity, NaN)
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2_t magnitude(uint4 x) {
+  auto mag = [](unsigned w) { return __builtin_bit_cast(u16x2_t, w & 0x7fff7fffu); };
+  return __builtin_elementwise_max(__builtin_elementwise_max(mag(x.x), mag(x.y)), __builtin_elementwise_max(mag(x.z), mag(x.w)));
 }
+__device__ __forceinline__ bool is_odd(u16x2_t m) { return m.x >= 0x7f80 || m.y >= 0x7f80; }
 __device__ __forceinline__ void make_finite(uint4& x) {       // such numbers to zero
   unsigned* w = reinterpret_cast<unsigned*>(&x);
 #pragma unroll
@@ -132,7 +132,7 @@ __device__ __forceinline__ void add_odd_values(const BatchAttnParams& p, int kvh
     if (at < 0) continue;
     const uint4* vrow = (kPaged ? p.v_pages : p.v_pre) + at;
     bool odd = false;
-    for (int i = 0; i < 16; ++i) odd |= has_odd(vrow[i]);
+    for (int i = 0; i < 16; ++i) odd |= is_odd(magnitude(vrow[i]));
     if (!odd) continue;                                        // (the same for all threads)
     const uint16_t* krow = reinterpret_cast<const uint16_t*>((kPaged ? p.k_pages : p.k_pre) + at);
     for (int64_t r = row0 + threadIdx.x; r < row_end; r += blockDim.x) {
@@ -141,7 +141,7 @@ __device__ __forceinline__ void add_odd_values(const BatchAttnParams& p, int kvh
       const uint16_t* qrow = reinterpret_cast<const uint16_t*>(p.q) + ((bt * p.hq) + (int64_t)kvh * p.G + (r - bt * p.G)) * 128;
       float s = 0.f;
       for (int d = 0; d < 128; ++d) s = __builtin_fmaf(bf16_bits_to_f32(qrow[d]), bf16_bits_to_f32(krow[d]), s);
-      const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c, -p.part_ml[slot0 + r].x * p.c));
+      const float pe = fmaxf(__builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c, -p.part_ml[slot0 + r].x * p.c)), kTiny);
       for (int d = 0; d < 128; ++d) {
         const uint16_t w = reinterpret_cast<const uint16_t*>(vrow)[d];
         if ((w & 0x7f80u) == 0x7f80u) p.part_o[(slot0 + r) * 128 + d] += pe * bf16_bits_to_f32(w);
@@ -159,37 +159,35 @@ __device__ __forceinline__ void add_odd_values(const BatchAttnParams& p, int kvh
 // P goes into the product as TWO bf16 numbers, bf16(p) and bf16(p - bf16(p)): 2^-17 of p is lost instead of 2^-9.  Rounded once, as the prefill and
 // decode kernels do it, the result's error against 64 bits is 0.0021 - 0.0027 of it, with two terms 0.0017, which is its own rounding; the second
 // product reuses the V fragments, and a step that waits for the prefix's bytes has the matrix pipe free.
+template <int WR, int WK>
+struct Shape {
+  static constexpr int NT = 64 * WR * WK, KB = WK == 1 ? 2 : 1, TILE = 32 * WK * KB, PT = TILE * 16 / NT;   // PT: 16-B pieces a thread stages of K and of V
+};
+struct Rows {                      // what a lane keeps of its row (both halves of a wave: the same row, other keys)
+  f32x16_t o[4];                   // [d / 32], unscaled
+  float m, l;
+};
+struct Shared {                    // LDS besides the tile
+  unsigned long long holes[2][4];  // by parity of the tile: its rows without a page
+  int odd;                         // a value that is not finite was met
+};
+
 template <int WR, int WK, bool kPaged>
-__device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int kvh, int b, int64_t row0, int64_t row_end, int k0, int k1,
-                                                 int part, unsigned char* lds, float* lds_ml, unsigned long long* hole_keys, int* odd_seen) {
-  constexpr bool kAhead = !kPaged || WR > 1;                   // (with 64 registers a thread in flight the paged form of the narrow one would spill)
-  constexpr int NT = 64 * WR * WK, PT = kTile * 16 / NT, KB = 2 / WK;
+__device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int b, int64_t r, bool row_live, bool wave_live, const bf16x8_t (&qf)[8], int k0,
+                                          int k1, unsigned char* lds, Shared& sh, Rows& st) {
+  using S = Shape<WR, WK>;
+  constexpr int NT = S::NT, PT = S::PT, KB = S::KB, TILE = S::TILE;
+  constexpr bool kAhead = !kPaged || PT < 8;                   // (with 64 registers a thread in flight the paged form would spill)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, l31 = lane & 31;
-  const int wr = wave % WR, wk = wave / WR;
-  const int64_t r = row0 + wr * 32 + l31;
-  const bool row_live = r < row_end;
-  const bool wave_live = row0 + wr * 32 < row_end;
+  const int wk = wave / WR;
   unsigned char* kl = lds;
-  unsigned char* vl = lds + kTile * 256;
-  bf16x8_t qf[8];
+  unsigned char* vl = lds + TILE * 256;
   int limit = INT32_MAX;                                       // last visible key of this lane's row
   int seen_by_all = INT32_MAX;                                 // keys below this are visible to every row of the sequence
-  {
-    const int64_t rr = row_live ? r : row0;
-    const int64_t bt = rr / p.G;
-    const int g = (int)(rr - bt * p.G);
-    const uint4* src = p.q + ((bt * p.hq) + (int64_t)kvh * p.G + g) * 16;
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (row_live) x = src[kk * 2 + hi];
-      qf[kk] = __builtin_bit_cast(bf16x8_t, x);
-    }
-    if (kPaged) {
-      const int stored = min(p.pg.seq_len[b], kMaxKeys);      // (a table has no more rows)
-      seen_by_all = stored + 1;
-      limit = stored + (int)(bt - (int64_t)b * p.t_max);
-    }
+  if (kPaged) {
+    const int stored = min(p.pg.seq_len[b], kMaxKeys);        // (a table has no more rows)
+    seen_by_all = stored + 1;
+    limit = stored + (row_live ? (int)(r / p.G - (int64_t)b * p.t_max) : 0);
   }
   const uint4* kbase = kPaged ? p.k_pages : p.k_pre + (int64_t)kvh * p.pre_hs16;
   const uint4* vbase = kPaged ? p.v_pages : p.v_pre + (int64_t)kvh * p.pre_hs16;
@@ -200,7 +198,7 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
     if (!kPaged) {
       const uint4* kt = kbase + (int64_t)t0 * 16;              // a tile of the prefix is 16 KB in a row
       const uint4* vt = vbase + (int64_t)t0 * 16;
-      if (t0 + kTile <= k1) {
+      if (t0 + TILE <= k1) {
 #pragma unroll
         for (int i = 0; i < PT; ++i) { kx[i] = kt[tid + i * NT]; vx[i] = vt[tid + i * NT]; }
       } else {
@@ -225,52 +223,56 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
       }
     }
   };
-  int koff[8];
-#pragma unroll
-  for (int kk = 0; kk < 8; ++kk) koff[kk] = l31 * 256 + (((kk * 2 + hi) ^ (l31 & 15)) << 4);
+  const int koff = l31 * 256 + ((hi ^ (l31 & 15)) << 4);       // fragment kk of the lane's key: slot (2 kk + hi) ^ (key % 16)
   const int voff = (((lane & 15) >> 2) << 6) + (((lane >> 4) & 1) << 5) + ((lane & 3) << 3) + (hi << 10);
-  f32x16_t o[4];
-#pragma unroll
-  for (int db = 0; db < 4; ++db) o[db] = (f32x16_t){0};
-  float m_run = -1e30f, l_run = 0.f;
-  if (tid < 2) hole_keys[tid] = 0;                             // by parity of the tile: its rows without a page
-  if (tid == 0) *odd_seen = 0;                                 // set when the range holds a value that is not finite
+  f32x16_t (&o)[4] = st.o;
+  float m_run = st.m, l_run = st.l;
   int par = 0;
   if (kAhead && k0 < k1) load(k0);
-  for (int t0 = k0; t0 < k1; t0 += kTile, par ^= 1) {
+  for (int t0 = k0; t0 < k1; t0 += TILE, par ^= 1) {
     if (!kAhead) load(t0);
     __syncthreads();                                           // everyone has read the previous tile
-    const bool masked = kPaged && t0 + kTile > seen_by_all;    // some row of the sequence does not see some key of this tile
+    const bool masked = kPaged && t0 + TILE > seen_by_all;    // some row of the sequence does not see some key of this tile
+    u16x2_t top = {0, 0};
+#pragma unroll
+    for (int i = 0; i < PT; ++i) top = __builtin_elementwise_max(top, magnitude(vx[i]));
+    if (is_odd(top)) {
+#pragma unroll
+      for (int i = 0; i < PT; ++i) make_finite(vx[i]);
+      sh.odd = 1;
+    }
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
       const int row = srow + i * (NT / 16);
-      if (kPaged && ((holes >> i) & 1) && slot16 == 0) atomicOr(&hole_keys[par], 1ull << row);
-      if (has_odd(vx[i])) { make_finite(vx[i]); *odd_seen = 1; }
+      if (kPaged && ((holes >> i) & 1) && slot16 == 0) atomicOr(&sh.holes[par][row >> 6], 1ull << (row & 63));
       *reinterpret_cast<uint4*>(kl + row * 256 + ((slot16 ^ (row & 15)) << 4)) = kx[i];
       *reinterpret_cast<uint4*>(vl + (((row >> 2) * 4 + (slot16 >> 2)) << 8) + ((row & 3) << 6) + ((slot16 & 3) << 4)) = vx[i];
     }
     __syncthreads();
-    const unsigned long long hole_bits = kPaged ? hole_keys[par] : 0;
-    if (kPaged && tid == 0) hole_keys[par ^ 1] = 0;            // last read before the barrier above, next written behind the next one
-    if (kAhead && t0 + kTile < k1) load(t0 + kTile);
+    const int word = WK >= 2 ? wk >> 1 : 0;                    // this wave's keys lie in one 64-key word of the mask
+    const unsigned long long hole_bits = kPaged ? sh.holes[par][word] : 0;
+    if (kPaged && tid < 4) sh.holes[par ^ 1][tid] = 0;         // last read before the barrier above, next written behind the next one
+    if (kAhead && t0 + TILE < k1) load(t0 + TILE);
     if (!wave_live) continue;
     f32x16_t s[KB];
 #pragma unroll
     for (int k = 0; k < KB; ++k) {
-      const int kb = WK == 2 ? wk : k;
+      const int kb = WK >= 2 ? wk : k;
       s[k] = (f32x16_t){0};
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
-        s[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_read_b128(kl, kb * 32 * 256 + koff[kk]), qf[kk], s[k], 0, 0, 0);
+      for (int kk = 0; kk < 8; ++kk) {
+        if (PT >= 8 && kk == 4) __builtin_amdgcn_sched_barrier(0);               // (half of the K fragments at a time: registers)
+        s[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_read_b128(kl, kb * 32 * 256 + (koff ^ (kk << 5))), qf[kk], s[k], 0, 0, 0);
+      }
     }
     __builtin_amdgcn_sched_barrier(0);                         // (keeps hipcc from holding K, V and the next tile in registers at once)
-    if (t0 + kTile > k1 || masked || hole_bits) {
+    if (t0 + TILE > k1 || masked || hole_bits) {
       const int last = (limit < k1 ? limit : k1 - 1) - t0 - 4 * hi;              // last visible row of the tile, seen from this lane's rows
       const unsigned long long here = ~hole_bits >> (4 * hi);
 #pragma unroll
       for (int k = 0; k < KB; ++k) {
-        const int kb = WK == 2 ? wk : k;
-        const unsigned have = (unsigned)(here >> (kb * 32));
+        const int kb = WK >= 2 ? wk : k;
+        const unsigned have = (unsigned)(here >> ((kb & 1) * 32));
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int row = (e & 3) + 8 * (e >> 2);
@@ -298,7 +300,7 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
     float rs = 0.f;
 #pragma unroll
     for (int k = 0; k < KB; ++k) {
-      const int kb = WK == 2 ? wk : k;
+      const int kb = WK >= 2 ? wk : k;
       bf16x8_t pf[2], pr[2];
 #pragma unroll
       for (int cc = 0; cc < 2; ++cc)
@@ -311,7 +313,7 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
         }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int cc = 0; cc < 2; ++cc)
+      for (int cc = 0; cc < 2; ++cc) {
 #pragma unroll
         for (int db = 0; db < 4; ++db) {
           const int off = voff + (((kb * 8 + cc * 4) * 4 + db) << 8);
@@ -321,9 +323,95 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
           o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), pf[cc], o[db], 0, 0, 0);
           o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), pr[cc], o[db], 0, 0, 0);
         }
+      }
     }
     l_run += xhalf_sum(rs);
   }
+  st.m = m_run; st.l = l_run;
+}
+
+// Q fragments of the lane's row, an empty running state and cleared flags (the first barrier of walk_keys orders the flags)
+__device__ __forceinline__ void begin_rows(const BatchAttnParams& p, int kvh, int64_t r, bool row_live, bf16x8_t (&qf)[8], Shared& sh, Rows& st) {
+  const int tid = threadIdx.x, hi = (tid >> 5) & 1;
+  const int64_t bt = row_live ? r / p.G : 0;
+  const uint4* src = p.q + ((bt * p.hq) + (int64_t)kvh * p.G + (row_live ? (int)(r - bt * p.G) : 0)) * 16;
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) {
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (row_live) x = src[kk * 2 + hi];
+    qf[kk] = __builtin_bit_cast(bf16x8_t, x);
+  }
+#pragma unroll
+  for (int db = 0; db < 4; ++db) st.o[db] = (f32x16_t){0};
+  st.m = -1e30f; st.l = 0.f;
+  if (tid < 8) sh.holes[tid >> 2][tid & 3] = 0;
+  if (tid == 0) sh.odd = 0;
+}
+
+// Joining the WK waves that took the keys of the same 32 rows: every wave lays its rows out in LDS, scaled to the rows' common maximum (the tiles
+// are read by then); joined() adds them up.  kJoinRow: 128 + 4 floats, so that the rows start on different banks.
+constexpr int kJoinRow = 132;
+template <int WK> constexpr int join_bytes() { return WK * 32 * kJoinRow * 4; }
+template <int WK>
+__device__ __forceinline__ void lay_out_rows(const Rows& st, float c, bool row_live, float* obuf, float* lds_m, float* lds_l) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hi = lane >> 5, l31 = lane & 31;
+  if (hi == 0) lds_m[wave * 32 + l31] = st.m;
+  __syncthreads();
+  float M = lds_m[l31];
+#pragma unroll
+  for (int w = 1; w < WK; ++w) M = fmaxf(M, lds_m[w * 32 + l31]);
+  const float a = __builtin_amdgcn_exp2f((st.m - M) * c);
+  if (hi == 0) lds_l[wave * 32 + l31] = st.l * a;
+  if (row_live) {
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        *reinterpret_cast<float4*>(obuf + (wave * 32 + l31) * kJoinRow + db * 32 + 8 * q4 + 4 * hi) =
+            make_float4(st.o[db][q4 * 4 + 0] * a, st.o[db][q4 * 4 + 1] * a, st.o[db][q4 * 4 + 2] * a, st.o[db][q4 * 4 + 3] * a);
+  }
+  __syncthreads();
+}
+template <int WK>
+__device__ __forceinline__ float4 joined(const float* obuf, const float* lds_m, const float* lds_l, int row, int d4, float& m, float& l) {
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  m = lds_m[row]; l = 0.f;
+#pragma unroll
+  for (int w = 0; w < WK; ++w) {
+    const float4 v = *reinterpret_cast<const float4*>(obuf + (w * 32 + row) * kJoinRow + d4);
+    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    m = fmaxf(m, lds_m[w * 32 + row]); l += lds_l[w * 32 + row];
+  }
+  return acc;
+}
+
+// one key range of one row block: partial results of its rows into part `part`
+template <int WR, int WK, bool kPaged>
+__device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int kvh, int b, int64_t row0, int64_t row_end, int k0, int k1, int part,
+                                                 unsigned char* lds, float* lds_ml, Shared& sh) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, l31 = lane & 31;
+  const int wr = wave % WR, wk = wave / WR;
+  const int64_t r = row0 + wr * 32 + l31;
+  const bool row_live = r < row_end, wave_live = row0 + wr * 32 < row_end;
+  bf16x8_t qf[8];
+  Rows st;
+  begin_rows(p, kvh, r, row_live, qf, sh, st);
+  walk_keys<WR, WK, kPaged>(p, kvh, b, r, row_live, wave_live, qf, k0, k1, lds, sh, st);
+  const int64_t slot0 = ((int64_t)kvh * (p.ns + p.ns2) + part) * p.R;
+  if (WR == 1) {
+    float* obuf = reinterpret_cast<float*>(lds);
+    lay_out_rows<WK>(st, p.c, row_live, obuf, lds_ml, lds_ml + WK * 32);
+    const int rows = (int)(row_end - row0 < 32 ? row_end - row0 : 32);
+    for (int i = tid; i < rows * 32; i += 64 * WK) {
+      const int row = i >> 5, d4 = (i & 31) * 4;
+      float m, l;
+      const float4 acc = joined<WK>(obuf, lds_ml, lds_ml + WK * 32, row, d4, m, l);
+      *reinterpret_cast<float4*>(p.part_o + (slot0 + row0 + row) * 128 + d4) = acc;
+      if (d4 == 0) p.part_ml[slot0 + row0 + row] = make_float2(m, l);
+    }
+  } else {
+  f32x16_t (&o)[4] = st.o;
+  float m_run = st.m, l_run = st.l;
   if (WK == 2) {                                               // join the two key halves of a row (the tile's LDS is free)
     __syncthreads();
     float* obuf = reinterpret_cast<float*>(lds);               // [WR][32 rows][128]
@@ -349,7 +437,6 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
       for (int e = 0; e < 16; ++e) o[db][e] = o[db][e] * a0 + obuf[(wr * 32 + l31) * 128 + db * 32 + 8 * (e >> 2) + 4 * hi + (e & 3)] * a1;
     }
   }
-  const int64_t slot0 = ((int64_t)kvh * (p.ns + p.ns2) + part) * p.R;
   if (row_live && wk == 0) {
     if (hi == 0) p.part_ml[slot0 + r] = make_float2(m_run, l_run);
 #pragma unroll
@@ -359,29 +446,40 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
         *reinterpret_cast<float4*>(p.part_o + (slot0 + r) * 128 + db * 32 + 8 * q4 + 4 * hi) =
             make_float4(o[db][q4 * 4 + 0], o[db][q4 * 4 + 1], o[db][q4 * 4 + 2], o[db][q4 * 4 + 3]);
   }
-  if (k0 < k1 && *odd_seen) {                                  // (read behind the loop's barriers)
+  }
+  if (k0 < k1 && sh.odd) {                                  // (read behind the loop's barriers)
     __threadfence_block();
     __syncthreads();
     add_odd_values<kPaged>(p, kvh, b, row0, row0 + 32 * WR < row_end ? row0 + 32 * WR : row_end, k0, k1, slot0);
   }
 }
 
-// range `split` of n keys cut into `ns` ranges of whole tiles (the last ones may be empty: k0 >= k1)
+// range `split` of n keys cut into `ns` ranges of whole 64-key tiles (the last ones may be empty: k0 >= k1)
 __device__ __forceinline__ void key_range(int n, int ns, int split, int& k0, int& k1) {
-  const int tiles = (n + kTile - 1) / kTile, per = (tiles + ns - 1) / ns;
-  const int64_t at = (int64_t)split * per * kTile, to = at + (int64_t)per * kTile;
+  const int tiles = (n + 63) / 64, per = (tiles + ns - 1) / ns;
+  const int64_t at = (int64_t)split * per * 64, to = at + (int64_t)per * 64;
   k0 = (int)(at < n ? at : n);
   k1 = (int)(to < n ? to : n);
+}
+
+// rows of sequence b with this step's, as far as its table goes
+__device__ __forceinline__ int stored_rows(const Pages& pg, int b, int n_new) {
+  const int64_t len = (int64_t)pg.seq_len[b] + n_new, cap = (int64_t)pg.max_pages * pg.page_size;
+  return (int)(len < 0 ? 0 : (len > cap ? cap : len));
 }
 
 // Grid: first the workgroups of the pages (short), then those of the prefix.  The row blocks that read the same keys are 8 workgroups apart, so that
 // they run on the same XCD (workgroups go to the 8 XCDs in turn) and share its L2.
 template <int WR, int WK>
+constexpr int lds_of() {
+  constexpr int tiles = 2 * Shape<WR, WK>::TILE * 256;
+  return WR == 1 && join_bytes<WK>() > tiles ? join_bytes<WK>() : tiles;
+}
+template <int WR, int WK>
 __global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnParams p) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * kTile * 256];
-  __shared__ float lds_ml[WR * 64];
-  __shared__ unsigned long long hole_keys[2];
-  __shared__ int odd_seen;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];          // lds_of<WR, WK>()
+  __shared__ float lds_ml[WR == 1 ? WK * 64 : WR * 64];
+  __shared__ Shared sh;
   if (blockIdx.x >= p.page_wgs) {
     const unsigned w = blockIdx.x - p.page_wgs, turn = 8u * p.nrb;
     const int item = (int)(w / turn) * 8 + (int)(w % 8), rb = (int)(w % turn) / 8;
@@ -389,7 +487,7 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnPa
     const int kvh = item / p.ns, split = item - kvh * p.ns;
     int k0, k1;
     key_range((int)p.P, p.ns, split, k0, k1);
-    batch_attn_range<WR, WK, false>(p, kvh, 0, (int64_t)rb * 32 * WR, p.R, k0, k1, split, lds, lds_ml, hole_keys, &odd_seen);
+    batch_attn_range<WR, WK, false>(p, kvh, 0, (int64_t)rb * 32 * WR, p.R, k0, k1, split, lds, lds_ml, sh);
     return;
   }
   const int w = (int)blockIdx.x;
@@ -397,55 +495,166 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnPa
   const int kvh = hb % p.hkv, b = hb / p.hkv;
   const int n_new = rows_new(p.pg, b, p.t_max);
   if (n_new == 0) return;                                      // nothing of this sequence is written
-  int64_t len = (int64_t)p.pg.seq_len[b] + n_new;
-  if (len > (int64_t)p.pg.max_pages * p.pg.page_size) len = (int64_t)p.pg.max_pages * p.pg.page_size;
-  if (len < 0) len = 0;
   int k0, k1;
-  key_range((int)len, p.ns2, split, k0, k1);
+  key_range(stored_rows(p.pg, b, n_new), p.ns2, split, k0, k1);
   const int64_t seq_row0 = (int64_t)b * p.t_max * p.G, row0 = seq_row0 + (int64_t)rb * 32 * WR, row_end = seq_row0 + (int64_t)n_new * p.G;
   if (row0 >= row_end) return;
-  batch_attn_range<WR, WK, true>(p, kvh, b, row0, row_end, k0, k1, p.ns + split, lds, lds_ml, hole_keys, &odd_seen);
+  batch_attn_range<WR, WK, true>(p, kvh, b, row0, row_end, k0, k1, p.ns + split, lds, lds_ml, sh);
 }
 
-// one workgroup per row: 8 groups of 32 lanes walk the partial results (16 B per lane), then join through LDS
+// Few keys: ONE launch.  A workgroup of 8 waves walks the prefix and then the pages for the (at most 32) rows of one sequence and kv head, 256
+// keys at a time, and joins its waves itself; the prefix is read again for every sequence, from L2.
+constexpr int kDirectWaves = 8, kDirectLds = join_bytes<kDirectWaves>();
+static_assert(kDirectLds >= 2 * Shape<1, kDirectWaves>::TILE * 256, "the tiles fit as well");
+
+__global__ __launch_bounds__(64 * kDirectWaves, 2) void batch_attn_direct_kernel(BatchAttnParams p) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  __shared__ float lds_m[kDirectWaves * 32], lds_l[kDirectWaves * 32];
+  __shared__ Shared sh;
+  const int tid = threadIdx.x, l31 = tid & 31;
+  const int kvh = (int)(blockIdx.x % p.hkv), b = (int)(blockIdx.x / p.hkv);
+  const int n_new = rows_new(p.pg, b, p.t_max);
+  if (n_new == 0) return;
+  const int len = stored_rows(p.pg, b, n_new);
+  const int64_t row0 = (int64_t)b * p.t_max * p.G, row_end = row0 + (int64_t)n_new * p.G, r = row0 + l31;
+  const bool row_live = r < row_end;
+  bf16x8_t qf[8];
+  Rows st;
+  begin_rows(p, kvh, r, row_live, qf, sh, st);
+  walk_keys<1, kDirectWaves, false>(p, kvh, b, r, row_live, true, qf, 0, (int)p.P, lds, sh, st);
+  walk_keys<1, kDirectWaves, true>(p, kvh, b, r, row_live, true, qf, 0, len, lds, sh, st);
+  float* obuf = reinterpret_cast<float*>(lds);
+  lay_out_rows<kDirectWaves>(st, p.c, row_live, obuf, lds_m, lds_l);
+  const int64_t slot0 = (int64_t)kvh * p.R;
+  const bool odd = sh.odd != 0;
+  for (int pass = 0; pass < 2; ++pass) {                       // second pass only behind add_odd_values, from where it left the rows
+    for (int i = tid; i < (int)(row_end - row0) * 32; i += 64 * kDirectWaves) {
+      const int row = i >> 5, d4 = (i & 31) * 4;
+      float m, l;
+      float4 acc = joined<kDirectWaves>(obuf, lds_m, lds_l, row, d4, m, l);
+      if (pass) acc = *reinterpret_cast<const float4*>(p.part_o + (slot0 + row0 + row) * 128 + d4);
+      if (pass == 0 && odd) {
+        *reinterpret_cast<float4*>(p.part_o + (slot0 + row0 + row) * 128 + d4) = acc;
+        if (d4 == 0) p.part_ml[slot0 + row0 + row] = make_float2(m, l);
+        continue;
+      }
+      uint2 y = make_uint2(0, 0);                              // a row that sees no key is zero
+      if (l != 0.f) {
+        const float inv = 1.0f / l;
+        y.x = (unsigned)f32_to_bf16_bits(acc.x * inv) | ((unsigned)f32_to_bf16_bits(acc.y * inv) << 16);
+        y.y = (unsigned)f32_to_bf16_bits(acc.z * inv) | ((unsigned)f32_to_bf16_bits(acc.w * inv) << 16);
+      }
+      const int64_t bt = (row0 + row) / p.G;
+      const int g = (int)(row0 + row - bt * p.G);
+      *reinterpret_cast<uint2*>(p.out + ((bt * p.hq) + (int64_t)kvh * p.G + g) * 128 + d4) = y;
+    }
+    if (!odd) break;
+    if (pass == 0) {
+      __threadfence_block();
+      __syncthreads();
+      add_odd_values<false>(p, kvh, b, row0, row_end, 0, (int)p.P, slot0);
+      add_odd_values<true>(p, kvh, b, row0, row_end, 0, len, slot0);             // (a row's thread is the same in both)
+      __threadfence_block();
+      __syncthreads();
+    }
+  }
+}
+
+// Joins the partial results of a row.  kWide: a workgroup per row, 8 groups of 32 lanes walk the parts (16 B of the row per lane), the
+// weights are found once, in LDS, so that no load waits for another; otherwise (few parts, many rows) a wave per row.
+constexpr int kMaxParts = 1280;
+template <bool kWide>
 __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
-  __shared__ float4 lds_o[8][32];
+  constexpr int GROUPS = kWide ? 8 : 2;
+  __shared__ float4 lds_o[4][32];
   __shared__ float red[8];
-  const int kvh = blockIdx.x % p.hkv;
-  const int64_t r = blockIdx.x / p.hkv, bt = r / p.G;
+  __shared__ float lds_a[kWide ? kMaxParts : 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lane32 = tid & 31, grp = kWide ? tid >> 5 : (tid >> 5) & 1;
+  const int64_t w = kWide ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  if (w >= p.R * p.hkv) return;                                // (whole waves)
+  const int kvh = (int)(w / p.R);
+  const int64_t r = w - (int64_t)kvh * p.R, bt = r / p.G;
   const int g = (int)(r - bt * p.G), b = (int)(bt / p.t_max), t = (int)(bt % p.t_max);
   if (t >= rows_new(p.pg, b, p.t_max)) return;                 // rows behind a sequence's last token stay as they are
-  const int np = p.ns + p.ns2, tid = threadIdx.x, lane32 = tid & 31, grp = tid >> 5;
+  const int np = p.ns + p.ns2;
   const float2* ml = p.part_ml + (int64_t)kvh * np * p.R + r;
-  const float* po = p.part_o + ((int64_t)kvh * np * p.R + r) * 128;
-  float M = -1e30f;
-  for (int i = tid; i < np; i += 256) M = fmaxf(M, ml[(int64_t)i * p.R].x);
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
-  if ((tid & 63) == 0) red[tid >> 6] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  __syncthreads();
+  const float* po = p.part_o + ((int64_t)kvh * np * p.R + r) * 128 + lane32 * 4;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
-  for (int i = grp; i < np; i += 8) {
-    const float2 x = ml[(int64_t)i * p.R];
-    if (x.y == 0.f) continue;                                  // an empty range left no o behind
-    const float a = __builtin_amdgcn_exp2f((x.x - M) * p.c);
-    const float4 v = *reinterpret_cast<const float4*>(po + (int64_t)i * p.R * 128 + lane32 * 4);
-    l = __builtin_fmaf(x.y, a, l);
-    acc.x = __builtin_fmaf(v.x, a, acc.x); acc.y = __builtin_fmaf(v.y, a, acc.y);
-    acc.z = __builtin_fmaf(v.z, a, acc.z); acc.w = __builtin_fmaf(v.w, a, acc.w);
-  }
-  lds_o[grp][lane32] = acc;
-  if (lane32 == 0) red[grp] = l;
-  __syncthreads();
-  if (grp) return;
-  l = ((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]));
+  if (kWide) {
+    float M = -1e30f;
+    for (int i = tid; i < np; i += 256) M = fmaxf(M, ml[(int64_t)i * p.R].x);
 #pragma unroll
-  for (int k = 1; k < 8; ++k) {
-    const float4 v = lds_o[k][lane32];
-    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+    if (lane == 0) red[wave] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    for (int i = tid; i < np; i += 256) {
+      const float2 x = ml[(int64_t)i * p.R];
+      const float a = __builtin_amdgcn_exp2f((x.x - M) * p.c);
+      lds_a[i] = x.y == 0.f ? 0.f : fmaxf(a, kTiny);           // an empty range left no o behind
+      l = __builtin_fmaf(x.y, a, l);
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
+    if (lane == 0) red[4 + wave] = l;
+    __syncthreads();
+    l = (red[4] + red[5]) + (red[6] + red[7]);
+    for (int i0 = grp; i0 < np; i0 += GROUPS * 4) {            // four parts of a group in flight
+      float4 v[4];
+      float a[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + k * GROUPS;
+        a[k] = i < np ? lds_a[i] : 0.f;
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (a[k] != 0.f) v[k] = *reinterpret_cast<const float4*>(po + (int64_t)i * p.R * 128);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        acc.x = __builtin_fmaf(v[k].x, a[k], acc.x); acc.y = __builtin_fmaf(v[k].y, a[k], acc.y);
+        acc.z = __builtin_fmaf(v[k].z, a[k], acc.z); acc.w = __builtin_fmaf(v[k].w, a[k], acc.w);
+      }
+    }
+  } else {                                                     // np <= 64: lane i holds part i
+    const float2 x = lane < np ? ml[(int64_t)lane * p.R] : make_float2(-1e30f, 0.f);
+    float M = x.x;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+    float a = __builtin_amdgcn_exp2f((x.x - M) * p.c);
+    l = x.y * a;
+    a = x.y == 0.f ? 0.f : fmaxf(a, kTiny);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
+    for (int i0 = 0; i0 < np; i0 += GROUPS * 4) {
+      float4 v[4];
+      float ak[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + k * GROUPS + grp;
+        ak[k] = __shfl(a, i & 63, 64);
+        if (i >= np) ak[k] = 0.f;
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (ak[k] != 0.f) v[k] = *reinterpret_cast<const float4*>(po + (int64_t)i * p.R * 128);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        acc.x = __builtin_fmaf(v[k].x, ak[k], acc.x); acc.y = __builtin_fmaf(v[k].y, ak[k], acc.y);
+        acc.z = __builtin_fmaf(v[k].z, ak[k], acc.z); acc.w = __builtin_fmaf(v[k].w, ak[k], acc.w);
+      }
+    }
+  }
+  acc.x += __shfl_xor(acc.x, 32, 64); acc.y += __shfl_xor(acc.y, 32, 64);
+  acc.z += __shfl_xor(acc.z, 32, 64); acc.w += __shfl_xor(acc.w, 32, 64);
+  if (kWide) {
+    if (lane < 32) lds_o[wave][lane32] = acc;
+    __syncthreads();
+    if (tid >= 32) return;
+    const float4 v1 = lds_o[1][lane32], v2 = lds_o[2][lane32], v3 = lds_o[3][lane32];
+    acc.x = (acc.x + v1.x) + (v2.x + v3.x); acc.y = (acc.y + v1.y) + (v2.y + v3.y);
+    acc.z = (acc.z + v1.z) + (v2.z + v3.z); acc.w = (acc.w + v1.w) + (v2.w + v3.w);
+  } else if (lane >= 32) {
+    return;
   }
   uint2 y = make_uint2(0, 0);                                  // a row that sees no key is zero
   if (l != 0.f) {
@@ -456,15 +665,22 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
   *reinterpret_cast<uint2*>(p.out + ((bt * p.hq) + (int64_t)kvh * p.G + g) * 128 + lane32 * 4) = y;
 }
 
-struct Plan { int wr, ns, nrb, ns2, nrb2; int64_t R; };
+struct Plan { bool direct; int wr, ns, nrb, ns2, nrb2; int64_t R; };
+
+constexpr int64_t kDirectKeys = 1536;
 
 // Row blocks as wide as the batch's rows (up to 256), key ranges so many that every CU is busy once.
 Plan make_plan(const qp_ctx* ctx, int batch, int t_max, int64_t P, int64_t suffix_cap, int hq, int hkv) {
   Plan pl;
   const int G = hq / hkv;
   pl.R = (int64_t)batch * t_max * G;
+  pl.direct = t_max * G <= 32 && (int64_t)hkv * batch <= ctx->cus && P + suffix_cap <= kDirectKeys;
+  if (pl.direct) {
+    pl.wr = 1; pl.ns = 0; pl.ns2 = 1; pl.nrb = pl.nrb2 = 1;
+    return pl;
+  }
   pl.wr = pl.R <= 32 ? 1 : (pl.R <= 64 ? 2 : (pl.R <= 128 ? 4 : 8));
-  const int rows = 32 * pl.wr, per_cu = pl.wr == 1 ? 4 : (pl.wr == 8 ? 1 : 2);     // resident workgroups (registers: two waves per SIMD)
+  const int rows = 32 * pl.wr, per_cu = pl.wr == 8 ? 1 : 2;     // resident workgroups (registers: two waves per SIMD)
   pl.nrb = (int)((pl.R + rows - 1) / rows);
   pl.nrb2 = (int)(((int64_t)t_max * G + rows - 1) / rows);
   const int64_t slots = (int64_t)per_cu * ctx->cus, seqs = (int64_t)hkv * batch * pl.nrb2;
@@ -474,8 +690,9 @@ Plan make_plan(const qp_ctx* ctx, int batch, int t_max, int64_t P, int64_t suffi
   pl.ns2 = (int)(ns2 < 1 ? 1 : (ns2 > 64 ? 64 : ns2));
   const int64_t page_wgs = seqs * pl.ns2, left = page_wgs * 2 < slots ? slots - page_wgs : slots;
   int64_t ns = left / ((int64_t)hkv * pl.nrb);
-  const int64_t most = (P + 2 * kTile - 1) / (2 * kTile);
+  const int64_t least = pl.wr == 1 ? 128 : 64, most = (P + least - 1) / least;   // a tile per range at least
   if (ns < 1) ns = 1;
+  if (ns > kMaxParts - 64) ns = kMaxParts - 64;
   pl.ns = (int)(ns < most ? ns : most);
   return pl;
 }
@@ -487,6 +704,18 @@ Pages pages_of(const int32_t* table, const int32_t* seq_len, const int32_t* n_ne
   pg.table = table; pg.seq_len = seq_len; pg.n_new = n_new;
   pg.max_pages = max_pages; pg.n_pages = n_pages; pg.page_size = page_size; pg.page_stride16 = page_stride / 8;
   return pg;
+}
+
+template <int WR, int WK>
+int launch_ranges(const BatchAttnParams& p, unsigned grid, hipStream_t s) {
+  constexpr int bytes = lds_of<WR, WK>();
+  if (bytes > 60 * 1024) {
+    static std::atomic<unsigned long long> opted{0};
+    int rc = qp_opt_in_lds(opted, (const void*)batch_attn_kernel<WR, WK>, bytes, "batch_attn");
+    if (rc) return rc;
+  }
+  batch_attn_kernel<WR, WK><<<grid, 64 * WR * WK, bytes, s>>>(p);
+  return qp_check_launch("batch_attn");
 }
 
 }  // namespace
@@ -522,15 +751,23 @@ int qp_launch_batch_attn(const qp_ctx* ctx, const void* q, const void* k_prefix,
   p.page_wgs = (unsigned)((int64_t)hkv * batch * pl.nrb2 * pl.ns2);
   p.part_ml = (float2*)workspace;
   p.part_o = (float*)((char*)workspace + ml_bytes(pl, hkv));
-  const unsigned grid = p.page_wgs + (unsigned)(((int64_t)hkv * pl.ns + 7) / 8 * 8 * pl.nrb);
-  switch (pl.wr) {
-    case 1: batch_attn_kernel<1, 2><<<grid, 128, 0, s>>>(p); break;
-    case 2: batch_attn_kernel<2, 2><<<grid, 256, 0, s>>>(p); break;
-    case 4: batch_attn_kernel<4, 1><<<grid, 256, 0, s>>>(p); break;
-    default: batch_attn_kernel<8, 1><<<grid, 512, 0, s>>>(p); break;
+  if (pl.direct) {
+    static std::atomic<unsigned long long> opted{0};
+    int rc = qp_opt_in_lds(opted, (const void*)batch_attn_direct_kernel, kDirectLds, "batch_attn_direct");
+    if (rc) return rc;
+    batch_attn_direct_kernel<<<(unsigned)(hkv * batch), 64 * kDirectWaves, kDirectLds, s>>>(p);
+    return qp_check_launch("batch_attn(direct)");
   }
-  int rc = qp_check_launch("batch_attn");
+  const unsigned grid = p.page_wgs + (unsigned)(((int64_t)hkv * pl.ns + 7) / 8 * 8 * pl.nrb);
+  int rc;
+  switch (pl.wr) {
+    case 1: rc = launch_ranges<1, 4>(p, grid, s); break;
+    case 2: rc = launch_ranges<2, 2>(p, grid, s); break;
+    case 4: rc = launch_ranges<4, 1>(p, grid, s); break;
+    default: rc = launch_ranges<8, 1>(p, grid, s); break;
+  }
   if (rc) return rc;
-  batch_combine_kernel<<<(unsigned)(pl.R * hkv), 256, 0, s>>>(p);
+  if (pl.ns + pl.ns2 > 32) batch_combine_kernel<true><<<(unsigned)(pl.R * hkv), 256, 0, s>>>(p);
+  else batch_combine_kernel<false><<<(unsigned)((pl.R * hkv + 3) / 4), 256, 0, s>>>(p);
   return qp_check_launch("batch_attn(combine)");
 }

@@ -22,8 +22,8 @@ struct VerifyParams {
   const float* probs; int64_t probs_seq_stride, probs_row_stride;
   const float* u;
   int batch, T, nc; int64_t V;
-  double inv_temp;
-  double* sum; double* rest; float* top; int* arg;             // [batch][T + 1][nc] (rest: [batch][nc])
+  double scale;                                                // log2(e) / temperature; 0: greedy
+  double *sum, *rest, *others; float* top; int* arg;           // [batch][T + 1][nc] (rest: [batch][nc], others: [batch][T])
   int* accepted; int64_t* tokens;
 };
 
@@ -37,22 +37,73 @@ __device__ __forceinline__ float logit(const VerifyParams& p, int64_t row, int64
   const float x = kF32 ? ((const float*)p.logits)[row + v] : bf16_bits_to_f32(((const uint16_t*)p.logits)[row + v]);
   return x == x ? x : -INFINITY;
 }
-__device__ __forceinline__ double weight(float x, float top, double inv_temp) {
-  return x == top ? 1.0 : exp(((double)x - (double)top) * inv_temp);
+// 2^y, y <= 0, in 64 bits: y = k + f with |f| <= 1/2 (k by adding 1.5 * 2^52, whose last bits then are k), the series of 2^f = e^(f ln 2) up to
+// f^11 (what is left out is (ln 2 / 2)^12 / 12! < 7e-15), k added to the exponent.  16 operations at the full rate of 64-bit arithmetic, where the
+// library's exp takes twice the time with its special cases; 0 below 2^-1020.
+__device__ __forceinline__ double exp2_neg(double y) {
+  constexpr double L = 0.693147180559945309417;                // ln 2
+  constexpr double c2 = L * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6, c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9,
+                   c10 = c9 * L / 10, c11 = c10 * L / 11;
+  constexpr double shift = 6755399441055744.0;                 // 1.5 * 2^52
+  const double in = fmax(y, -1021.0), t = in + shift, f = in - (t - shift);
+  double r = fma(c11, f, c10);
+  r = fma(r, f, c9); r = fma(r, f, c8); r = fma(r, f, c7); r = fma(r, f, c6); r = fma(r, f, c5); r = fma(r, f, c4); r = fma(r, f, c3); r = fma(r, f, c2);
+  r = fma(r, f, L); r = fma(r, f, 1.0);
+  const unsigned long long bits = __builtin_bit_cast(unsigned long long, r) + (__builtin_bit_cast(unsigned long long, t) << 52);
+  return y < -1020.0 ? 0.0 : __builtin_bit_cast(double, bits);
+}
+// weight of a logit against the row's maximum (above -infinity): 1 at the maximum, also an infinite one; 0 for -infinity
+__device__ __forceinline__ double weight(float x, float top, double scale) {
+  return exp2_neg(x == top ? 0.0 : ((double)x - (double)top) * scale);
 }
 __device__ __forceinline__ double wave_sum_f64(double v) {
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
   return v;
 }
-__device__ __forceinline__ double block_sum_f64(double v, double* red) {       // red: 4 doubles; all threads get the sum
+template <int kWaves = 4>
+__device__ __forceinline__ double block_sum_f64(double v, double* red) {       // red: a double per wave; all threads get the sum
   v = wave_sum_f64(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
+  double s = 0.0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) s += red[w];
+  return s;
 }
 
+// 16 logits of a chunk per thread: 16 B a load where the row lies on a 16-B boundary, one by one where it does not or ends.  place(i) = the i-th one's token
+template <bool kF32>
+struct Chunk {
+  static constexpr int W = kF32 ? 4 : 8;                       // logits in 16 B
+  float x[kPer];
+  bool wide;
+  __device__ __forceinline__ int place(int i) const { return wide ? ((i / W) * kThreads + (int)threadIdx.x) * W + i % W : i * kThreads + (int)threadIdx.x; }
+  __device__ __forceinline__ void load(const VerifyParams& p, int64_t row, int64_t v0) {
+    const char* at = (const char*)p.logits + (row + v0) * (kF32 ? 4 : 2);
+    wide = ((uintptr_t)at & 15) == 0;
+    if (wide && v0 + kChunk <= p.V) {
+#pragma unroll
+      for (int j = 0; j < kPer / W; ++j) {
+        const uint4 u = reinterpret_cast<const uint4*>(at)[j * kThreads + threadIdx.x];
+        const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (kF32) x[j * W + e] = __uint_as_float(w[e]);
+          else { x[j * W + 2 * e] = __uint_as_float(w[e] << 16); x[j * W + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+        }
+      }
+    } else {
+      wide = false;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) { const int64_t v = v0 + place(i); x[i] = v < p.V ? logit<kF32>(p, row, v) : -INFINITY; }
+    }
+  }
+};
+
+// What bounds it in a large batch is about half the logits' bytes and half the 64-bit exponentials: 32 x 5 rows of 152064 fp32 logits take 23 us, 14 us
+// with the 32-bit exponential instead.  More or fewer workgroups on a CU, or several chunks per workgroup with the next one's loads ahead, gained nothing.
 template <bool kF32>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyParams p) {
   __shared__ double red[4];
@@ -61,13 +112,14 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyParams p) 
   const int ch = blockIdx.x, t = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   if (t > drafts_of(p, b)) return;
   const int64_t row = (int64_t)b * p.seq_stride + (int64_t)t * p.row_stride, v0 = (int64_t)ch * kChunk;
-  float x[kPer], m = -INFINITY;
+  Chunk<kF32> c;
+  c.load(p, row, v0);
+  float m = -INFINITY;
   int arg = INT32_MAX;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int64_t v = v0 + tid + i * kThreads;
-    x[i] = v < p.V ? logit<kF32>(p, row, v) : -INFINITY;
-    if (x[i] > m) { m = x[i]; arg = (int)v; }
+  for (int i = 0; i < kPer; ++i) {                             // (a thread's places ascend; NaN is never chosen)
+    if (!(c.x[i] == c.x[i])) c.x[i] = -INFINITY;
+    if (c.x[i] > m) { m = c.x[i]; arg = (int)v0 + c.place(i); }
   }
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) {
@@ -81,13 +133,30 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyParams p) 
 #pragma unroll
   for (int w = 1; w < 4; ++w)
     if (red_m[w] > m || (red_m[w] == m && red_i[w] < arg)) { m = red_m[w]; arg = red_i[w]; }
+  const bool sums = p.scale != 0.0 && m != -INFINITY;
   double s = 0.0;
-  if (p.inv_temp != 0.0 && m != -INFINITY) {
+  if (sums) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (x[i] != -INFINITY) s += weight(x[i], m, p.inv_temp);
+    for (int i = 0; i < kPer; ++i) s += weight(c.x[i], m, p.scale);
   }
+  const double mine = s;
   s = block_sum_f64(s, red);
+  if (!p.probs && t < p.T && sums) {                           // a certain draft: its chunk's sum without it, which may be next to nothing of the whole
+    const int64_t draft = p.drafts[(int64_t)b * p.T + t];
+    if (draft >= v0 && draft < v0 + kChunk) {                  // (uniform)
+      double o = mine;
+      bool holds = false;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) holds |= v0 + c.place(i) == draft;
+      if (holds) {                                             // one thread sums again
+        o = 0.0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) o += v0 + c.place(i) == draft ? 0.0 : weight(c.x[i], m, p.scale);
+      }
+      o = block_sum_f64(o, red);
+      if (tid == 0) p.others[(int64_t)b * p.T + t] = o;
+    }
+  }
   if (tid == 0) {
     const int64_t at = ((int64_t)b * (p.T + 1) + t) * p.nc + ch;
     p.sum[at] = s; p.top[at] = m; p.arg[at] = arg;
@@ -104,14 +173,25 @@ __device__ Decision decide(const VerifyParams& p, int b, int n) {
   __shared__ double zs[kMaxDrafts + 1];
   __shared__ int args[kMaxDrafts + 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int t = wave; t <= n; t += kThreads / 64) {
+  for (int t = wave; t <= n; t += (int)blockDim.x / 64) {
     const int64_t at = ((int64_t)b * (p.T + 1) + t) * p.nc;
-    float m = -INFINITY;
+    // the draft's own numbers are on their way while the chunks are joined
+    const int64_t x = t < n ? p.drafts[(int64_t)b * p.T + t] : -1;
+    const bool inside = x >= 0 && x < p.V;
+    float lx = -INFINITY, qx = 1.f, u = 0.f;
+    if (inside && p.scale != 0.0) {
+      u = p.u[(int64_t)b * (p.T + 1) + t];
+      lx = logit<kF32>(p, (int64_t)b * p.seq_stride + (int64_t)t * p.row_stride, x);
+      if (p.probs) qx = p.probs[(int64_t)b * p.probs_seq_stride + (int64_t)t * p.probs_row_stride + x];
+    }
+    float m = -INFINITY, cm = -INFINITY;                       // cm, cs: of the lane's first chunk (mostly its only one)
+    double cs = 0.0;
     int arg = INT32_MAX;
     for (int c = lane; c < p.nc; c += 64) {
-      const float cm = p.top[at + c];
-      const int ca = p.arg[at + c];
-      if (cm > m || (cm == m && ca < arg)) { m = cm; arg = ca; }
+      const float om = p.top[at + c];
+      const int oa = p.arg[at + c];
+      if (c == lane) { cm = om; cs = p.sum[at + c]; }
+      if (om > m || (om == m && oa < arg)) { m = om; arg = oa; }
     }
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
@@ -119,28 +199,16 @@ __device__ Decision decide(const VerifyParams& p, int b, int n) {
       const int oa = __shfl_xor(arg, d, 64);
       if (om > m || (om == m && oa < arg)) { m = om; arg = oa; }
     }
-    double z = 0.0;
-    if (p.inv_temp != 0.0)
-      for (int c = lane; c < p.nc; c += 64) {
-        const float cm = p.top[at + c];
-        if (cm != -INFINITY) z += p.sum[at + c] * weight(cm, m, p.inv_temp);
-      }
-    z = wave_sum_f64(z);
+    double z = 0.0, px = 0.0;
+    if (p.scale != 0.0 && m != -INFINITY) {
+      z = cs * weight(cm, m, p.scale);
+      for (int c = lane + 64; c < p.nc; c += 64) z += p.sum[at + c] * weight(p.top[at + c], m, p.scale);
+      z = wave_sum_f64(z);
+      px = weight(lx, m, p.scale);
+    }
     if (lane == 0) {
-      bool stands = false;
-      if (t < n && m != -INFINITY) {
-        const int64_t x = p.drafts[(int64_t)b * p.T + t];
-        if (x >= 0 && x < p.V) {
-          if (p.inv_temp == 0.0) {
-            stands = x == arg;
-          } else {
-            const float lx = logit<kF32>(p, (int64_t)b * p.seq_stride + (int64_t)t * p.row_stride, x);
-            const double px = lx == -INFINITY ? 0.0 : weight(lx, m, p.inv_temp);
-            const double q = p.probs ? (double)p.probs[(int64_t)b * p.probs_seq_stride + (int64_t)t * p.probs_row_stride + x] : 1.0;
-            stands = (double)p.u[(int64_t)b * (p.T + 1) + t] * q * z < px;
-          }
-        }
-      }
+      bool stands = inside && m != -INFINITY;
+      if (stands) stands = p.scale == 0.0 ? x == arg : (double)u * (double)qx * z < px;
       ok[t] = stands; tops[t] = m; zs[t] = z; args[t] = arg;
     }
   }
@@ -154,14 +222,10 @@ __device__ Decision decide(const VerifyParams& p, int b, int n) {
 
 enum { FROM_ROW = 0, WITHOUT_DRAFT = 1, LESS_DRAFT = 2 };      // what the next token is drawn from: p, p without x, max(p - q, 0)
 
-// weight of token v in the draw, in units of the row's exp((x - max) / temperature)
-template <bool kF32>
-__device__ __forceinline__ double draw_weight(const VerifyParams& p, int64_t row, int64_t q_row, int64_t v, int kind, int64_t x, const Decision& d) {
-  if (v >= p.V || (kind == WITHOUT_DRAFT && v == x)) return 0.0;
-  const float l = logit<kF32>(p, row, v);
-  double w = l == -INFINITY ? 0.0 : weight(l, d.top, p.inv_temp);
-  if (kind == LESS_DRAFT) w = fmax(w - (double)p.probs[q_row + v] * d.z, 0.0);
-  return w;
+// weight of a token in the draw, in units of the row's exp((x - max) / temperature): l its logit, q the draft's probability of it
+__device__ __forceinline__ double draw_weight(float l, float q, int kind, const Decision& d, double scale) {
+  const double w = weight(l, d.top, scale);
+  return kind == LESS_DRAFT ? fmax(w - (double)q * d.z, 0.0) : w;
 }
 
 template <bool kF32>
@@ -172,107 +236,133 @@ __global__ __launch_bounds__(kThreads) void verify_rest_kernel(VerifyParams p) {
   const Decision d = decide<kF32>(p, b, n);
   if (d.a == n || d.top == -INFINITY) return;
   const int64_t row = (int64_t)b * p.seq_stride + (int64_t)d.a * p.row_stride, q_row = (int64_t)b * p.probs_seq_stride + (int64_t)d.a * p.probs_row_stride;
+  float l[kPer], q[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int64_t v = (int64_t)ch * kChunk + threadIdx.x + i * kThreads;
+    l[i] = v < p.V ? logit<kF32>(p, row, v) : -INFINITY;
+    q[i] = v < p.V ? p.probs[q_row + v] : 0.f;
+  }
   double s = 0.0;
-  for (int i = 0; i < kPer; ++i) s += draw_weight<kF32>(p, row, q_row, (int64_t)ch * kChunk + threadIdx.x + i * kThreads, LESS_DRAFT, -1, d);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) s += draw_weight(l[i], q[i], LESS_DRAFT, d, p.scale);
   s = block_sum_f64(s, red);
   if (threadIdx.x == 0) p.rest[(int64_t)b * p.nc + ch] = s;
 }
 
+constexpr int kPickThreads = 1024, kPickPer = kChunk / kPickThreads, kPickWaves = kPickThreads / 64;
+
 template <bool kF32>
-__global__ __launch_bounds__(kThreads) void verify_pick_kernel(VerifyParams p) {
-  __shared__ double red[4], share[kMaxChunks], before[kThreads];
-  __shared__ int found[2];
+__global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyParams p) {
+  __shared__ double red[kPickWaves], start, target;
+  __shared__ int first, last, at_chunk, draw_kind;
+  __shared__ int64_t draft;
   const int b = blockIdx.x, tid = threadIdx.x, n = drafts_of(p, b);
   int64_t* out = p.tokens + (int64_t)b * (p.T + 1);
   if (n < 0) {
-    for (int t = tid; t <= p.T; t += kThreads) out[t] = -1;
+    for (int t = tid; t <= p.T; t += kPickThreads) out[t] = -1;
     if (tid == 0) p.accepted[b] = 0;
     return;
   }
   const Decision d = decide<kF32>(p, b, n);
-  for (int t = tid; t <= p.T; t += kThreads)
+  for (int t = tid; t <= p.T; t += kPickThreads)
     if (t != d.a) out[t] = t < d.a ? p.drafts[(int64_t)b * p.T + t] : -1;
   if (tid == 0) p.accepted[b] = d.a;
-  if (d.top == -INFINITY || p.inv_temp == 0.0) {               // greedy, or a row that offers nothing
+  if (d.top == -INFINITY || p.scale == 0.0) {               // greedy, or a row that offers nothing
     if (tid == 0) out[d.a] = d.top == -INFINITY ? -1 : d.arg;
     return;
   }
   const int64_t row = (int64_t)b * p.seq_stride + (int64_t)d.a * p.row_stride, q_row = (int64_t)b * p.probs_seq_stride + (int64_t)d.a * p.probs_row_stride;
-  const int64_t at = ((int64_t)b * (p.T + 1) + d.a) * p.nc;
-  int kind = d.a == n ? FROM_ROW : (p.probs ? LESS_DRAFT : WITHOUT_DRAFT);
-  int64_t x = -1;
-  if (kind == WITHOUT_DRAFT) x = p.drafts[(int64_t)b * p.T + d.a];
-  double total = 0.0;
-  for (;;) {                                                   // twice at most: nothing left of p - q (they are equal) -> p itself
-    double mine = 0.0;
-    for (int c = tid; c < p.nc; c += kThreads) {
-      double w;
-      if (kind == LESS_DRAFT) w = p.rest[(int64_t)b * p.nc + c];
-      else { const float cm = p.top[at + c]; w = cm == -INFINITY ? 0.0 : p.sum[at + c] * weight(cm, d.top, p.inv_temp); }
-      share[c] = w;
+  if (tid < 64) {                                              // one wave finds the chunk that the draw falls into
+    const int64_t at = ((int64_t)b * (p.T + 1) + d.a) * p.nc;
+    int kind = d.a == n ? FROM_ROW : (p.probs ? LESS_DRAFT : WITHOUT_DRAFT);
+    int64_t x = -1;
+    if (kind == WITHOUT_DRAFT) {
+      x = p.drafts[(int64_t)b * p.T + d.a];
+      if (x < 0 || x >= p.V) { x = -1; kind = FROM_ROW; }
     }
-    __syncthreads();
-    if (kind == WITHOUT_DRAFT && x >= 0 && x < p.V) {          // summed again without x: its share may be nearly all there is
-      const int64_t c = x / kChunk;
-      double s = 0.0;
-      for (int i = 0; i < kPer; ++i) s += draw_weight<kF32>(p, row, q_row, c * kChunk + tid + i * kThreads, kind, x, d);
-      s = block_sum_f64(s, red);
-      if (tid == 0) share[c] = s;
-      __syncthreads();
+    const int cx = x >= 0 ? (int)(x / kChunk) : -1;
+    auto share = [&](int c) {
+      if (c >= p.nc) return 0.0;
+      if (kind == LESS_DRAFT) return p.rest[(int64_t)b * p.nc + c];
+      const double* s = kind == WITHOUT_DRAFT && c == cx ? p.others + (int64_t)b * p.T + d.a : p.sum + at + c;
+      return *s * weight(p.top[at + c], d.top, p.scale);
+    };
+    const float u = p.u[(int64_t)b * (p.T + 1) + p.T];
+    double total, held;                                        // held: this lane's share of the first 64 chunks (mostly all there are)
+    for (;;) {                                                 // twice at most: nothing left of p - q (they are equal) -> p itself
+      double mine = held = share(tid);
+      for (int c = tid + 64; c < p.nc; c += 64) mine += share(c);
+      total = wave_sum_f64(mine);
+      if (total > 0.0 || kind == FROM_ROW) break;
+      kind = FROM_ROW; x = -1;
     }
-    for (int c = tid; c < p.nc; c += kThreads) mine += share[c];
-    total = block_sum_f64(mine, red);
-    if (total > 0.0 || kind == FROM_ROW) break;
-    kind = FROM_ROW;
-    __syncthreads();
-  }
-  const double want = (double)p.u[(int64_t)b * (p.T + 1) + p.T] * total;
-  if (tid == 0) {
-    double run = 0.0, base = 0.0;
-    int hit = -1, last = 0;
-    double last_base = 0.0;
-    for (int c = 0; c < p.nc; ++c) {
-      const double w = share[c];
-      if (!(w > 0.0)) continue;
-      last = c; last_base = run;
-      if (run + w > want) { hit = c; base = run; break; }
-      run += w;
+    const double want = (double)u * total;
+    double run = 0.0, base = 0.0;                              // run: of the chunks before this round's 64
+    int chunk = 0;                                             // the last one with a share so far
+    for (int c0 = 0; c0 < p.nc; c0 += 64) {
+      const double w = c0 ? share(c0 + tid) : held;
+      double incl = w;
+#pragma unroll
+      for (int k = 1; k < 64; k <<= 1) {
+        const double o = __shfl_up(incl, k, 64);
+        if (tid >= k) incl += o;
+      }
+      const double before = run + (incl - w);
+      const unsigned long long has = __ballot(w > 0.0), over = __ballot(w > 0.0 && run + incl > want);
+      const unsigned long long pick = over ? (over & -over) : has;
+      if (pick) {
+        const int l = over ? __ffsll((long long)pick) - 1 : 63 - __clzll((long long)pick);
+        chunk = c0 + l;
+        base = __shfl(before, l, 64);
+      }
+      if (over) break;
+      run += __shfl(incl, 63, 64);
     }
-    found[0] = hit >= 0 ? hit : last;
-    before[0] = hit >= 0 ? base : last_base;
+    if (tid == 0) { at_chunk = chunk; start = base; target = want; draw_kind = kind; draft = x; first = INT32_MAX; last = -1; }
   }
   __syncthreads();
-  const int c = found[0];
-  const double base = before[0];
-  __syncthreads();
-  double w[kPer], sum = 0.0;
-  const int64_t v0 = (int64_t)c * kChunk + (int64_t)tid * kPer;
+  const int kind = draw_kind;
+  const int64_t x = draft;
+  float l[kPickPer], q[kPickPer];
+  const int64_t v0 = (int64_t)at_chunk * kChunk + (int64_t)tid * kPickPer;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) { w[i] = draw_weight<kF32>(p, row, q_row, v0 + i, kind, x, d); sum += w[i]; }
-  double incl = sum;                                           // running sum over the workgroup's threads
+  for (int i = 0; i < kPickPer; ++i) {
+    const bool in = v0 + i < p.V && v0 + i != x;               // (x: the refused certain draft, or -1)
+    l[i] = in ? logit<kF32>(p, row, v0 + i) : -INFINITY;
+    q[i] = in && kind == LESS_DRAFT ? p.probs[q_row + v0 + i] : 0.f;
+  }
+  double w[kPickPer], sum = 0.0;
 #pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const double o = __shfl_up(incl, s, 64);
-    if ((tid & 63) >= s) incl += o;
+  for (int i = 0; i < kPickPer; ++i) { w[i] = draw_weight(l[i], q[i], kind, d, p.scale); sum += w[i]; }
+  double incl = sum;
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    const double o = __shfl_up(incl, k, 64);
+    if ((tid & 63) >= k) incl += o;
   }
   if ((tid & 63) == 63) red[tid >> 6] = incl;
-  if (tid < 2) found[tid] = tid == 0 ? INT32_MAX : -1;
   __syncthreads();
-  double run = base + (incl - sum);
-  for (int k = 0; k < (tid >> 6); ++k) run += red[k];
-  int first = INT32_MAX, last = -1;
+  double run = start + (incl - sum);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
+  for (int k = 0; k < kPickWaves - 1; ++k) run += k < (tid >> 6) ? red[k] : 0.0;
+  int hit = INT32_MAX, able = -1;
+#pragma unroll
+  for (int i = 0; i < kPickPer; ++i) {
     run += w[i];
     if (w[i] > 0.0) {
-      last = (int)(v0 + i);
-      if (first == INT32_MAX && run > want) first = last;
+      able = (int)(v0 + i);
+      if (hit == INT32_MAX && run > target) hit = able;
     }
   }
-  if (first != INT32_MAX) atomicMin(&found[0], first);
-  if (last >= 0) atomicMax(&found[1], last);
+  const unsigned long long hits = __ballot(hit != INT32_MAX), ables = __ballot(able >= 0);        // (one LDS atomic per wave: 1024 of them take 5 us)
+  const int wave_hit = __shfl(hit, hits ? __ffsll((long long)hits) - 1 : 0, 64), wave_able = __shfl(able, ables ? 63 - __clzll((long long)ables) : 0, 64);
+  if ((tid & 63) == 0) {
+    if (hits) atomicMin(&first, wave_hit);
+    if (ables) atomicMax(&last, wave_able);
+  }
   __syncthreads();
-  if (tid == 0) out[d.a] = found[0] != INT32_MAX ? found[0] : found[1];
+  if (tid == 0) out[d.a] = first != INT32_MAX ? first : last;
 }
 
 template <bool kF32>
@@ -280,11 +370,11 @@ int launch(const VerifyParams& p, hipStream_t s) {
   verify_stats_kernel<kF32><<<dim3((unsigned)p.nc, (unsigned)(p.T + 1), (unsigned)p.batch), kThreads, 0, s>>>(p);
   int rc = qp_check_launch("verify_drafts(stats)");
   if (rc) return rc;
-  if (p.probs && p.inv_temp != 0.0) {
+  if (p.probs && p.scale != 0.0) {
     verify_rest_kernel<kF32><<<dim3((unsigned)p.nc, (unsigned)p.batch), kThreads, 0, s>>>(p);
     if ((rc = qp_check_launch("verify_drafts(rest)"))) return rc;
   }
-  verify_pick_kernel<kF32><<<(unsigned)p.batch, kThreads, 0, s>>>(p);
+  verify_pick_kernel<kF32><<<(unsigned)p.batch, kPickThreads, 0, s>>>(p);
   return qp_check_launch("verify_drafts(pick)");
 }
 
@@ -295,7 +385,7 @@ int qp_verify_max_drafts() { return kMaxDrafts; }
 
 size_t qp_verify_workspace_bytes_impl(int batch, int t_max, int64_t vocab) {
   const size_t nc = (size_t)((vocab + kChunk - 1) / kChunk), rows = (size_t)batch * (t_max + 1);
-  return rows * nc * (sizeof(double) + sizeof(float) + sizeof(int)) + (size_t)batch * nc * sizeof(double);
+  return rows * nc * (sizeof(double) + sizeof(float) + sizeof(int)) + (size_t)batch * (nc + t_max) * sizeof(double);
 }
 
 int qp_launch_verify_drafts(const void* logits, int logits_f32, int64_t seq_stride, int64_t row_stride, const int64_t* drafts, const int32_t* n_draft,
@@ -307,11 +397,12 @@ int qp_launch_verify_drafts(const void* logits, int logits_f32, int64_t seq_stri
   p.probs = t_max > 0 ? probs : nullptr; p.probs_seq_stride = probs_seq_stride; p.probs_row_stride = probs_row_stride;
   p.u = uniforms; p.batch = batch; p.T = t_max; p.V = vocab;
   p.nc = (int)((vocab + kChunk - 1) / kChunk);
-  p.inv_temp = temperature > 0.f ? 1.0 / (double)temperature : 0.0;
+  p.scale = temperature > 0.f ? 1.4426950408889634074 / (double)temperature : 0.0;
   const size_t rows = (size_t)batch * (t_max + 1) * p.nc;
   p.sum = (double*)workspace;
   p.rest = p.sum + rows;
-  p.top = (float*)(p.rest + (size_t)batch * p.nc);
+  p.others = p.rest + (size_t)batch * p.nc;
+  p.top = (float*)(p.others + (size_t)batch * t_max);
   p.arg = (int*)(p.top + rows);
   p.accepted = n_accepted; p.tokens = tokens;
   return logits_f32 ? launch<true>(p, s) : launch<false>(p, s);
