@@ -330,6 +330,147 @@ __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int
   st.m = m_run; st.l = l_run;
 }
 
+// The same for ONE row tile (WR = 1): nothing is shared, so every wave stages and computes 32-key blocks of its own (block first, first + WK, ... of the
+// range) in its own 16 KB of LDS, without a barrier; waves drift apart and hide each other's waiting.
+template <int WK, bool kPaged>
+__device__ __forceinline__ void walk_alone(const BatchAttnParams& p, int kvh, int b, int64_t r, bool row_live, const bf16x8_t (&qf)[8], int k0, int k1, int first,
+                                           unsigned char* lds, Shared& sh, Rows& st) {
+  const int lane = threadIdx.x & 63, hi = lane >> 5, l31 = lane & 31, r4 = lane >> 4, slot16 = lane & 15;
+  unsigned char* kl = lds + (threadIdx.x >> 6) * 16384;
+  unsigned char* vl = kl + 8192;
+  int limit = INT32_MAX, seen_by_all = INT32_MAX;              // as in walk_keys
+  if (kPaged) {
+    const int stored = min(p.pg.seq_len[b], kMaxKeys);
+    seen_by_all = stored + 1;
+    limit = stored + (row_live ? (int)(r / p.G - (int64_t)b * p.t_max) : 0);
+  }
+  const uint4* kbase = kPaged ? p.k_pages : p.k_pre + (int64_t)kvh * p.pre_hs16;
+  const uint4* vbase = kPaged ? p.v_pages : p.v_pre + (int64_t)kvh * p.pre_hs16;
+  uint4 kx[8], vx[8];
+  unsigned holes = 0;                                          // bit i: staged row r4 + 4 i has no page
+  auto load = [&](int t0) {
+    if (!kPaged) {
+      const uint4* kt = kbase + (int64_t)t0 * 16;              // 8 KB in a row
+      const uint4* vt = vbase + (int64_t)t0 * 16;
+      if (t0 + 32 <= k1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { kx[i] = kt[lane + i * 64]; vx[i] = vt[lane + i * 64]; }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          kx[i] = vx[i] = make_uint4(0, 0, 0, 0);
+          if (t0 + r4 + 4 * i < k1) { kx[i] = kt[lane + i * 64]; vx[i] = vt[lane + i * 64]; }
+        }
+      }
+    } else {
+      holes = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int key = t0 + r4 + 4 * i;
+        kx[i] = vx[i] = make_uint4(0, 0, 0, 0);
+        if (key < k1) {
+          const int64_t at = page_row16(p.pg, b, kvh, key);
+          if (at < 0) { holes |= 1u << i; continue; }
+          kx[i] = kbase[at + slot16]; vx[i] = vbase[at + slot16];
+        }
+      }
+    }
+  };
+  const int koff = l31 * 256 + ((hi ^ (l31 & 15)) << 4);
+  const int voff = (((lane & 15) >> 2) << 6) + (((lane >> 4) & 1) << 5) + ((lane & 3) << 3) + (hi << 10);
+  f32x16_t (&o)[4] = st.o;
+  float m_run = st.m, l_run = st.l;
+  constexpr bool kAhead = !kPaged;                             // (the paged form would spill)
+  int t0 = k0 + first * 32;
+  if (kAhead && t0 < k1) load(t0);
+  for (; t0 < k1; t0 += 32 * WK) {
+    if (!kAhead) load(t0);
+    u16x2_t top = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = __builtin_elementwise_max(top, magnitude(vx[i]));
+    if (__any(is_odd(top))) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) make_finite(vx[i]);
+      sh.odd = 1;
+    }
+    __builtin_amdgcn_wave_barrier();                           // the last block's fragment reads stay ahead of these writes
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = r4 + 4 * i;
+      *reinterpret_cast<uint4*>(kl + row * 256 + ((slot16 ^ (row & 15)) << 4)) = kx[i];
+      *reinterpret_cast<uint4*>(vl + (((row >> 2) * 4 + (slot16 >> 2)) << 8) + ((row & 3) << 6) + ((slot16 & 3) << 4)) = vx[i];
+    }
+    unsigned have = ~0u;                                       // rows of the block that have a page
+    if (kPaged && __any(holes)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const unsigned long long m = __ballot((holes >> i) & 1);
+        have &= ~(((unsigned)(m & 1) | ((unsigned)(m >> 16) & 1) << 1 | ((unsigned)(m >> 32) & 1) << 2 | ((unsigned)(m >> 48) & 1) << 3) << (4 * i));
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (kAhead && t0 + 32 * WK < k1) load(t0 + 32 * WK);
+    f32x16_t s = (f32x16_t){0};
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      if (kk == 4) __builtin_amdgcn_sched_barrier(0);          // (half of the K fragments at a time: registers)
+      s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_read_b128(kl, koff ^ (kk << 5)), qf[kk], s, 0, 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (t0 + 32 > k1 || t0 + 32 > seen_by_all || have != ~0u) {
+      const int last = (limit < k1 ? limit : k1 - 1) - t0 - 4 * hi;
+      const unsigned seen = have >> (4 * hi);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int row = (e & 3) + 8 * (e >> 2);
+        s[e] = row <= last && ((seen >> row) & 1) ? s[e] : -INFINITY;
+      }
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
+    mx = xhalf_max(mx);
+    if (!__all((mx - m_run) * p.c <= 8.0f)) {
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * p.c);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
+    }
+    const float mc = m_run * p.c;
+    float rs = 0.f;
+    bf16x8_t pf[2], pr[2];
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cc * 8 + e], p.c, -mc));
+        rs += pe;
+        pf[cc][e] = (__bf16)pe;
+        pr[cc][e] = (__bf16)(pe - (float)pf[cc][e]);
+      }
+    l_run += xhalf_sum(rs);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        const int off = voff + (((cc * 4) * 4 + db) << 8);
+        const s16x4_t v0 = lds_read_tr16(vl, off);
+        const s16x4_t v1 = lds_read_tr16(vl, off + (2 * 4 << 8));
+        const s16x8_t av = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), pf[cc], o[db], 0, 0, 0);
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), pr[cc], o[db], 0, 0, 0);
+      }
+  }
+  st.m = m_run; st.l = l_run;
+}
+
 // Q fragments of the lane's row, an empty running state and cleared flags (the first barrier of walk_keys orders the flags)
 __device__ __forceinline__ void begin_rows(const BatchAttnParams& p, int kvh, int64_t r, bool row_live, bf16x8_t (&qf)[8], Shared& sh, Rows& st) {
   const int tid = threadIdx.x, hi = (tid >> 5) & 1;
@@ -396,7 +537,13 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
   bf16x8_t qf[8];
   Rows st;
   begin_rows(p, kvh, r, row_live, qf, sh, st);
-  walk_keys<WR, WK, kPaged>(p, kvh, b, r, row_live, wave_live, qf, k0, k1, lds, sh, st);
+  if (WR == 1) {
+    __syncthreads();                                           // flags cleared
+    walk_alone<WK, kPaged>(p, kvh, b, r, row_live, qf, k0, k1, wave, lds, sh, st);
+    __syncthreads();                                           // the blocks are read: their LDS joins the rows
+  } else {
+    walk_keys<WR, WK, kPaged>(p, kvh, b, r, row_live, wave_live, qf, k0, k1, lds, sh, st);
+  }
   const int64_t slot0 = ((int64_t)kvh * (p.ns + p.ns2) + part) * p.R;
   if (WR == 1) {
     float* obuf = reinterpret_cast<float*>(lds);
@@ -502,8 +649,8 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnPa
   batch_attn_range<WR, WK, true>(p, kvh, b, row0, row_end, k0, k1, p.ns + split, lds, lds_ml, sh);
 }
 
-// Few keys: ONE launch.  A workgroup of 8 waves walks the prefix and then the pages for the (at most 32) rows of one sequence and kv head, 256
-// keys at a time, and joins its waves itself; the prefix is read again for every sequence, from L2.
+// Few keys: ONE launch.  The 8 waves of a workgroup deal the prefix's and the pages' 32-key blocks among themselves for the (at most 32) rows of one
+// sequence and kv head and join their results; the prefix is read again for every sequence, from L2.
 constexpr int kDirectWaves = 8, kDirectLds = join_bytes<kDirectWaves>();
 static_assert(kDirectLds >= 2 * Shape<1, kDirectWaves>::TILE * 256, "the tiles fit as well");
 
@@ -521,8 +668,11 @@ __global__ __launch_bounds__(64 * kDirectWaves, 2) void batch_attn_direct_kernel
   bf16x8_t qf[8];
   Rows st;
   begin_rows(p, kvh, r, row_live, qf, sh, st);
-  walk_keys<1, kDirectWaves, false>(p, kvh, b, r, row_live, true, qf, 0, (int)p.P, lds, sh, st);
-  walk_keys<1, kDirectWaves, true>(p, kvh, b, r, row_live, true, qf, 0, len, lds, sh, st);
+  __syncthreads();                                             // flags cleared
+  const int wave = tid >> 6, blocks = ((int)p.P + 31) / 32;
+  walk_alone<kDirectWaves, false>(p, kvh, b, r, row_live, qf, 0, (int)p.P, wave, lds, sh, st);
+  walk_alone<kDirectWaves, true>(p, kvh, b, r, row_live, qf, 0, len, (wave - blocks) & (kDirectWaves - 1), lds, sh, st);   // the pages go on where the prefix ended
+  __syncthreads();                                             // the blocks are read: their LDS joins the rows
   float* obuf = reinterpret_cast<float*>(lds);
   lay_out_rows<kDirectWaves>(st, p.c, row_live, obuf, lds_m, lds_l);
   const int64_t slot0 = (int64_t)kvh * p.R;
