@@ -167,8 +167,18 @@ struct Rows {                      // what a lane keeps of its row (both halves 
   f32x16_t o[4];                   // [d / 32], unscaled
   float m, l;
 };
+// p = hi + lo with both in bf16, two probabilities at a time (one conversion instruction per pair and term)
+__device__ __forceinline__ void split_pair(float a, float b, unsigned& hi, unsigned& lo) {
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  const bf2 h = {(__bf16)a, (__bf16)b};
+  hi = __builtin_bit_cast(unsigned, h);
+  const bf2 l = {(__bf16)(a - __uint_as_float(hi << 16)), (__bf16)(b - __uint_as_float(hi & 0xffff0000u))};
+  lo = __builtin_bit_cast(unsigned, l);
+}
+typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
+
 struct Shared {                    // LDS besides the tile
-  unsigned long long holes[2][4];  // by parity of the tile: its rows without a page
+  unsigned long long holes[3][4];  // by number of the tile: its rows without a page
   int odd;                         // a value that is not finite was met
 };
 
@@ -301,15 +311,17 @@ __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int
 #pragma unroll
     for (int k = 0; k < KB; ++k) {
       const int kb = WK >= 2 ? wk : k;
-      bf16x8_t pf[2], pr[2];
+      u32x4_t pf[2], pr[2];
 #pragma unroll
       for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][cc * 8 + e], p.c, -mc));
-          rs += pe;
-          pf[cc][e] = (__bf16)pe;
-          pr[cc][e] = (__bf16)(pe - (float)pf[cc][e]);
+        for (int e = 0; e < 4; ++e) {
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][cc * 8 + 2 * e], p.c, -mc));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][cc * 8 + 2 * e + 1], p.c, -mc));
+          rs += p0 + p1;
+          unsigned h, l;
+          split_pair(p0, p1, h, l);
+          pf[cc][e] = h; pr[cc][e] = l;
         }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -320,8 +332,8 @@ __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int
           const s16x4_t v0 = lds_read_tr16(vl, off);
           const s16x4_t v1 = lds_read_tr16(vl, off + (2 * 4 << 8));
           const s16x8_t av = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), pf[cc], o[db], 0, 0, 0);
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), pr[cc], o[db], 0, 0, 0);
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), __builtin_bit_cast(bf16x8_t, pf[cc]), o[db], 0, 0, 0);
+          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), __builtin_bit_cast(bf16x8_t, pr[cc]), o[db], 0, 0, 0);
         }
       }
     }
@@ -444,15 +456,17 @@ __device__ __forceinline__ void walk_alone(const BatchAttnParams& p, int kvh, in
     }
     const float mc = m_run * p.c;
     float rs = 0.f;
-    bf16x8_t pf[2], pr[2];
+    u32x4_t pf[2], pr[2];
 #pragma unroll
     for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float pe = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cc * 8 + e], p.c, -mc));
-        rs += pe;
-        pf[cc][e] = (__bf16)pe;
-        pr[cc][e] = (__bf16)(pe - (float)pf[cc][e]);
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cc * 8 + 2 * e], p.c, -mc));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cc * 8 + 2 * e + 1], p.c, -mc));
+        rs += p0 + p1;
+        unsigned h, l;
+        split_pair(p0, p1, h, l);
+        pf[cc][e] = h; pr[cc][e] = l;
       }
     l_run += xhalf_sum(rs);
     __builtin_amdgcn_sched_barrier(0);
@@ -464,8 +478,8 @@ __device__ __forceinline__ void walk_alone(const BatchAttnParams& p, int kvh, in
         const s16x4_t v0 = lds_read_tr16(vl, off);
         const s16x4_t v1 = lds_read_tr16(vl, off + (2 * 4 << 8));
         const s16x8_t av = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), pf[cc], o[db], 0, 0, 0);
-        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), pr[cc], o[db], 0, 0, 0);
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), __builtin_bit_cast(bf16x8_t, pf[cc]), o[db], 0, 0, 0);
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), __builtin_bit_cast(bf16x8_t, pr[cc]), o[db], 0, 0, 0);
       }
   }
   st.m = m_run; st.l = l_run;
@@ -485,7 +499,7 @@ __device__ __forceinline__ void begin_rows(const BatchAttnParams& p, int kvh, in
 #pragma unroll
   for (int db = 0; db < 4; ++db) st.o[db] = (f32x16_t){0};
   st.m = -1e30f; st.l = 0.f;
-  if (tid < 8) sh.holes[tid >> 2][tid & 3] = 0;
+  if (tid < 12) sh.holes[tid >> 2][tid & 3] = 0;
   if (tid == 0) sh.odd = 0;
 }
 
