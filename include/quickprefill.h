@@ -276,7 +276,7 @@ int qp_decode_attn_fused(qp_ctx* ctx, const void* qkv, const void* cos, const vo
 int qp_decode_advance(qp_ctx* ctx, int64_t* state, int64_t n_values, void* stream);
 
 /* ---- a batch of sequences over one prefilled video -----------------------------------------------------------------------------
- * Beams, sampled answers, several questions, drafted tokens (the reference hands `num_beams`, `prompt_lookup_num_tokens`, ... to HF
+ * Beams, sampled answers, several questions, drafted tokens (the reference hands `num_beams` and the other generation kwargs to HF
  * generate, lvu/models/qwen25_lvu.py:744-761): `batch` sequences share the video's K/V rows of a layer ([0, prefix_len) of the arena,
  * frozen meanwhile), and every sequence keeps the rows of its own tokens in pages.
  *   pages        K and V bf16, page p at k_pages + p * page_stride (elements): [n_kv_heads][page_size][128]; any page_size >= 1

@@ -12,7 +12,8 @@
 The model is a callback `advance(parents, tokens) -> fp32 logits [B, V]`: running beam i of the next step extends beam `parents[i]` of
 this step by `tokens[i]`.  The engine side (`EngineBeams`) keeps ONE KV arena: the prefilled video + prompt rows are shared by all beams
 (504 k rows per layer for the 1-hour video), each beam only owns the few rows of its generated tokens, which are swapped into the
-arena tail before the beam's decode step (B sequential steps per token — HF batches them; the answer is the same).
+arena tail before the beam's decode step (B sequential steps per token — HF batches them; the answer is the same).  `batched=True` (generate's
+`batched_beams`): all beams go through the layers as one batch and the shared rows are read once per token (batch.py).
 Pinned against the installed transformers' `generate(num_beams=...)` on a tiny text model (tests/test_beam_search.py)."""
 from __future__ import annotations
 
@@ -127,11 +128,15 @@ class EngineBeams:
     """`advance` over a QuickPrefillEngine whose arena holds the prefilled video + prompt: beams share rows [0, P) of every layer; beam b owns
     a small tail block [L, 2, Hkv, T, D] with the K/V rows of its generated tokens."""
 
-    def __init__(self, eng, rope_delta: int, num_beams: int, max_new_tokens: int):
+    def __init__(self, eng, rope_delta: int, num_beams: int, max_new_tokens: int, batched: bool = False):
         self.eng, self.delta, self.B = eng, rope_delta, num_beams
+        self.batch = None
+        if batched:
+            from .batch import BatchDecoder
+            self.batch = BatchDecoder(eng, rope_delta, num_beams, max_new_tokens)
         self.base_len, self.base_pos = list(eng.arena.len), eng.seq_pos
         L, hkv, D = len(eng.arena.len), eng.hkv, eng.D
-        self.tails = [torch.empty(L, 2, hkv, max_new_tokens, D, dtype=eng.dtype, device=eng.device) for _ in range(num_beams)]
+        self.tails = [] if batched else [torch.empty(L, 2, hkv, max_new_tokens, D, dtype=eng.dtype, device=eng.device) for _ in range(num_beams)]
         self.t = 0                                                     # generated tokens already cached per running beam
 
     def _load(self, tail):
@@ -144,6 +149,11 @@ class EngineBeams:
 
     def advance(self, parents: List[int], tokens: List[int]) -> torch.Tensor:
         eng, t = self.eng, self.t
+        if self.batch is not None:
+            self.batch.reorder(parents)
+            logits = self.batch.step(torch.tensor(tokens, dtype=torch.int64, device=eng.device)[:, None])
+            self.batch.keep([1] * self.B)
+            return logits[:, 0].float()
         new_tails = [torch.empty_like(self.tails[0]) for _ in range(self.B)]
         out = []
         for i, (par, tok) in enumerate(zip(parents, tokens)):

@@ -537,13 +537,21 @@ class PrefillPipeline:
     def _generate(self, question, video, max_new_tokens: int = 16, overlap: bool = True, eos_token_id=None,
                   do_sample: Optional[bool] = None, temperature: Optional[float] = None, top_k: Optional[int] = None,
                   top_p: Optional[float] = None, repetition_penalty: Optional[float] = None, seed: Optional[int] = None,
-                  num_beams: int = 1, length_penalty: float = 1.0, early_stopping=False, **unused) -> List[int]:
+                  num_beams: int = 1, length_penalty: float = 1.0, early_stopping=False, batched_beams: bool = False,
+                  lookup_tokens: int = 0, **unused) -> List[int]:
         """generation kwargs as the reference hands them to HF `generate` (qwen25_lvu.py:744-761); unset ones fall back to the
         checkpoint's generation_config.json (`model.generation_defaults`), then to greedy.  `num_beams > 1`: beam search with HF's
-        semantics (`length_penalty`, `early_stopping`, with `do_sample` beam-search multinomial sampling; beam.py).
+        semantics (`length_penalty`, `early_stopping`, with `do_sample` beam-search multinomial sampling; beam.py); `batched_beams`: the
+        beams of a step go through the model together and read the video's cache once (batch.py; one GPU).  `lookup_tokens`: up to that many
+        tokens a step are drafted from the prompt and the answer so far and verified in one pass over the cache (HF's prompt lookup, batch.py; one
+        GPU, one beam).  Both are refused where they cannot work; neither changes what a call without them computes.
         `question`: the user's text, or the reference's `messages` list (chat(); qwen25_lvu.py:546-548) when the processor can
         template it.  eos_token_id: an id or a list of ids (HF stops on ANY of generation_config.eos_token_id)."""
         num_beams = int(num_beams)
+        if (batched_beams or lookup_tokens) and (self.par.on or self.cfg.do_top_k_for_query):
+            raise ValueError("batched_beams / lookup_tokens decode several rows in one process: not with a multi-GPU layout or do_top_k_for_query")
+        if lookup_tokens and (int(lookup_tokens) < 1 or num_beams > 1):
+            raise ValueError(f"lookup_tokens (={lookup_tokens}) must be >= 1 and goes with one beam")
         gd = getattr(self.model, "generation_defaults", None) or {}
         pick = lambda v, k: gd.get(k) if v is None else v
         selector = TokenSelector(pick(do_sample, "do_sample") or False, pick(temperature, "temperature"), pick(top_k, "top_k"),
@@ -748,7 +756,7 @@ class PrefillPipeline:
             if first is not None:
                 _ = float(first[0].item())
             tm.ttft = time.perf_counter() - t_e2e
-            beams = EngineBeams(eng, P["delta"], num_beams, max_new_tokens)
+            beams = EngineBeams(eng, P["delta"], num_beams, max_new_tokens, batched=bool(batched_beams))
             search = lambda adv: beam_search(first, adv, num_beams, max_new_tokens, eos_ids=sorted(eos_set), length_penalty=float(length_penalty),   # noqa: E731
                                              early_stopping=early_stopping, repetition_penalty=selector.penalty, prompt_ids=list(P["prompt"].tail_ids),
                                              do_sample=selector.do_sample, temperature=selector.temperature, top_k=selector.top_k,
@@ -798,10 +806,16 @@ class PrefillPipeline:
         tok = choose(logits)                                                  # first token on the host = TTFT point
         tm.ttft = time.perf_counter() - t_e2e
         out = [tok]
-        graph = (not par.on) and GraphDecoder.supported(eng)                  # one hipGraph replay per token (decode.py); multi-GPU: eager
+        lookup = None
+        if lookup_tokens and max_new_tokens > 1:
+            from .batch import LookupDecoder
+            lookup = LookupDecoder(eng, P["delta"], max_new_tokens, min(int(lookup_tokens), eng.n_max - 1, max_new_tokens), selector)
+        graph = (not par.on) and lookup is None and GraphDecoder.supported(eng)                  # one hipGraph replay per token (decode.py); multi-GPU: eager
         if graph and getattr(eng, "_graph_decoder", None) is None:
             eng._graph_decoder = GraphDecoder(eng)
-        if graph and selector.trivial:                                        # argmax stays on the device inside the graph
+        if lookup is not None:
+            out += lookup.generate(tok, list(P["prompt"].tail_ids), max_new_tokens - 1, eos_set)
+        elif graph and selector.trivial:                                      # argmax stays on the device inside the graph
             out += eng._graph_decoder.generate(tok, max_new_tokens - 1, P["delta"], eos_set or None)
         else:                                                                 # logits come back per step: processors / sampling, or the
             if graph and max_new_tokens > 1:                                  # per-op path (CPU test doubles, parallel engines)
