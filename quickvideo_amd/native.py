@@ -146,6 +146,15 @@ def load_library(path: str = LIB_PATH, hold_gil: bool = False) -> ctypes.CDLL:
     return lib
 
 
+def load_face():
+    """The module that reads torch tensors for the batch operators (csrc/qp_torch.cpp, built beside the library)."""
+    try:
+        from . import _qp_torch
+    except ImportError as e:
+        raise QuickPrefillUnavailable(f"quickvideo_amd/_qp_torch.so cannot be loaded ({e}): build it with `python -c 'import __graft_entry__ as g; g.build()'`") from e
+    return _qp_torch
+
+
 _HOST_LIB = None
 
 
@@ -178,8 +187,7 @@ class QuickPrefillOps:
         # lock-releasing handle of the same .so: the producer thread, RCCL/gloo progress and Ctrl-C keep running meanwhile
         self.lib_blocking = load_library(hold_gil=False)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        self._dev = self.device.index or 0
-        self._stream_of = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(dev).cuda_stream without making a Stream object
+        self._bind_face()
         h = _vp()
         self._check(self.lib.qp_create(ctypes.byref(h), self.device.index or 0))
         self.ctx = h
@@ -418,8 +426,23 @@ class QuickPrefillOps:
         self._check(self.lib.qp_decode_advance(self.ctx, state.data_ptr(), state.numel(), self._stream()))
 
     # -- a batch of sequences over one prefilled video (include/quickprefill.h; batch.py drives them)
-    # These run once per layer and token, so what they check of a tensor is one short expression each; the message is made only on a refusal.
-    def _refuse(self, name, t, dtype, shape=None, contiguous=True):
+    # These run once per layer and token, so the module _qp_torch (csrc/qp_torch.cpp) reads the tensors and makes the call; it returns REFUSED, without a
+    # call, when a tensor is not what the kernels take, and the _why_* functions here say what is wrong with it.
+    def _bind_face(self):
+        self._face = load_face()
+        self._dev = self.device.index or 0
+        self._stream_of = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(dev).cuda_stream without making a Stream object
+        self._fns = {n: ctypes.cast(getattr(self.lib, n), _vp).value for n in ("qp_batch_rope_append", "qp_batch_attn", "qp_verify_drafts")}
+
+    def _after(self, status, why, *args):
+        if status == self._face.REFUSED:
+            why(*args)
+            raise ValueError("libquickprefill: arguments refused")
+        self._check(status)
+
+    def _need(self, name, t, dtype, shape=None, contiguous=True):
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"libquickprefill: {name} is {type(t).__name__}, a tensor is needed")
         if t.dtype != dtype:
             raise ValueError(f"libquickprefill: {name} is {t.dtype}, {dtype} is needed")
         if shape is not None and t.shape != shape:
@@ -429,47 +452,35 @@ class QuickPrefillOps:
         if t.get_device() != self._dev:
             raise ValueError(f"libquickprefill: {name} is on {t.device}, the operators are on {self.device}")
 
-    def _batch_pages(self, k, v, table, seq_len, n_new, batch, n_kv, head_dim, dev):
-        """-> (page stride, page size, pages per sequence); k / v pages [n_pages, n_kv, page_size, head_dim], each page contiguous."""
-        shape, st = k.shape, k.stride()
-        if len(shape) != 4:
-            raise ValueError(f"libquickprefill: k_pages has shape {tuple(shape)}, [n_pages, {n_kv}, page_size, {head_dim}] is needed")
-        n_pages, ps = shape[0], shape[2]
-        want = (n_pages, n_kv, ps, head_dim)
-        if shape != want or k.dtype is not torch.bfloat16 or k.get_device() != dev:
-            self._refuse("k_pages", k, torch.bfloat16, want, False)
-        if v.shape != want or v.dtype is not torch.bfloat16 or v.get_device() != dev:
-            self._refuse("v_pages", v, torch.bfloat16, want, False)
-        if st != v.stride() or st[1:] != (ps * head_dim, head_dim, 1):
-            raise ValueError(f"libquickprefill: k_pages / v_pages: strides {st} / {v.stride()}: a page must be contiguous, and both kinds equally far apart")
-        width = table.shape[-1]
-        if table.dtype is not torch.int32 or table.shape != (batch, width) or not table.is_contiguous() or table.get_device() != dev:
-            self._refuse("page_table", table, torch.int32, (batch, width))
-        if seq_len.dtype is not torch.int32 or seq_len.shape != (batch,) or not seq_len.is_contiguous() or seq_len.get_device() != dev:
-            self._refuse("seq_len", seq_len, torch.int32, (batch,))
-        if n_new is not None and (n_new.dtype is not torch.int32 or n_new.shape != (batch,) or not n_new.is_contiguous() or n_new.get_device() != dev):
-            self._refuse("n_new", n_new, torch.int32, (batch,))
-        return st[0] if n_pages > 1 else n_kv * ps * head_dim, n_pages, ps, width
+    def _why_pages(self, k, v, table, seq_len, n_new, batch, n_kv, head_dim):
+        if not isinstance(k, torch.Tensor) or k.dim() != 4:
+            raise ValueError(f"libquickprefill: k_pages must be [n_pages, {n_kv}, page_size, {head_dim}]")
+        n_pages, ps = k.shape[0], k.shape[2]
+        for name, t in (("k_pages", k), ("v_pages", v)):
+            self._need(name, t, torch.bfloat16, (n_pages, n_kv, ps, head_dim), False)
+        if k.stride() != v.stride() or k.stride()[1:] != (ps * head_dim, head_dim, 1):
+            raise ValueError(f"libquickprefill: k_pages / v_pages: strides {k.stride()} / {v.stride()}: a page must be contiguous, and both kinds equally far apart")
+        self._need("page_table", table, torch.int32, (batch, table.shape[-1]))
+        self._need("seq_len", seq_len, torch.int32, (batch,))
+        if n_new is not None:
+            self._need("n_new", n_new, torch.int32, (batch,))
+
+    def _why_append(self, qkv, cos, sin, seq_len, n_new, table, k_pages, v_pages, n_q, n_kv, head_dim, q_out):
+        B, T = qkv.shape[:2]
+        self._need("qkv", qkv, torch.bfloat16, (B, T, (n_q + 2 * n_kv) * head_dim))
+        self._need("q_out", q_out, torch.bfloat16, (B, T, n_q, head_dim))
+        for name, t in (("cos", cos), ("sin", sin)):
+            self._need(name, t, torch.bfloat16, None if t.numel() == B * T * head_dim // 2 else (B, T, head_dim // 2))
+        self._why_pages(k_pages, v_pages, table, seq_len, n_new, B, n_kv, head_dim)
 
     def batch_rope_append(self, qkv, cos, sin, seq_len, n_new, table, k_pages, v_pages, n_q, n_kv, head_dim, q_out):
         """qkv [B, T, (n_q + 2 n_kv) * D] -> q_out [B, T, n_q, D] rotated; rotated keys and values into the sequences' pages
         [n_pages, n_kv, page_size, D] at rows seq_len[b] ...  cos / sin: bf16 [B, T, D/2] (or the [B * T, D/2] mrope_table returns).
         seq_len int32 [B], n_new int32 [B] or None (T each), table int32 [B, max_pages]."""
-        dev, bf16 = self._dev, torch.bfloat16
-        B, T, n = qkv.shape
-        stride, n_pages, ps, width = self._batch_pages(k_pages, v_pages, table, seq_len, n_new, B, n_kv, head_dim, dev)
-        if qkv.dtype is not bf16 or n != (n_q + 2 * n_kv) * head_dim or not qkv.is_contiguous() or qkv.get_device() != dev:
-            self._refuse("qkv", qkv, bf16, (B, T, (n_q + 2 * n_kv) * head_dim))
-        if q_out.dtype is not bf16 or q_out.shape != (B, T, n_q, head_dim) or not q_out.is_contiguous() or q_out.get_device() != dev:
-            self._refuse("q_out", q_out, bf16, (B, T, n_q, head_dim))
-        need = B * T * head_dim // 2
-        if cos.dtype is not bf16 or cos.numel() != need or not cos.is_contiguous() or cos.get_device() != dev:
-            self._refuse("cos", cos, bf16, (B, T, head_dim // 2) if cos.numel() != need else None)
-        if sin.dtype is not bf16 or sin.numel() != need or not sin.is_contiguous() or sin.get_device() != dev:
-            self._refuse("sin", sin, bf16, (B, T, head_dim // 2) if sin.numel() != need else None)
-        self._check(self.lib.qp_batch_rope_append(self.ctx, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), B, T, seq_len.data_ptr(), _ptr(n_new), n_q, n_kv,
-                                                  head_dim, q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), stride, n_pages, ps, table.data_ptr(),
-                                                  width, self._stream_of(dev)))
+        rc = self._face.batch_rope_append(self._fns["qp_batch_rope_append"], self.ctx.value or 0, self._dev, self._stream_of(self._dev), qkv, cos, sin, seq_len, n_new,
+                                          table, k_pages, v_pages, n_q, n_kv, head_dim, q_out)
+        if rc:
+            self._after(rc, self._why_append, qkv, cos, sin, seq_len, n_new, table, k_pages, v_pages, n_q, n_kv, head_dim, q_out)
 
     def batch_attn_workspace(self, batch, t_max, prefix_len, suffix_capacity, n_q, n_kv):
         """Scratch of a batch_attn call of this size; one per stream (or captured graph) that may run at the same time."""
@@ -478,32 +489,27 @@ class QuickPrefillOps:
             raise ValueError(f"libquickprefill: no batch of {batch} x {t_max} rows over {prefix_len} + {suffix_capacity} keys with {n_q} / {n_kv} heads")
         return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
 
+    def _why_attn(self, q, k_prefix, v_prefix, prefix_head_stride, prefix_len, k_pages, v_pages, table, seq_len, n_new, n_q, n_kv, head_dim, scale, out, workspace):
+        B, T = q.shape[:2]
+        self._need("q", q, torch.bfloat16, (B, T, n_q, head_dim))
+        self._need("out", out, torch.bfloat16, (B, T, n_q, head_dim))
+        if prefix_len > 0:
+            for name, t in (("k_prefix", k_prefix), ("v_prefix", v_prefix)):
+                self._need(name, t, torch.bfloat16, None, False)
+                if prefix_head_stride < 0 or t.untyped_storage().nbytes() // 2 - t.storage_offset() < (n_kv - 1) * prefix_head_stride + prefix_len * head_dim:
+                    raise ValueError(f"libquickprefill: {name} holds fewer than {prefix_len} rows of {n_kv} heads {prefix_head_stride} elements apart")
+        self._need("workspace", workspace, workspace.dtype)
+        self._why_pages(k_pages, v_pages, table, seq_len, n_new, B, n_kv, head_dim)
+
     def batch_attn(self, q, k_prefix, v_prefix, prefix_head_stride, prefix_len, k_pages, v_pages, table, seq_len, n_new, n_q, n_kv, head_dim, scale, out,
                    workspace):
         """q, out [B, T, n_q, D]: attention of every row over the shared prefix rows [0, prefix_len) (k_prefix / v_prefix as in prefill_attn, None
         without a prefix) and its sequence's pages up to and including its own row."""
-        dev, bf16 = self._dev, torch.bfloat16
-        B, T = q.shape[:2]
-        stride, n_pages, ps, width = self._batch_pages(k_pages, v_pages, table, seq_len, n_new, B, n_kv, head_dim, dev)
-        shape = (B, T, n_q, head_dim)
-        if q.dtype is not bf16 or q.shape != shape or not q.is_contiguous() or q.get_device() != dev:
-            self._refuse("q", q, bf16, shape)
-        if out.dtype is not bf16 or out.shape != shape or not out.is_contiguous() or out.get_device() != dev:
-            self._refuse("out", out, bf16, shape)
-        kp = vp = None
-        if prefix_len > 0:
-            elements = (n_kv - 1) * prefix_head_stride + prefix_len * head_dim
-            for name, t in (("k_prefix", k_prefix), ("v_prefix", v_prefix)):
-                if t.dtype is not bf16 or t.get_device() != dev:
-                    self._refuse(name, t, bf16, None, False)
-                if t.numel() < elements and t.untyped_storage().nbytes() // 2 - t.storage_offset() < elements:
-                    raise ValueError(f"libquickprefill: {name} holds fewer than {prefix_len} rows of {n_kv} heads {prefix_head_stride} elements apart")
-            kp, vp = k_prefix.data_ptr(), v_prefix.data_ptr()
-        if workspace.get_device() != dev or not workspace.is_contiguous():
-            self._refuse("workspace", workspace, workspace.dtype)
-        self._check(self.lib.qp_batch_attn(self.ctx, q.data_ptr(), kp, vp, prefix_head_stride, prefix_len, k_pages.data_ptr(), v_pages.data_ptr(), stride,
-                                           n_pages, ps, table.data_ptr(), width, seq_len.data_ptr(), _ptr(n_new), B, T, n_q, n_kv, head_dim, scale,
-                                           out.data_ptr(), workspace.data_ptr(), workspace.nbytes, self._stream_of(dev)))
+        rc = self._face.batch_attn(self._fns["qp_batch_attn"], self.ctx.value or 0, self._dev, self._stream_of(self._dev), q, k_prefix, v_prefix, prefix_head_stride,
+                                   prefix_len, k_pages, v_pages, table, seq_len, n_new, n_q, n_kv, head_dim, scale, out, workspace)
+        if rc:
+            self._after(rc, self._why_attn, q, k_prefix, v_prefix, prefix_head_stride, prefix_len, k_pages, v_pages, table, seq_len, n_new, n_q, n_kv, head_dim,
+                        scale, out, workspace)
 
     def verify_drafts_workspace(self, batch, t_max, vocab):
         nbytes = int(self.lib.qp_verify_drafts_workspace_bytes(batch, t_max, vocab))
@@ -511,44 +517,31 @@ class QuickPrefillOps:
             raise ValueError(f"libquickprefill: no verification of {batch} x {t_max} drafts over {vocab} tokens")
         return torch.empty(nbytes, dtype=torch.uint8, device=self.device)
 
+    def _why_verify(self, logits, drafts, n_draft, draft_probs, uniforms, temperature, n_accepted, tokens, workspace):
+        B, T, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+        if logits.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"libquickprefill: logits are {logits.dtype}, torch.bfloat16 or torch.float32 is needed")
+        for name, t, dtype, shape in (("logits", logits, logits.dtype, (B, T + 1, V)), ("draft_probs", draft_probs, torch.float32, (B, T, V))):
+            if t is not None:
+                self._need(name, t, dtype, shape, False)
+                if t.numel() and V > 1 and t.stride(2) != 1:
+                    raise ValueError(f"libquickprefill: {name}: rows must be contiguous")
+        self._need("drafts", drafts, torch.int64, (B, T))
+        if n_draft is not None:
+            self._need("n_draft", n_draft, torch.int32, (B,))
+        if uniforms is not None:
+            self._need("uniforms", uniforms, torch.float32, (B, T + 1))
+        self._need("n_accepted", n_accepted, torch.int32, (B,))
+        self._need("tokens", tokens, torch.int64, (B, T + 1))
+        self._need("workspace", workspace, workspace.dtype)
+
     def verify_drafts(self, logits, drafts, n_draft, draft_probs, uniforms, temperature, n_accepted, tokens, workspace):
         """logits [B, T + 1, V] (bf16 or fp32, rows contiguous), drafts int64 [B, T], n_draft int32 [B] or None, draft_probs fp32 [B, T, V] or None,
         uniforms fp32 [B, T + 1] (None when temperature is 0) -> n_accepted int32 [B], tokens int64 [B, T + 1]."""
-        dev = self._dev
-        B, rows, V = logits.shape
-        T = rows - 1
-        f32 = logits.dtype is torch.float32
-        if not f32 and logits.dtype is not torch.bfloat16:
-            raise ValueError(f"libquickprefill: logits are {logits.dtype}, torch.bfloat16 or torch.float32 is needed")
-        if logits.get_device() != dev:
-            self._refuse("logits", logits, logits.dtype, None, False)
-        s0, s1, s2 = logits.stride()
-        if s2 != 1 and V > 1:
-            raise ValueError("libquickprefill: logits: rows must be contiguous")
-        pp, p0, p1 = None, 0, 0
-        if draft_probs is not None and T:
-            if draft_probs.dtype is not torch.float32 or draft_probs.shape != (B, T, V) or draft_probs.get_device() != dev:
-                self._refuse("draft_probs", draft_probs, torch.float32, (B, T, V), False)
-            p0, p1, p2 = draft_probs.stride()
-            if p2 != 1 and V > 1:
-                raise ValueError("libquickprefill: draft_probs: rows must be contiguous")
-            pp = draft_probs.data_ptr()
-        if drafts.dtype is not torch.int64 or drafts.shape != (B, T) or not drafts.is_contiguous() or drafts.get_device() != dev:
-            self._refuse("drafts", drafts, torch.int64, (B, T))
-        if n_draft is not None and (n_draft.dtype is not torch.int32 or n_draft.shape != (B,) or not n_draft.is_contiguous() or n_draft.get_device() != dev):
-            self._refuse("n_draft", n_draft, torch.int32, (B,))
-        if uniforms is not None and (uniforms.dtype is not torch.float32 or uniforms.shape != (B, rows) or not uniforms.is_contiguous() or
-                                     uniforms.get_device() != dev):
-            self._refuse("uniforms", uniforms, torch.float32, (B, rows))
-        if n_accepted.dtype is not torch.int32 or n_accepted.shape != (B,) or not n_accepted.is_contiguous() or n_accepted.get_device() != dev:
-            self._refuse("n_accepted", n_accepted, torch.int32, (B,))
-        if tokens.dtype is not torch.int64 or tokens.shape != (B, rows) or not tokens.is_contiguous() or tokens.get_device() != dev:
-            self._refuse("tokens", tokens, torch.int64, (B, rows))
-        if workspace.get_device() != dev or not workspace.is_contiguous():
-            self._refuse("workspace", workspace, workspace.dtype)
-        self._check(self.lib.qp_verify_drafts(self.ctx, logits.data_ptr(), f32, s0, s1, drafts.data_ptr() if T else None, _ptr(n_draft), pp, p0, p1,
-                                              _ptr(uniforms), B, T, V, temperature, n_accepted.data_ptr(), tokens.data_ptr(), workspace.data_ptr(),
-                                              workspace.nbytes, self._stream_of(dev)))
+        rc = self._face.verify_drafts(self._fns["qp_verify_drafts"], self.ctx.value or 0, self._dev, self._stream_of(self._dev), logits, drafts, n_draft, draft_probs,
+                                      uniforms, temperature, n_accepted, tokens, workspace)
+        if rc:
+            self._after(rc, self._why_verify, logits, drafts, n_draft, draft_probs, uniforms, temperature, n_accepted, tokens, workspace)
 
     # -- vision front end
     def vit_rope(self, qkv, cos, sin, heads, head_dim):

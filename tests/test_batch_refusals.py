@@ -95,9 +95,12 @@ def test_workspace_sizes(lib, ctx):
 
 @pytest.fixture
 def ops(ctx):
-    o = object.__new__(native.QuickPrefillOps)          # no GPU: everything below is refused before a pointer or a stream is taken
-    o.lib, o.ctx, o.device, o._dev = native.load_library(), None, torch.device("cuda", 0), -1          # -1: where torch says CPU tensors are
-    return o
+    o = object.__new__(native.QuickPrefillOps)          # no GPU: everything below is refused before a pointer is taken
+    o.lib, o.ctx, o.device = native.load_library(), ctypes.c_void_p(None), torch.device("cuda", 0)
+    o._bind_face()
+    o._dev, o._stream_of = -1, lambda dev: 0            # -1: where torch says CPU tensors are
+    yield o
+    o.ctx = None
 
 
 def batch_tensors(B=2, T=3, hq=4, hkv=2, ps=4, pages=6, width=3):
@@ -140,9 +143,41 @@ def test_python_verify_refuses(ops, name, make, word):
 
 
 def test_python_workspaces_refuse(ops, ctx):
-    ops.ctx = ctx[0]
+    ops.ctx = ctypes.c_void_p(ctx[0])
     with pytest.raises(ValueError, match="no batch"):
         ops.batch_attn_workspace(0, 1, 10, 16, 28, 4)
     with pytest.raises(ValueError, match="no verification"):
         ops.verify_drafts_workspace(1, 256, 1000)
-    ops.ctx = None
+
+
+def test_python_good_calls_reach_the_library(ops):
+    """Well-formed tensors pass the face and end at the library's own first check (no context here)."""
+    with pytest.raises(ValueError, match="qp_batch_rope_append: NULL"):
+        ops.batch_rope_append(*batch_tensors().values())
+    kw = batch_tensors()
+    q, kp = torch.zeros(2, 3, 4, 128, dtype=torch.bfloat16), torch.zeros(2, 10, 128, dtype=torch.bfloat16)
+    attn = [q, kp, kp, 1280, 10, kw["k_pages"], kw["v_pages"], kw["table"], kw["seq_len"], None, 4, 2, 128, 0.1, q.clone(), torch.zeros(64, dtype=torch.uint8)]
+    with pytest.raises(ValueError, match="qp_batch_attn: NULL"):
+        ops.batch_attn(*attn)
+    for at, bad, word in ((4, 11, "fewer"), (3, 1408, "fewer"), (1, kp.float(), "float32"), (0, q[:, :2], "contiguous"), (14, q.transpose(0, 1), "shape"), (15, torch.zeros(8, 8).t(), "contiguous"),
+                          (5, kw["k_pages"][0], "n_pages"), (10, 8, "shape")):
+        with pytest.raises(ValueError, match=word):
+            ops.batch_attn(*[bad if i == at else v for i, v in enumerate(attn)])
+    with pytest.raises(ValueError, match="qp_verify_drafts: NULL"):
+        ops.verify_drafts(torch.zeros(2, 3, 7), torch.zeros(2, 2, dtype=torch.int64), None, None, torch.zeros(2, 3), 1.0, torch.zeros(2, dtype=torch.int32),
+                          torch.zeros(2, 3, dtype=torch.int64), torch.zeros(4096, dtype=torch.uint8))
+    with pytest.raises(TypeError):
+        ops._face.batch_attn(1, 2)
+    for name in ("qkv", "table", "n_new"):
+        kw = batch_tensors()
+        kw[name] = "no tensor"
+        with pytest.raises((ValueError, AttributeError)):
+            ops.batch_rope_append(*kw.values())
+
+
+def test_missing_face_fails_loudly(monkeypatch):
+    import sys
+    monkeypatch.setitem(sys.modules, "quickvideo_amd._qp_torch", None)
+    monkeypatch.delattr("quickvideo_amd._qp_torch", raising=False)
+    with pytest.raises(native.QuickPrefillUnavailable, match="_qp_torch"):
+        native.load_face()
