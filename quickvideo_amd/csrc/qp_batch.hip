@@ -96,13 +96,41 @@ struct BatchAttnParams {
   const uint4* k_pre; const uint4* v_pre; int64_t pre_hs16; int64_t P;
   const uint4* k_pages; const uint4* v_pages;
   Pages pg;
-  int t_max, hq, hkv, G; float c;
+  int batch, t_max, hq, hkv, G; float c;
   int64_t R;
-  int ns, nrb;                    // prefix: key ranges, row blocks (per kv head)
-  int ns2, nrb2;                  // pages: key ranges, row blocks (per sequence and kv head)
-  unsigned page_wgs;              // batch * hkv * nrb2 * ns2
-  float* part_o; float2* part_ml; // [hkv][ns + ns2][R] rows of 128 floats / (max, sum)
+  // prefix: `prefix_wgs` workgroups share (row blocks of the batch's live rows) x (key ranges, ns_max at most) as split_prefix() says
+  unsigned prefix_wgs; int ns_max; bool compact;
+  float* pre_o; float2* pre_ml;   // [hkv][ns][live rows] rows of 128 floats / (max, sum)
+  int* starts;                    // with `compact`: [batch + 1] live tokens before a sequence, left for the joining kernel
+  // pages: ns2 key ranges, nrb2 row blocks per sequence and kv head
+  int ns2, nrb2; unsigned page_wgs;
+  float* part_o; float2* part_ml; // [hkv][ns2][R]
+  // many tokens: the prefix parts come from the prefill kernel (qp_attn_s6.hip) in its own layout, `wide_ns` per item of wide_rows tokens and a head
+  const float* wide; int wide_rows, wide_ns, wide_nqb;
 };
+
+// A padded batch (n_new given) is computed without its padding: the live tokens are numbered through, row = (live token) * G + g, and the workgroups are
+// dealt over as many row blocks as that makes, so that with few live rows every block's keys are cut into more ranges.
+constexpr int kMaxCompact = 512;  // sequences whose counts fit in LDS (a larger padded batch is computed with its padding)
+struct Split { int64_t rows; int nrb, ns; };
+__host__ __device__ inline Split split_prefix(int64_t tokens, int G, int block_rows, unsigned wgs, int hkv, int ns_max) {
+  Split s;
+  s.rows = tokens * G;
+  s.nrb = (int)((s.rows + block_rows - 1) / block_rows);
+  const int ns = s.nrb ? (int)(wgs / (unsigned)s.nrb / 8 * 8) / hkv : 1;       // 8: see the mapping of workgroups to XCDs
+  s.ns = ns < 1 ? 1 : (ns < ns_max ? ns : ns_max);
+  return s;
+}
+// live token -> b * t_max + t
+__device__ __forceinline__ int64_t token_place(const BatchAttnParams& p, const int* starts, int64_t tok) {
+  if (!p.compact) return tok;
+  int lo = 0, hi = p.batch;                                    // starts[lo] <= tok < starts[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= (int)tok) lo = mid; else hi = mid;
+  }
+  return (int64_t)lo * p.t_max + (tok - starts[lo]);
+}
 
 constexpr float kTiny = 1e-38f;   // least weight of a key or range that is seen: an infinite value shows however small its probability
 constexpr int kMaxKeys = 1 << 30; // of the prefix, and of a sequence's table: key numbers and their sums fit in 32 bits
@@ -126,7 +154,8 @@ __device__ __forceinline__ void make_finite(uint4& x) {       // such numbers to
 // The rare end of a range: every value that is not finite is added, times its probability, to the rows that see it, where their partial results
 // lie (one thread per row: it wrote none of them itself, the barrier before the call orders the writes).
 template <bool kPaged>
-__device__ __forceinline__ void add_odd_values(const BatchAttnParams& p, int kvh, int b, int64_t row0, int64_t row_end, int k0, int k1, int64_t slot0) {
+__device__ __forceinline__ void add_odd_values(const BatchAttnParams& p, int kvh, int b, int64_t row0, int64_t row_end, int k0, int k1, float* part_o,
+                                               const float2* part_ml, const int* starts) {
   for (int key = k0; key < k1; ++key) {
     const int64_t at = kPaged ? page_row16(p.pg, b, kvh, key) : (int64_t)kvh * p.pre_hs16 + (int64_t)key * 16;
     if (at < 0) continue;
@@ -136,15 +165,15 @@ __device__ __forceinline__ void add_odd_values(const BatchAttnParams& p, int kvh
     if (!odd) continue;                                        // (the same for all threads)
     const uint16_t* krow = reinterpret_cast<const uint16_t*>((kPaged ? p.k_pages : p.k_pre) + at);
     for (int64_t r = row0 + threadIdx.x; r < row_end; r += blockDim.x) {
-      const int64_t bt = r / p.G;
+      const int64_t bt = kPaged ? r / p.G : token_place(p, starts, r / p.G);
       if (kPaged && key > (int64_t)p.pg.seq_len[b] + (bt - (int64_t)b * p.t_max)) continue;
-      const uint16_t* qrow = reinterpret_cast<const uint16_t*>(p.q) + ((bt * p.hq) + (int64_t)kvh * p.G + (r - bt * p.G)) * 128;
+      const uint16_t* qrow = reinterpret_cast<const uint16_t*>(p.q) + ((bt * p.hq) + (int64_t)kvh * p.G + r % p.G) * 128;
       float s = 0.f;
       for (int d = 0; d < 128; ++d) s = __builtin_fmaf(bf16_bits_to_f32(qrow[d]), bf16_bits_to_f32(krow[d]), s);
-      const float pe = fmaxf(__builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c, -p.part_ml[slot0 + r].x * p.c)), kTiny);
+      const float pe = fmaxf(__builtin_amdgcn_exp2f(__builtin_fmaf(s, p.c, -part_ml[r].x * p.c)), kTiny);
       for (int d = 0; d < 128; ++d) {
         const uint16_t w = reinterpret_cast<const uint16_t*>(vrow)[d];
-        if ((w & 0x7f80u) == 0x7f80u) p.part_o[(slot0 + r) * 128 + d] += pe * bf16_bits_to_f32(w);
+        if ((w & 0x7f80u) == 0x7f80u) part_o[r * 128 + d] += pe * bf16_bits_to_f32(w);
       }
     }
   }
@@ -486,10 +515,9 @@ __device__ __forceinline__ void walk_alone(const BatchAttnParams& p, int kvh, in
 }
 
 // Q fragments of the lane's row, an empty running state and cleared flags (the first barrier of walk_keys orders the flags)
-__device__ __forceinline__ void begin_rows(const BatchAttnParams& p, int kvh, int64_t r, bool row_live, bf16x8_t (&qf)[8], Shared& sh, Rows& st) {
+__device__ __forceinline__ void begin_rows(const BatchAttnParams& p, int kvh, int64_t bt, int g, bool row_live, bf16x8_t (&qf)[8], Shared& sh, Rows& st) {
   const int tid = threadIdx.x, hi = (tid >> 5) & 1;
-  const int64_t bt = row_live ? r / p.G : 0;
-  const uint4* src = p.q + ((bt * p.hq) + (int64_t)kvh * p.G + (row_live ? (int)(r - bt * p.G) : 0)) * 16;
+  const uint4* src = p.q + ((bt * p.hq) + (int64_t)kvh * p.G + g) * 16;
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) {
     uint4 x = make_uint4(0, 0, 0, 0);
@@ -540,17 +568,22 @@ __device__ __forceinline__ float4 joined(const float* obuf, const float* lds_m, 
   return acc;
 }
 
-// one key range of one row block: partial results of its rows into part `part`
+// one key range of one row block: partial results of its rows r into part_o[r], part_ml[r].  Rows of the pages are numbered with the batch's padding
+// (b * t_max + t) * G + g, those of the prefix without it.
 template <int WR, int WK, bool kPaged>
-__device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int kvh, int b, int64_t row0, int64_t row_end, int k0, int k1, int part,
-                                                 unsigned char* lds, float* lds_ml, Shared& sh) {
+__device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int kvh, int b, int64_t row0, int64_t row_end, int k0, int k1, float* part_o,
+                                                 float2* part_ml, const int* starts, unsigned char* lds, float* lds_ml, Shared& sh) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, l31 = lane & 31;
   const int wr = wave % WR, wk = wave / WR;
   const int64_t r = row0 + wr * 32 + l31;
   const bool row_live = r < row_end, wave_live = row0 + wr * 32 < row_end;
   bf16x8_t qf[8];
   Rows st;
-  begin_rows(p, kvh, r, row_live, qf, sh, st);
+  {
+    const int64_t tok = row_live ? r / p.G : 0;
+    const int g = row_live ? (int)(r - tok * p.G) : 0;
+    begin_rows(p, kvh, row_live && !kPaged ? token_place(p, starts, tok) : tok, g, row_live, qf, sh, st);
+  }
   if (WR == 1) {
     __syncthreads();                                           // flags cleared
     walk_alone<WK, kPaged>(p, kvh, b, r, row_live, qf, k0, k1, wave, lds, sh, st);
@@ -558,7 +591,6 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
   } else {
     walk_keys<WR, WK, kPaged>(p, kvh, b, r, row_live, wave_live, qf, k0, k1, lds, sh, st);
   }
-  const int64_t slot0 = ((int64_t)kvh * (p.ns + p.ns2) + part) * p.R;
   if (WR == 1) {
     float* obuf = reinterpret_cast<float*>(lds);
     lay_out_rows<WK>(st, p.c, row_live, obuf, lds_ml, lds_ml + WK * 32);
@@ -567,8 +599,8 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
       const int row = i >> 5, d4 = (i & 31) * 4;
       float m, l;
       const float4 acc = joined<WK>(obuf, lds_ml, lds_ml + WK * 32, row, d4, m, l);
-      *reinterpret_cast<float4*>(p.part_o + (slot0 + row0 + row) * 128 + d4) = acc;
-      if (d4 == 0) p.part_ml[slot0 + row0 + row] = make_float2(m, l);
+      *reinterpret_cast<float4*>(part_o + (row0 + row) * 128 + d4) = acc;
+      if (d4 == 0) part_ml[row0 + row] = make_float2(m, l);
     }
   } else {
   f32x16_t (&o)[4] = st.o;
@@ -599,19 +631,19 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
     }
   }
   if (row_live && wk == 0) {
-    if (hi == 0) p.part_ml[slot0 + r] = make_float2(m_run, l_run);
+    if (hi == 0) part_ml[r] = make_float2(m_run, l_run);
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4)
-        *reinterpret_cast<float4*>(p.part_o + (slot0 + r) * 128 + db * 32 + 8 * q4 + 4 * hi) =
+        *reinterpret_cast<float4*>(part_o + r * 128 + db * 32 + 8 * q4 + 4 * hi) =
             make_float4(o[db][q4 * 4 + 0], o[db][q4 * 4 + 1], o[db][q4 * 4 + 2], o[db][q4 * 4 + 3]);
   }
   }
   if (k0 < k1 && sh.odd) {                                  // (read behind the loop's barriers)
     __threadfence_block();
     __syncthreads();
-    add_odd_values<kPaged>(p, kvh, b, row0, row0 + 32 * WR < row_end ? row0 + 32 * WR : row_end, k0, k1, slot0);
+    add_odd_values<kPaged>(p, kvh, b, row0, row0 + 32 * WR < row_end ? row0 + 32 * WR : row_end, k0, k1, part_o, part_ml, starts);
   }
 }
 
@@ -641,14 +673,41 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnPa
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];          // lds_of<WR, WK>()
   __shared__ float lds_ml[WR == 1 ? WK * 64 : WR * 64];
   __shared__ Shared sh;
+  __shared__ int starts[kMaxCompact + 1];
   if (blockIdx.x >= p.page_wgs) {
-    const unsigned w = blockIdx.x - p.page_wgs, turn = 8u * p.nrb;
+    const unsigned w = blockIdx.x - p.page_wgs;
+    int64_t tokens = (int64_t)p.batch * p.t_max;
+    if (p.compact) {
+      if (threadIdx.x < 64) {                                  // running sum of the counts
+        int carry = 0;
+        for (int b0 = 0; b0 < p.batch; b0 += 64) {
+          const int b = b0 + (int)threadIdx.x, v = b < p.batch ? rows_new(p.pg, b, p.t_max) : 0;
+          int incl = v;
+#pragma unroll
+          for (int k = 1; k < 64; k <<= 1) {
+            const int o = __shfl_up(incl, k, 64);
+            if ((int)threadIdx.x >= k) incl += o;
+          }
+          if (b < p.batch) starts[b] = carry + incl - v;
+          carry += __shfl(incl, 63, 64);
+        }
+        if (threadIdx.x == 0) starts[p.batch] = carry;
+      }
+      __syncthreads();
+      tokens = starts[p.batch];
+      if (w == 0)
+        for (int b = threadIdx.x; b <= p.batch; b += 64 * WR * WK) p.starts[b] = starts[b];
+    }
+    const Split sp = split_prefix(tokens, p.G, 32 * WR, p.prefix_wgs, p.hkv, p.ns_max);
+    if (sp.nrb == 0) return;
+    const unsigned turn = 8u * sp.nrb;
     const int item = (int)(w / turn) * 8 + (int)(w % 8), rb = (int)(w % turn) / 8;
-    if (item >= p.hkv * p.ns) return;
-    const int kvh = item / p.ns, split = item - kvh * p.ns;
+    if (item >= p.hkv * sp.ns) return;
+    const int kvh = item / sp.ns, split = item - kvh * sp.ns;
     int k0, k1;
-    key_range((int)p.P, p.ns, split, k0, k1);
-    batch_attn_range<WR, WK, false>(p, kvh, 0, (int64_t)rb * 32 * WR, p.R, k0, k1, split, lds, lds_ml, sh);
+    key_range((int)p.P, sp.ns, split, k0, k1);
+    const int64_t slot = ((int64_t)kvh * sp.ns + split) * sp.rows;
+    batch_attn_range<WR, WK, false>(p, kvh, 0, (int64_t)rb * 32 * WR, sp.rows, k0, k1, p.pre_o + slot * 128, p.pre_ml + slot, starts, lds, lds_ml, sh);
     return;
   }
   const int w = (int)blockIdx.x;
@@ -660,7 +719,8 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnPa
   key_range(stored_rows(p.pg, b, n_new), p.ns2, split, k0, k1);
   const int64_t seq_row0 = (int64_t)b * p.t_max * p.G, row0 = seq_row0 + (int64_t)rb * 32 * WR, row_end = seq_row0 + (int64_t)n_new * p.G;
   if (row0 >= row_end) return;
-  batch_attn_range<WR, WK, true>(p, kvh, b, row0, row_end, k0, k1, p.ns + split, lds, lds_ml, sh);
+  const int64_t slot = ((int64_t)kvh * p.ns2 + split) * p.R;
+  batch_attn_range<WR, WK, true>(p, kvh, b, row0, row_end, k0, k1, p.part_o + slot * 128, p.part_ml + slot, nullptr, lds, lds_ml, sh);
 }
 
 // Few keys: ONE launch.  The 8 waves of a workgroup deal the prefix's and the pages' 32-key blocks among themselves for the (at most 32) rows of one
@@ -681,7 +741,7 @@ __global__ __launch_bounds__(64 * kDirectWaves, 2) void batch_attn_direct_kernel
   const bool row_live = r < row_end;
   bf16x8_t qf[8];
   Rows st;
-  begin_rows(p, kvh, r, row_live, qf, sh, st);
+  begin_rows(p, kvh, row_live ? r / p.G : 0, row_live ? (int)(r % p.G) : 0, row_live, qf, sh, st);
   __syncthreads();                                             // flags cleared
   const int wave = tid >> 6, blocks = ((int)p.P + 31) / 32;
   walk_alone<kDirectWaves, false>(p, kvh, b, r, row_live, qf, 0, (int)p.P, wave, lds, sh, st);
@@ -716,8 +776,8 @@ __global__ __launch_bounds__(64 * kDirectWaves, 2) void batch_attn_direct_kernel
     if (pass == 0) {
       __threadfence_block();
       __syncthreads();
-      add_odd_values<false>(p, kvh, b, row0, row_end, 0, (int)p.P, slot0);
-      add_odd_values<true>(p, kvh, b, row0, row_end, 0, len, slot0);             // (a row's thread is the same in both)
+      add_odd_values<false>(p, kvh, b, row0, row_end, 0, (int)p.P, p.part_o + slot0 * 128, p.part_ml + slot0, nullptr);       // (compact is off: rows as they are)
+      add_odd_values<true>(p, kvh, b, row0, row_end, 0, len, p.part_o + slot0 * 128, p.part_ml + slot0, nullptr);           // (a row's thread is the same in both)
       __threadfence_block();
       __syncthreads();
     }
@@ -740,21 +800,27 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
   const int64_t r = w - (int64_t)kvh * p.R, bt = r / p.G;
   const int g = (int)(r - bt * p.G), b = (int)(bt / p.t_max), t = (int)(bt % p.t_max);
   if (t >= rows_new(p.pg, b, p.t_max)) return;                 // rows behind a sequence's last token stay as they are
-  const int np = p.ns + p.ns2;
-  const float2* ml = p.part_ml + (int64_t)kvh * np * p.R + r;
-  const float* po = p.part_o + ((int64_t)kvh * np * p.R + r) * 128 + lane32 * 4;
+  // parts 0 .. ns - 1: the prefix, row `live`; parts ns ...: the pages, row r
+  int64_t tokens = (int64_t)p.batch * p.t_max, live = r;
+  if (p.compact) { tokens = p.starts[p.batch]; live = (int64_t)(p.starts[b] + t) * p.G + g; }
+  const Split sp = p.ns_max ? split_prefix(tokens, p.G, p.wide_rows, p.prefix_wgs, p.hkv, p.ns_max) : Split{0, 0, 0};
+  const int np = sp.ns + p.ns2;
+  const float2 *ml0 = p.pre_ml + (int64_t)kvh * sp.ns * sp.rows + live, *ml1 = p.part_ml + (int64_t)kvh * p.ns2 * p.R + r;
+  const float *po0 = p.pre_o + ((int64_t)kvh * sp.ns * sp.rows + live) * 128 + lane32 * 4, *po1 = p.part_o + ((int64_t)kvh * p.ns2 * p.R + r) * 128 + lane32 * 4;
+  auto ml = [&](int i) { return i < sp.ns ? ml0[(int64_t)i * sp.rows] : ml1[(int64_t)(i - sp.ns) * p.R]; };
+  auto po = [&](int i) { return *reinterpret_cast<const float4*>(i < sp.ns ? po0 + (int64_t)i * sp.rows * 128 : po1 + (int64_t)(i - sp.ns) * p.R * 128); };
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
   if (kWide) {
     float M = -1e30f;
-    for (int i = tid; i < np; i += 256) M = fmaxf(M, ml[(int64_t)i * p.R].x);
+    for (int i = tid; i < np; i += 256) M = fmaxf(M, ml(i).x);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
     if (lane == 0) red[wave] = M;
     __syncthreads();
     M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     for (int i = tid; i < np; i += 256) {
-      const float2 x = ml[(int64_t)i * p.R];
+      const float2 x = ml(i);
       const float a = __builtin_amdgcn_exp2f((x.x - M) * p.c);
       lds_a[i] = x.y == 0.f ? 0.f : fmaxf(a, kTiny);           // an empty range left no o behind
       l = __builtin_fmaf(x.y, a, l);
@@ -772,7 +838,7 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
         const int i = i0 + k * GROUPS;
         a[k] = i < np ? lds_a[i] : 0.f;
         v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (a[k] != 0.f) v[k] = *reinterpret_cast<const float4*>(po + (int64_t)i * p.R * 128);
+        if (a[k] != 0.f) v[k] = po(i);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -781,7 +847,7 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
       }
     }
   } else {                                                     // np <= 64: lane i holds part i
-    const float2 x = lane < np ? ml[(int64_t)lane * p.R] : make_float2(-1e30f, 0.f);
+    const float2 x = lane < np ? ml(lane) : make_float2(-1e30f, 0.f);
     float M = x.x;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
@@ -799,7 +865,7 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
         ak[k] = __shfl(a, i & 63, 64);
         if (i >= np) ak[k] = 0.f;
         v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (ak[k] != 0.f) v[k] = *reinterpret_cast<const float4*>(po + (int64_t)i * p.R * 128);
+        if (ak[k] != 0.f) v[k] = po(i);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -829,39 +895,139 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
   *reinterpret_cast<uint2*>(p.out + ((bt * p.hq) + (int64_t)kvh * p.G + g) * 128 + lane32 * 4) = y;
 }
 
-struct Plan { bool direct; int wr, ns, nrb, ns2, nrb2; int64_t R; };
+// Many tokens over a long prefix: joins, for 32 tokens of a head and 32 of the 128 dimensions, the prefill kernel's partial results (a lane reads
+// what the lane of the same number wrote: [wave][d / 8][lane][4], then (max, sum) [wave][2][lane]) and those of the pages.
+__global__ __launch_bounds__(64) void batch_combine_wide_kernel(BatchAttnParams p) {
+  const int items = p.wide_nqb * p.G, item = blockIdx.x % items, kvh = blockIdx.x / items;
+  const int qb = p.wide_nqb - 1 - item / p.G, g = item % p.G, wave = blockIdx.y, db = blockIdx.z, lane = threadIdx.x, hi = lane >> 5;
+  const int64_t rows = p.R / p.G, bt = (int64_t)qb * p.wide_rows + wave * 32 + (lane & 31);
+  if ((int64_t)qb * p.wide_rows + wave * 32 >= rows) return;
+  const int b = bt < rows ? (int)(bt / p.t_max) : 0, t = bt < rows ? (int)(bt - (int64_t)b * p.t_max) : 0;
+  const bool live = bt < rows && t < rows_new(p.pg, b, p.t_max);
+  const int pf = qpattn::partial_floats(p.wide_rows);
+  const float* base = p.wide + (int64_t)(kvh * items + item) * p.wide_ns * pf;
+  const float* ml = base + p.wide_rows * 128 + wave * 128 + lane;
+  const int64_t r = live ? bt * p.G + g : 0;
+  const float2* pml = p.part_ml + (int64_t)kvh * p.ns2 * p.R + r;
+  float M = -1e30f;
+  for (int i = 0; i < p.wide_ns; ++i) M = fmaxf(M, ml[(int64_t)i * pf]);
+  if (live)
+    for (int i = 0; i < p.ns2; ++i) M = fmaxf(M, pml[(int64_t)i * p.R].x);
+  float l = 0.f;
+  f32x4_t acc[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) acc[k] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < p.wide_ns; ++i) {
+    const float m = ml[(int64_t)i * pf], a = m == -1e30f ? 0.f : fmaxf(__builtin_amdgcn_exp2f((m - M) * p.c), kTiny);
+    l = __builtin_fmaf(ml[(int64_t)i * pf + 64], a, l);
+    const f32x4_t* o = reinterpret_cast<const f32x4_t*>(base + (int64_t)i * pf) + (wave * 16 + db * 4) * 64 + lane;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] += o[k * 64] * a;
+  }
+  if (!live) return;
+  for (int i = 0; i < p.ns2; ++i) {
+    const float2 x = pml[(int64_t)i * p.R];
+    if (x.y == 0.f) continue;                                  // an empty range left no o behind
+    const float a = fmaxf(__builtin_amdgcn_exp2f((x.x - M) * p.c), kTiny);
+    l = __builtin_fmaf(x.y, a, l);
+    const float* o = p.part_o + ((int64_t)kvh * p.ns2 * p.R + (int64_t)i * p.R + r) * 128 + db * 32 + 4 * hi;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] += *reinterpret_cast<const f32x4_t*>(o + 8 * k) * a;
+  }
+  const float inv = l != 0.f ? 1.0f / l : 0.f;                 // a row that sees no key is zero
+  uint16_t* out = p.out + ((bt * p.hq) + (int64_t)kvh * p.G + g) * 128 + db * 32 + 4 * hi;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint2 y = make_uint2(0, 0);
+    if (l != 0.f) {
+      y.x = (unsigned)f32_to_bf16_bits(acc[k][0] * inv) | ((unsigned)f32_to_bf16_bits(acc[k][1] * inv) << 16);
+      y.y = (unsigned)f32_to_bf16_bits(acc[k][2] * inv) | ((unsigned)f32_to_bf16_bits(acc[k][3] * inv) << 16);
+    }
+    *reinterpret_cast<uint2*>(out + 8 * k) = y;
+  }
+}
 
-constexpr int64_t kDirectKeys = 1536;
+struct Plan {
+  enum { kDirect, kWide, kRanges } form;
+  int wr, ns2, nrb2, ns_max, wide_rows, wide_nqb, wide_ns;
+  int64_t R;
+  unsigned prefix_wgs;
+  bool compact, many_parts;
+};
 
-// Row blocks as wide as the batch's rows (up to 256), key ranges so many that every CU is busy once.
-Plan make_plan(const qp_ctx* ctx, int batch, int t_max, int64_t P, int64_t suffix_cap, int hq, int hkv) {
-  Plan pl;
+constexpr int64_t kDirectKeys = 1536, kWideTokens = 96;
+
+// ranges of a sequence's pages: about 256 keys each at most, fewer where sequences fill the card
+int page_ranges(int64_t wgs, int64_t seqs, int64_t suffix_cap, int most) {
+  int64_t ns2 = wgs / seqs;
+  const int64_t by_keys = (suffix_cap + 255) / 256;
+  if (ns2 > by_keys) ns2 = by_keys;
+  return (int)(ns2 < 1 ? 1 : (ns2 > most ? most : ns2));
+}
+
+// padded: n_new is given, so that tokens may be missing
+Plan make_plan(const qp_ctx* ctx, int batch, int t_max, bool padded, int64_t P, int64_t suffix_cap, int hq, int hkv) {
+  Plan pl = {};
   const int G = hq / hkv;
-  pl.R = (int64_t)batch * t_max * G;
-  pl.direct = t_max * G <= 32 && (int64_t)hkv * batch <= ctx->cus && P + suffix_cap <= kDirectKeys;
-  if (pl.direct) {
-    pl.wr = 1; pl.ns = 0; pl.ns2 = 1; pl.nrb = pl.nrb2 = 1;
+  const int64_t tokens = (int64_t)batch * t_max;
+  pl.R = tokens * G;
+  if (t_max * G <= 32 && (int64_t)hkv * batch <= ctx->cus && P + suffix_cap <= kDirectKeys) {
+    pl.form = Plan::kDirect;
+    pl.ns2 = 1;
     return pl;
   }
+  // Tokens enough to fill row blocks of the prefill kernel head by head, all of them there, and a prefix long enough that its masked tiles (one per 64
+  // tokens: it takes the last prefix row for a new one) do not count.  Its probabilities are rounded to bf16 once, as in every prefill of this library.
+  if (!padded && tokens >= kWideTokens && P >= 4 * tokens && P < (1 << 23)) {
+    pl.form = Plan::kWide;
+    const int64_t by128 = (tokens + 127) / 128 * 128, by256 = (tokens + 255) / 256 * 256;
+    pl.wide_rows = by128 < by256 ? 128 : 256;
+    pl.wide_nqb = (int)((tokens + pl.wide_rows - 1) / pl.wide_rows);
+    const int64_t items = (int64_t)hkv * G * pl.wide_nqb, slots = (int64_t)ctx->cus * (pl.wide_rows == 256 ? 1 : 2), tiles = (P + 63) / 64;
+    int64_t best = 0;
+    for (int ns = 1; ns <= 32 && ns * 8 <= tiles + 8; ++ns) {  // rounds of workgroups x (their tiles + what a range costs besides, about 4 tiles)
+      const int64_t cost = (items * ns + slots - 1) / slots * ((tiles + ns - 1) / ns + 4);
+      if (best == 0 || cost < best) { best = cost; pl.wide_ns = ns; }
+    }
+    pl.wr = pl.R / batch <= 64 ? 2 : 4;                        // the pages' own launch: narrow row blocks, many workgroups
+    pl.nrb2 = (int)(((int64_t)t_max * G + 32 * pl.wr - 1) / (32 * pl.wr));
+    pl.ns2 = page_ranges(2LL * ctx->cus, (int64_t)hkv * batch * pl.nrb2, suffix_cap, 16);
+    return pl;
+  }
+  // Row blocks as wide as the batch's rows (up to 256), key ranges so many that every CU is busy once.
+  pl.form = Plan::kRanges;
   pl.wr = pl.R <= 32 ? 1 : (pl.R <= 64 ? 2 : (pl.R <= 128 ? 4 : 8));
   const int rows = 32 * pl.wr, per_cu = pl.wr == 8 ? 1 : 2;     // resident workgroups (registers: two waves per SIMD)
-  pl.nrb = (int)((pl.R + rows - 1) / rows);
+  const int64_t nrb = (pl.R + rows - 1) / rows, slots = (int64_t)per_cu * ctx->cus;
   pl.nrb2 = (int)(((int64_t)t_max * G + rows - 1) / rows);
-  const int64_t slots = (int64_t)per_cu * ctx->cus, seqs = (int64_t)hkv * batch * pl.nrb2;
-  int64_t ns2 = slots / (4 * seqs);
-  const int64_t most2 = (suffix_cap + 255) / 256;
-  if (ns2 > most2) ns2 = most2;
-  pl.ns2 = (int)(ns2 < 1 ? 1 : (ns2 > 64 ? 64 : ns2));
-  const int64_t page_wgs = seqs * pl.ns2, left = page_wgs * 2 < slots ? slots - page_wgs : slots;
-  int64_t ns = left / ((int64_t)hkv * pl.nrb);
-  const int64_t least = pl.wr == 1 ? 128 : 64, most = (P + least - 1) / least;   // a tile per range at least
-  if (ns < 1) ns = 1;
-  if (ns > kMaxParts - 64) ns = kMaxParts - 64;
-  pl.ns = (int)(ns < most ? ns : most);
+  const int64_t seqs = (int64_t)hkv * batch * pl.nrb2;
+  pl.ns2 = page_ranges(slots / 4, seqs, suffix_cap, 32);
+  pl.compact = padded && t_max > 1 && batch <= kMaxCompact && P > 0;
+  if (P > 0) {
+    const int64_t page_wgs = seqs * pl.ns2, left = page_wgs * 2 < slots ? slots - page_wgs : slots, once = (hkv + 7) / 8 * 8 * nrb;
+    pl.prefix_wgs = (unsigned)(left > once ? left : once);
+    const int64_t least = pl.wr == 1 ? 128 : 64, most = (P + least - 1) / least;   // a tile per range at least
+    pl.many_parts = pl.R * hkv <= 4096;                        // few rows: a workgroup each joins any number of parts; many: a wave each, 64 parts at most
+    const int cap = pl.many_parts ? kMaxParts - 32 : 64 - pl.ns2;
+    pl.ns_max = (int)(most < cap ? most : cap);
+  }
   return pl;
 }
 
-size_t ml_bytes(const Plan& pl, int hkv) { return ((size_t)hkv * (pl.ns + pl.ns2) * pl.R * sizeof(float2) + 15) & ~(size_t)15; }
+// where things lie in the workspace
+struct Layout { size_t pre_o, pre_ml, part_o, part_ml, starts, wide, end; };
+Layout layout_of(const Plan& pl, int batch, int hq, int hkv) {
+  Layout l;
+  size_t at = 0;
+  auto take = [&](size_t bytes) { const size_t a = at; at += (bytes + 255) & ~(size_t)255; return a; };
+  const size_t pages = (size_t)hkv * pl.ns2 * pl.R, prefix = (size_t)pl.prefix_wgs * 32 * pl.wr;       // hkv * ns * live rows <= workgroups * block rows
+  l.pre_o = take(prefix * 512); l.pre_ml = take(prefix * sizeof(float2));
+  l.part_o = take(pages * 512); l.part_ml = take(pages * sizeof(float2));
+  l.starts = take(pl.compact ? ((size_t)batch + 1) * sizeof(int) : 0);
+  l.wide = take(pl.form == Plan::kWide ? (size_t)hq * pl.wide_nqb * pl.wide_ns * qpattn::partial_floats(pl.wide_rows) * sizeof(float) : 0);
+  l.end = at;
+  return l;
+}
 
 Pages pages_of(const int32_t* table, const int32_t* seq_len, const int32_t* n_new, int max_pages, int n_pages, int page_size, int64_t page_stride) {
   Pages pg;
@@ -896,34 +1062,56 @@ int qp_launch_batch_rope_append(const void* qkv, const void* cos, const void* si
 }
 
 size_t qp_batch_attn_workspace_bytes_impl(const qp_ctx* ctx, int batch, int t_max, int64_t P, int64_t suffix_cap, int hq, int hkv) {
-  const Plan pl = make_plan(ctx, batch, t_max, P, suffix_cap, hq, hkv);
-  return ml_bytes(pl, hkv) + (size_t)hkv * (pl.ns + pl.ns2) * pl.R * 128 * sizeof(float);
+  const size_t a = layout_of(make_plan(ctx, batch, t_max, false, P, suffix_cap, hq, hkv), batch, hq, hkv).end;
+  const size_t b = layout_of(make_plan(ctx, batch, t_max, true, P, suffix_cap, hq, hkv), batch, hq, hkv).end;
+  return a > b ? a : b;
 }
 
 int qp_launch_batch_attn(const qp_ctx* ctx, const void* q, const void* k_prefix, const void* v_prefix, int64_t prefix_head_stride, int64_t P,
                          const void* k_pages, const void* v_pages, int64_t page_stride, int n_pages, int page_size, const int32_t* table, int max_pages,
                          const int32_t* seq_len, const int32_t* n_new, int batch, int t_max, int hq, int hkv, float scale, void* out, void* workspace,
                          hipStream_t s) {
-  const Plan pl = make_plan(ctx, batch, t_max, P, (int64_t)max_pages * page_size, hq, hkv);
-  BatchAttnParams p;
+  const Plan pl = make_plan(ctx, batch, t_max, n_new != nullptr, P, (int64_t)max_pages * page_size, hq, hkv);
+  const Layout l = layout_of(pl, batch, hq, hkv);
+  char* ws = (char*)workspace;
+  BatchAttnParams p = {};
   p.q = (const uint4*)q; p.out = (uint16_t*)out;
   p.k_pre = (const uint4*)k_prefix; p.v_pre = (const uint4*)v_prefix; p.pre_hs16 = prefix_head_stride / 8; p.P = P;
   p.k_pages = (const uint4*)k_pages; p.v_pages = (const uint4*)v_pages;
   p.pg = pages_of(table, seq_len, n_new, max_pages, n_pages, page_size, page_stride);
-  p.t_max = t_max; p.hq = hq; p.hkv = hkv; p.G = hq / hkv; p.c = scale * 1.4426950408889634f;
-  p.R = pl.R; p.ns = pl.ns; p.nrb = pl.nrb; p.ns2 = pl.ns2; p.nrb2 = pl.nrb2;
+  p.batch = batch; p.t_max = t_max; p.hq = hq; p.hkv = hkv; p.G = hq / hkv; p.c = scale * 1.4426950408889634f;
+  p.R = pl.R; p.prefix_wgs = pl.prefix_wgs; p.ns_max = pl.ns_max; p.compact = pl.compact;
+  p.pre_o = (float*)(ws + l.pre_o); p.pre_ml = (float2*)(ws + l.pre_ml);
+  p.part_o = (float*)(ws + l.part_o); p.part_ml = (float2*)(ws + l.part_ml);
+  p.starts = (int*)(ws + l.starts);
+  p.ns2 = pl.ns2; p.nrb2 = pl.nrb2;
   p.page_wgs = (unsigned)((int64_t)hkv * batch * pl.nrb2 * pl.ns2);
-  p.part_ml = (float2*)workspace;
-  p.part_o = (float*)((char*)workspace + ml_bytes(pl, hkv));
-  if (pl.direct) {
+  int rc;
+  if (pl.form == Plan::kDirect) {
     static std::atomic<unsigned long long> opted{0};
-    int rc = qp_opt_in_lds(opted, (const void*)batch_attn_direct_kernel, kDirectLds, "batch_attn_direct");
-    if (rc) return rc;
+    if ((rc = qp_opt_in_lds(opted, (const void*)batch_attn_direct_kernel, kDirectLds, "batch_attn_direct"))) return rc;
     batch_attn_direct_kernel<<<(unsigned)(hkv * batch), 64 * kDirectWaves, kDirectLds, s>>>(p);
     return qp_check_launch("batch_attn(direct)");
   }
-  const unsigned grid = p.page_wgs + (unsigned)(((int64_t)hkv * pl.ns + 7) / 8 * 8 * pl.nrb);
-  int rc;
+  if (pl.form == Plan::kWide) {
+    if ((rc = pl.wr == 2 ? launch_ranges<2, 2>(p, p.page_wgs, s) : launch_ranges<4, 1>(p, p.page_wgs, s))) return rc;
+    qpattn::AttnParams a = {};
+    a.q = (const uint4*)q; a.kp = p.k_pre; a.vp = p.v_pre; a.pre_hs16 = p.pre_hs16; a.P = P - 1;
+    a.kn = p.k_pre + (P - 1) * 16; a.vn = p.v_pre + (P - 1) * 16; a.new_hs16 = p.pre_hs16; a.n = 1;       // token i sees new rows 0 .. i: the one there is
+    a.hq = hq; a.group = p.G; a.c = p.c; a.nqb = pl.wide_nqb; a.hkv = hkv; a.items = pl.wide_nqb * p.G;
+    a.n_whole = 0; a.nsplit = pl.wide_ns; a.ws = (float*)(ws + l.wide);          // every item leaves partial results
+    a.heads_per_seq = hkv; a.kv_row_bytes = 256;
+    a.nq = batch * t_max; a.qb_rows = pl.wide_rows;
+    const qp_dev_switches& dev = qp_dev();
+    a.prio_mode = (dev.s6_prio.load(std::memory_order_relaxed) & 3) | ((dev.s6_early_out.load(std::memory_order_relaxed) & 3) << 2);
+    qp_launch_attn_s6(a, hkv <= 8 && 8 % hkv == 0, (unsigned)(a.items * a.nsplit), s);
+    if ((rc = qp_check_launch("batch_attn(wide)"))) return rc;
+    p.wide = a.ws; p.wide_rows = pl.wide_rows; p.wide_ns = pl.wide_ns; p.wide_nqb = pl.wide_nqb;
+    batch_combine_wide_kernel<<<dim3((unsigned)(hkv * a.items), (unsigned)(pl.wide_rows / 32), 4), 64, 0, s>>>(p);
+    return qp_check_launch("batch_attn(wide combine)");
+  }
+  p.wide_rows = 32 * pl.wr;                                    // (the joining kernel needs the block's rows)
+  const unsigned grid = p.page_wgs + pl.prefix_wgs;
   switch (pl.wr) {
     case 1: rc = launch_ranges<1, 4>(p, grid, s); break;
     case 2: rc = launch_ranges<2, 2>(p, grid, s); break;
@@ -931,7 +1119,7 @@ int qp_launch_batch_attn(const qp_ctx* ctx, const void* q, const void* k_prefix,
     default: rc = launch_ranges<8, 1>(p, grid, s); break;
   }
   if (rc) return rc;
-  if (pl.ns + pl.ns2 > 32) batch_combine_kernel<true><<<(unsigned)(pl.R * hkv), 256, 0, s>>>(p);
+  if (pl.many_parts) batch_combine_kernel<true><<<(unsigned)(pl.R * hkv), 256, 0, s>>>(p);
   else batch_combine_kernel<false><<<(unsigned)((pl.R * hkv + 3) / 4), 256, 0, s>>>(p);
   return qp_check_launch("batch_attn(combine)");
 }

@@ -229,7 +229,7 @@ def check(got, ref, tol):
     inf = np.isinf(ref)
     assert np.array_equal(got[inf], ref[inf])
     ok = ~np.isnan(ref) & ~inf
-    bad = np.abs(got - ref)[ok] - tol[ok]
+    bad = np.abs(got[ok] - ref[ok]) - tol[ok]
     assert (bad <= 0).all(), bad.max()
 
 
@@ -260,6 +260,55 @@ def test_attn(ops, hq, hkv, P, ps, seq, new, T):
     check(got, ref, tol)
     again = run_attn(ops, qd, kpre, vpre, P, bt, hq, D ** -0.5)          # no order that changes: the same bits
     assert np.array_equal(f64(got), f64(again), equal_nan=True)
+
+
+@pytest.mark.parametrize("hq,hkv,P,ps,seq,T", [
+    (8, 1, 500, 16, [3, 0], 62), (7, 7, 1030, 16, [30, 5, 0], 40), (28, 4, 1024, 24, [9, 100], 128), (4, 2, 2000, 16, [0], 129), (12, 2, 700, 16, list(range(100)), 1),
+    (16, 1, 4100, 16, [7], 300), (6, 3, 999, 1, [2, 1, 4], 32),
+])
+def test_attn_full_batches_of_many_tokens(ops, hq, hkv, P, ps, seq, T):
+    """n_new None: many tokens over a longer prefix go through the prefill kernel, head by head (its probabilities are rounded once: within the bound)."""
+    bt = Batch(hkv, ps, seq, [T] * len(seq), T, seed=P)
+    bt.fill([s + T for s in seq])
+    kpre, vpre = prefix_of(bt, P)
+    q = bt.randn(bt.B, T, hq, D, scale=1.3)
+    ref, tol = attn_ref(q, kpre, vpre, P, bt, hq, D ** -0.5)
+    check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5, n_new=None), ref, tol)
+    check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5), ref, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,P,B,T", [(8, 2, 300, 100, 3), (4, 1, 700, 65, 9), (4, 2, 129, 600, 2), (2, 2, 64, 513, 3), (28, 4, 400, 5, 61), (4, 1, 2500, 512, 2)])
+@pytest.mark.parametrize("fill", ["some", "one", "none"])
+def test_attn_padded_batches(ops, hq, hkv, P, B, T, fill):
+    """Most places of the batch empty: only the live tokens count, wherever they are."""
+    rs = np.random.RandomState(B + T)
+    new = rs.randint(0, T + 1, B) * (rs.rand(B) < 0.5) if fill == "some" else np.zeros(B, dtype=int)
+    if fill == "one":
+        new[B // 2] = T
+    seq = rs.randint(0, 20, B)
+    bt = Batch(hkv, 4, seq.tolist(), new.tolist(), T, seed=B)
+    bt.fill([s + n for s, n in zip(bt.seq, bt.new)])
+    kpre, vpre = prefix_of(bt, P)
+    q = torch.full((B, T, hq, D), float("nan"), dtype=torch.bfloat16)               # what a dead row holds must not matter
+    for b in range(B):
+        q[b, :bt.new[b]] = bt.randn(bt.new[b], hq, D, scale=1.3)
+    ref, tol = attn_ref(q, kpre, vpre, P, bt, hq, D ** -0.5)
+    check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5), ref, tol)
+
+
+@pytest.mark.parametrize("P", [50, 3000])
+@pytest.mark.parametrize("T,B", [(1, 2), (5, 3), (70, 2)])
+def test_attn_infinite_values_in_the_prefix(ops, P, T, B):
+    """A value row of the prefix that is not finite reaches every row that sees it (all of them), through every form of the operator, and no other column."""
+    for n_new in ("given", None):
+        bt = Batch(2, 16, [5] * B, [T] * B, T, seed=T)
+        bt.fill([5 + T] * B)
+        kpre, vpre = prefix_of(bt, P)
+        vpre[0, P // 2, 3] = float("inf"); vpre[1, P - 1, 100] = float("-inf"); vpre[1, 0, 7] = float("nan")
+        q = bt.randn(B, T, 8, D)
+        ref, tol = attn_ref(q, kpre, vpre, P, bt, 8, D ** -0.5)
+        assert np.isinf(ref[:, :, :4, 3]).all() and np.isinf(ref[:, :, 4:, 100]).all() and np.isnan(ref[:, :, 4:, 7]).all() and np.isfinite(ref[:, :, :4, :3]).all()
+        check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, 8, D ** -0.5, n_new=n_new), ref, tol)
 
 
 @pytest.mark.parametrize("sigma,scale", [(0.0, D ** -0.5), (12.0, D ** -0.5), (150.0, D ** -0.5), (1.0, 3.0), (1.0, 1e-4)])
