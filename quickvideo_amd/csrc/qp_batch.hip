@@ -7,6 +7,7 @@
 //   batch_rope_append_kernel   rotates the step's q and k rows and stores k / v into the pages
 //   batch_attn_kernel          attention of (batch x t_max) query rows over (shared prefix, own pages): partial results per key range
 //   batch_combine_kernel       joins the partial results of a row
+#include <type_traits>
 #include "qp_attn.h"
 
 namespace {
@@ -216,7 +217,7 @@ __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int
                                           int k1, unsigned char* lds, Shared& sh, Rows& st) {
   using S = Shape<WR, WK>;
   constexpr int NT = S::NT, PT = S::PT, KB = S::KB, TILE = S::TILE;
-  constexpr bool kAhead = !kPaged || PT < 8;                   // (with 64 registers a thread in flight the paged form would spill)
+  constexpr bool kAhead = !kPaged;                             // (the paged form would spill; pages are short)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, l31 = lane & 31;
   const int wk = wave / WR;
   unsigned char* kl = lds;
@@ -293,39 +294,47 @@ __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int
     if (kPaged && tid < 4) sh.holes[par ^ 1][tid] = 0;         // last read before the barrier above, next written behind the next one
     if (kAhead && t0 + TILE < k1) load(t0 + TILE);
     if (!wave_live) continue;
-    f32x16_t s[KB];
+    int ko = koff;
+    asm volatile("" : "+v"(ko));                             // (eight addresses derived again in each tile, not kept in eight registers)
+    // LDS reads run ahead of the products that need them: hipcc left to itself reads each fragment just before its use and waits for it
+    auto read_k = [&](int kb, bf16x8_t (&f)[8]) {
 #pragma unroll
-    for (int k = 0; k < KB; ++k) {
-      const int kb = WK >= 2 ? wk : k;
-      s[k] = (f32x16_t){0};
+      for (int kk = 0; kk < 8; ++kk) f[kk] = lds_read_b128(kl, kb * 32 * 256 + (ko ^ (kk << 5)));
+    };
+    auto read_v = [&](int kb, int cc, s16x8_t (&v)[4]) {       // the 16 keys of chunk cc, all 128 dimensions
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        if (PT >= 8 && kk == 4) __builtin_amdgcn_sched_barrier(0);               // (half of the K fragments at a time: registers)
-        s[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lds_read_b128(kl, kb * 32 * 256 + (koff ^ (kk << 5))), qf[kk], s[k], 0, 0, 0);
+      for (int db = 0; db < 4; ++db) {
+        const int off = voff + (((kb * 8 + cc * 4) * 4 + db) << 8);
+        const s16x4_t v0 = lds_read_tr16(vl, off);
+        const s16x4_t v1 = lds_read_tr16(vl, off + (2 * 4 << 8));
+        v[db] = (s16x8_t){v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
       }
-    }
-    __builtin_amdgcn_sched_barrier(0);                         // (keeps hipcc from holding K, V and the next tile in registers at once)
-    if (t0 + TILE > k1 || masked || hole_bits) {
-      const int last = (limit < k1 ? limit : k1 - 1) - t0 - 4 * hi;              // last visible row of the tile, seen from this lane's rows
-      const unsigned long long here = ~hole_bits >> (4 * hi);
+    };
+    auto scores = [&](const bf16x8_t (&f)[8]) {
+      f32x16_t s = (f32x16_t){0};
 #pragma unroll
-      for (int k = 0; k < KB; ++k) {
-        const int kb = WK >= 2 ? wk : k;
-        const unsigned have = (unsigned)(here >> ((kb & 1) * 32));
+      for (int kk = 0; kk < 8; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[kk], qf[kk], s, 0, 0, 0);
+      return s;
+    };
+    auto hide = [&](int kb, f32x16_t& s) {                     // scores of keys this lane's row does not see
+      if (t0 + TILE > k1 || masked || hole_bits) {
+        const int last = (limit < k1 ? limit : k1 - 1) - t0 - 4 * hi;              // last visible row of the tile, seen from this lane's rows
+        const unsigned have = (unsigned)((~hole_bits >> (4 * hi)) >> ((kb & 1) * 32));
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int row = (e & 3) + 8 * (e >> 2);
-          s[k][e] = kb * 32 + row <= last && ((have >> row) & 1) ? s[k][e] : -INFINITY;
+          s[e] = kb * 32 + row <= last && ((have >> row) & 1) ? s[e] : -INFINITY;
         }
       }
-    }
-    float mx = s[0][0];
+    };
+    auto largest = [&](const f32x16_t& s) {
+      float mx = s[0];
 #pragma unroll
-    for (int k = 0; k < KB; ++k)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[k][e]);
-    mx = xhalf_max(mx);
-    if (!__all((mx - m_run) * p.c <= 8.0f)) {                  // the reference moves only when a row outgrows it by 2^8
+      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
+      return xhalf_max(mx);
+    };
+    auto outgrown = [&](float mx) { return !__all((mx - m_run) * p.c <= 8.0f); };       // the reference moves only when a row outgrows it by 2^8
+    auto move_reference = [&](float mx) {
       const float m_new = fmaxf(m_run, mx);
       const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * p.c);
       m_run = m_new;
@@ -334,39 +343,112 @@ __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int
       for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
-    }
-    const float mc = m_run * p.c;
-    float rs = 0.f;
-#pragma unroll
-    for (int k = 0; k < KB; ++k) {
-      const int kb = WK >= 2 ? wk : k;
-      u32x4_t pf[2], pr[2];
+      return alpha;
+    };
+    auto exponentials = [&](const f32x16_t& s, u32x4_t (&pf)[2], u32x4_t (&pr)[2]) {
+      const float mc = m_run * p.c;
+      float rs = 0.f;
 #pragma unroll
       for (int cc = 0; cc < 2; ++cc)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][cc * 8 + 2 * e], p.c, -mc));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][cc * 8 + 2 * e + 1], p.c, -mc));
+          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cc * 8 + 2 * e], p.c, -mc));
+          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cc * 8 + 2 * e + 1], p.c, -mc));
           rs += p0 + p1;
           unsigned h, l;
           split_pair(p0, p1, h, l);
           pf[cc][e] = h; pr[cc][e] = l;
         }
-      __builtin_amdgcn_sched_barrier(0);
+      return rs;                                               // (this half's keys)
+    };
+    auto product = [&](int i, const s16x8_t (&va)[4], const s16x8_t (&vb)[4], const u32x4_t (&pf)[2], const u32x4_t (&pr)[2]) {       // i-th of a block's 16
+      const int db = i & 3;
+      const s16x8_t v = i < 8 ? va[db] : vb[db];
+      const u32x4_t pp = ((i >> 2) & 1 ? pr : pf)[i >> 3];
+      o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, pp), o[db], 0, 0, 0);
+    };
+    // exponentials() dealt among MFMAS matrix instructions, mfma(0) ... mfma(MFMAS - 1): a wave issues in order, so what is to run beside a matrix
+    // instruction has to stand behind it, and the fences keep it there (left to itself hipcc puts all of one kind first)
+    auto exponentials_beside = [&](auto mfmas, auto&& mfma, const f32x16_t& s, u32x4_t (&pf)[2], u32x4_t (&pr)[2]) {
+      constexpr int N = decltype(mfmas)::value, EACH = 16 / N;
+      const float mc = m_run * p.c;
+      float rs = 0.f, pe[16];
+      auto pack = [&](int q) {                                 // the q-th pair
+        rs += pe[2 * q] + pe[2 * q + 1];
+        unsigned h, l;
+        split_pair(pe[2 * q], pe[2 * q + 1], h, l);
+        pf[q >> 2][q & 3] = h; pr[q >> 2][q & 3] = l;
+      };
 #pragma unroll
-      for (int cc = 0; cc < 2; ++cc) {
+      for (int i = 0; i < N; ++i) {
+        mfma(i);
 #pragma unroll
-        for (int db = 0; db < 4; ++db) {
-          const int off = voff + (((kb * 8 + cc * 4) * 4 + db) << 8);
-          const s16x4_t v0 = lds_read_tr16(vl, off);
-          const s16x4_t v1 = lds_read_tr16(vl, off + (2 * 4 << 8));
-          const s16x8_t av = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), __builtin_bit_cast(bf16x8_t, pf[cc]), o[db], 0, 0, 0);
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, av), __builtin_bit_cast(bf16x8_t, pr[cc]), o[db], 0, 0, 0);
-        }
+        for (int u = 0; u < EACH; ++u) pe[i * EACH + u] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i * EACH + u], p.c, -mc));
+        if (i * EACH >= 2 && (i * EACH) % 2 == 0) pack(i * EACH / 2 - 1);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      pack(7);
+      asm volatile("" : "+v"(pf[0]), "+v"(pf[1]), "+v"(pr[0]), "+v"(pr[1]));      // (made here, not sunk to their use)
+      return rs;
+    };
+#define QP_BATCH_FENCE() __builtin_amdgcn_sched_barrier(0)
+    if constexpr (KB == 1 || kPaged) {
+#pragma unroll
+    for (int kb = KB == 1 ? wk : 0, n = 0; n < KB; ++n, ++kb) {
+      bf16x8_t kf[8];
+      s16x8_t va[4], vb[4];
+      u32x4_t pf[2], pr[2];
+      read_k(kb, kf);
+      QP_BATCH_FENCE();
+      f32x16_t s = scores(kf);
+      read_v(kb, 0, va);
+      QP_BATCH_FENCE();
+      hide(kb, s);
+      const float mx = largest(s);
+      if (outgrown(mx)) move_reference(mx);
+      l_run += xhalf_sum(exponentials(s, pf, pr));
+      QP_BATCH_FENCE();
+      read_v(kb, 1, vb);
+      QP_BATCH_FENCE();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) product(i, va, vb, pf, pr);
+      QP_BATCH_FENCE();
     }
-    l_run += xhalf_sum(rs);
+    } else {
+      // Both blocks' scores, then the first one's products beside the second one's exponentials.
+      s16x8_t va[4], vb[4];
+      u32x4_t pf0[2], pr0[2], pf1[2], pr1[2];
+      f32x16_t s0, s1;
+      {
+        bf16x8_t f[8];
+        read_k(0, f);
+        QP_BATCH_FENCE();
+        s0 = scores(f);
+      }
+      QP_BATCH_FENCE();
+      {
+        bf16x8_t f[8];
+        read_k(1, f);
+        QP_BATCH_FENCE();
+        hide(0, s0);
+        s1 = scores(f);
+      }
+      QP_BATCH_FENCE();
+      read_v(0, 0, va);
+      QP_BATCH_FENCE();
+      hide(1, s1);
+      float mx = fmaxf(largest(s0), largest(s1));
+      if (outgrown(mx)) move_reference(mx);
+      float rs = exponentials(s0, pf0, pr0);
+      QP_BATCH_FENCE();
+      rs += exponentials_beside(std::integral_constant<int, 16>(), [&](int i) { if (i == 4) read_v(0, 1, vb); product(i, va, vb, pf0, pr0); }, s1, pf1, pr1);
+      read_v(1, 0, va);
+      read_v(1, 1, vb);
+      QP_BATCH_FENCE();
+      l_run += xhalf_sum(rs);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) product(i, va, vb, pf1, pr1);
+    }
   }
   st.m = m_run; st.l = l_run;
 }
