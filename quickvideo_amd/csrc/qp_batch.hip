@@ -289,7 +289,7 @@ __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int
       *reinterpret_cast<uint4*>(vl + (((row >> 2) * 4 + (slot16 >> 2)) << 8) + ((row & 3) << 6) + ((slot16 & 3) << 4)) = vx[i];
     }
     __syncthreads();
-    const int word = WK >= 2 ? wk >> 1 : 0;                    // this wave's keys lie in one 64-key word of the mask
+    const int word = wk * KB / 2;                              // this wave's keys lie in one 64-key word of the mask
     const unsigned long long hole_bits = kPaged ? sh.holes[par][word] : 0;
     if (kPaged && tid < 4) sh.holes[par ^ 1][tid] = 0;         // last read before the barrier above, next written behind the next one
     if (kAhead && t0 + TILE < k1) load(t0 + TILE);
@@ -394,7 +394,8 @@ __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int
 #define QP_BATCH_FENCE() __builtin_amdgcn_sched_barrier(0)
     if constexpr (KB == 1 || kPaged) {
 #pragma unroll
-    for (int kb = KB == 1 ? wk : 0, n = 0; n < KB; ++n, ++kb) {
+    for (int n = 0; n < KB; ++n) {
+      const int kb = wk * KB + n;
       bf16x8_t kf[8];
       s16x8_t va[4], vb[4];
       u32x4_t pf[2], pr[2];
@@ -416,34 +417,35 @@ __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int
     }
     } else {
       // Both blocks' scores, then the first one's products beside the second one's exponentials.
+      const int kb = wk * KB;
       s16x8_t va[4], vb[4];
       u32x4_t pf0[2], pr0[2], pf1[2], pr1[2];
       f32x16_t s0, s1;
       {
         bf16x8_t f[8];
-        read_k(0, f);
+        read_k(kb, f);
         QP_BATCH_FENCE();
         s0 = scores(f);
       }
       QP_BATCH_FENCE();
       {
         bf16x8_t f[8];
-        read_k(1, f);
+        read_k(kb + 1, f);
         QP_BATCH_FENCE();
-        hide(0, s0);
+        hide(kb, s0);
         s1 = scores(f);
       }
       QP_BATCH_FENCE();
-      read_v(0, 0, va);
+      read_v(kb, 0, va);
       QP_BATCH_FENCE();
-      hide(1, s1);
+      hide(kb + 1, s1);
       float mx = fmaxf(largest(s0), largest(s1));
       if (outgrown(mx)) move_reference(mx);
       float rs = exponentials(s0, pf0, pr0);
       QP_BATCH_FENCE();
-      rs += exponentials_beside(std::integral_constant<int, 16>(), [&](int i) { if (i == 4) read_v(0, 1, vb); product(i, va, vb, pf0, pr0); }, s1, pf1, pr1);
-      read_v(1, 0, va);
-      read_v(1, 1, vb);
+      rs += exponentials_beside(std::integral_constant<int, 16>(), [&](int i) { if (i == 4) read_v(kb, 1, vb); product(i, va, vb, pf0, pr0); }, s1, pf1, pr1);
+      read_v(kb + 1, 0, va);
+      read_v(kb + 1, 1, vb);
       QP_BATCH_FENCE();
       l_run += xhalf_sum(rs);
 #pragma unroll
@@ -689,14 +691,14 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
   float m_run = st.m, l_run = st.l;
   if (WK == 2) {                                               // join the two key halves of a row (the tile's LDS is free)
     __syncthreads();
-    float* obuf = reinterpret_cast<float*>(lds);               // [WR][32 rows][128]
+    float* obuf = reinterpret_cast<float*>(lds);               // [WR][32 rows][kJoinRow]
     if (wk == 1) {
       if (hi == 0) { lds_ml[(wr * 32 + l31) * 2] = m_run; lds_ml[(wr * 32 + l31) * 2 + 1] = l_run; }
 #pragma unroll
       for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4)
-          *reinterpret_cast<float4*>(obuf + (wr * 32 + l31) * 128 + db * 32 + 8 * q4 + 4 * hi) =
+          *reinterpret_cast<float4*>(obuf + (wr * 32 + l31) * kJoinRow + db * 32 + 8 * q4 + 4 * hi) =
               make_float4(o[db][q4 * 4 + 0], o[db][q4 * 4 + 1], o[db][q4 * 4 + 2], o[db][q4 * 4 + 3]);
     }
     __syncthreads();
@@ -709,7 +711,13 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[db][e] = o[db][e] * a0 + obuf[(wr * 32 + l31) * 128 + db * 32 + 8 * (e >> 2) + 4 * hi + (e & 3)] * a1;
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const float4 other = *reinterpret_cast<const float4*>(obuf + (wr * 32 + l31) * kJoinRow + db * 32 + 8 * q4 + 4 * hi);
+        o[db][q4 * 4 + 0] = o[db][q4 * 4 + 0] * a0 + other.x * a1;
+        o[db][q4 * 4 + 1] = o[db][q4 * 4 + 1] * a0 + other.y * a1;
+        o[db][q4 * 4 + 2] = o[db][q4 * 4 + 2] * a0 + other.z * a1;
+        o[db][q4 * 4 + 3] = o[db][q4 * 4 + 3] * a0 + other.w * a1;
+      }
     }
   }
   if (row_live && wk == 0) {
@@ -727,6 +735,20 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
     __syncthreads();
     add_odd_values<kPaged>(p, kvh, b, row0, row0 + 32 * WR < row_end ? row0 + 32 * WR : row_end, k0, k1, part_o, part_ml, starts);
   }
+}
+
+// A row block that is at most half full (the last one; a padded batch's only one; a sequence's pages) is taken by WR / 2 x 2 waves, which deal the keys of
+// a tile among two: no wave is without rows.
+template <int WR, int WK, bool kPaged>
+__device__ __forceinline__ void batch_attn_block(const BatchAttnParams& p, int kvh, int b, int64_t row0, int64_t row_end, int k0, int k1, float* part_o,
+                                                 float2* part_ml, const int* starts, unsigned char* lds, float* lds_ml, Shared& sh) {
+  if constexpr (WK == 1) {
+    if (row_end - row0 <= 16 * WR) {
+      batch_attn_range<WR / 2, 2, kPaged>(p, kvh, b, row0, row_end, k0, k1, part_o, part_ml, starts, lds, lds_ml, sh);
+      return;
+    }
+  }
+  batch_attn_range<WR, WK, kPaged>(p, kvh, b, row0, row_end, k0, k1, part_o, part_ml, starts, lds, lds_ml, sh);
 }
 
 // range `split` of n keys cut into `ns` ranges of whole 64-key tiles (the last ones may be empty: k0 >= k1)
@@ -747,8 +769,8 @@ __device__ __forceinline__ int stored_rows(const Pages& pg, int b, int n_new) {
 // they run on the same XCD (workgroups go to the 8 XCDs in turn) and share its L2.
 template <int WR, int WK>
 constexpr int lds_of() {
-  constexpr int tiles = 2 * Shape<WR, WK>::TILE * 256;
-  return WR == 1 && join_bytes<WK>() > tiles ? join_bytes<WK>() : tiles;
+  constexpr int tiles = 2 * Shape<WR, WK>::TILE * 256, join = WR == 1 ? join_bytes<WK>() : (WK == 1 ? WR / 2 : WR) * 32 * kJoinRow * 4;      // (WK = 1: of the narrow form)
+  return join > tiles ? join : tiles;
 }
 template <int WR, int WK>
 __global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnParams p) {
@@ -789,7 +811,7 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnPa
     int k0, k1;
     key_range((int)p.P, sp.ns, split, k0, k1);
     const int64_t slot = ((int64_t)kvh * sp.ns + split) * sp.rows;
-    batch_attn_range<WR, WK, false>(p, kvh, 0, (int64_t)rb * 32 * WR, sp.rows, k0, k1, p.pre_o + slot * 128, p.pre_ml + slot, starts, lds, lds_ml, sh);
+    batch_attn_block<WR, WK, false>(p, kvh, 0, (int64_t)rb * 32 * WR, sp.rows, k0, k1, p.pre_o + slot * 128, p.pre_ml + slot, starts, lds, lds_ml, sh);
     return;
   }
   const int w = (int)blockIdx.x;
@@ -802,7 +824,7 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnPa
   const int64_t seq_row0 = (int64_t)b * p.t_max * p.G, row0 = seq_row0 + (int64_t)rb * 32 * WR, row_end = seq_row0 + (int64_t)n_new * p.G;
   if (row0 >= row_end) return;
   const int64_t slot = ((int64_t)kvh * p.ns2 + split) * p.R;
-  batch_attn_range<WR, WK, true>(p, kvh, b, row0, row_end, k0, k1, p.part_o + slot * 128, p.part_ml + slot, nullptr, lds, lds_ml, sh);
+  batch_attn_block<WR, WK, true>(p, kvh, b, row0, row_end, k0, k1, p.part_o + slot * 128, p.part_ml + slot, nullptr, lds, lds_ml, sh);
 }
 
 // Few keys: ONE launch.  The 8 waves of a workgroup deal the prefix's and the pages' 32-key blocks among themselves for the (at most 32) rows of one
@@ -1039,10 +1061,10 @@ struct Plan {
 
 constexpr int64_t kDirectKeys = 1536, kWideTokens = 96;
 
-// ranges of a sequence's pages: about 256 keys each at most, fewer where sequences fill the card
-int page_ranges(int64_t wgs, int64_t seqs, int64_t suffix_cap, int most) {
+// ranges of a sequence's pages: `keys` each, fewer ranges where sequences fill the card
+int page_ranges(int64_t wgs, int64_t seqs, int64_t suffix_cap, int most, int64_t keys = 256) {
   int64_t ns2 = wgs / seqs;
-  const int64_t by_keys = (suffix_cap + 255) / 256;
+  const int64_t by_keys = (suffix_cap + keys - 1) / keys;
   if (ns2 > by_keys) ns2 = by_keys;
   return (int)(ns2 < 1 ? 1 : (ns2 > most ? most : ns2));
 }
@@ -1083,7 +1105,9 @@ Plan make_plan(const qp_ctx* ctx, int batch, int t_max, bool padded, int64_t P, 
   const int64_t nrb = (pl.R + rows - 1) / rows, slots = (int64_t)per_cu * ctx->cus;
   pl.nrb2 = (int)(((int64_t)t_max * G + rows - 1) / rows);
   const int64_t seqs = (int64_t)hkv * batch * pl.nrb2;
-  pl.ns2 = page_ranges(slots / 4, seqs, suffix_cap, 32);
+  // A page's key costs about twice a prefix's (two loads one behind the other, no tile ahead): no workgroup of the pages runs longer than one of the prefix.
+  const int64_t even = P * hkv * nrb / slots / 2;
+  pl.ns2 = page_ranges(slots / 4, seqs, suffix_cap, 32, even > 256 ? even : 256);
   pl.compact = padded && t_max > 1 && batch <= kMaxCompact && P > 0;
   if (P > 0) {
     const int64_t page_wgs = seqs * pl.ns2, left = page_wgs * 2 < slots ? slots - page_wgs : slots, once = (hkv + 7) / 8 * 8 * nrb;
