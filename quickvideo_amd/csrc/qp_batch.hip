@@ -192,6 +192,7 @@ __device__ __forceinline__ void add_odd_values(const BatchAttnParams& p, int kvh
 template <int WR, int WK>
 struct Shape {
   static constexpr int NT = 64 * WR * WK, KB = WK == 1 ? 2 : 1, TILE = 32 * WK * KB, PT = TILE * 16 / NT;   // PT: 16-B pieces a thread stages of K and of V
+  static constexpr int kBuffers = NT == 512 ? 3 : 2;
 };
 struct Rows {                      // what a lane keeps of its row (both halves of a wave: the same row, other keys)
   f32x16_t o[4];                   // [d / 32], unscaled
@@ -212,12 +213,175 @@ struct Shared {                    // LDS besides the tile
   int odd;                         // a value that is not finite was met
 };
 
+#define QP_BATCH_FENCE() __builtin_amdgcn_sched_barrier(0)
+
+// The matrix work of one wave on KB 32-key blocks (kb0 ...) of a staged tile.  `hidden`: some key of the tile is not seen by some row; then this lane's
+// row sees rows up to last_row of the tile, without those of hole_bits.  kBeside (two blocks): the first one's products run beside the second one's
+// exponentials; otherwise block after block.
+template <int KB, bool kBeside>
+__device__ __forceinline__ void take_tile(float c, const unsigned char* kl, const unsigned char* vl, int koff, int voff, int kb0, const bf16x8_t (&qf)[8],
+                                          bool hidden, int last_row, unsigned long long hole_bits, int hi, float& m_run, float& l_run, f32x16_t (&o)[4]) {
+  // LDS reads run ahead of the products that need them: hipcc left to itself reads each fragment just before its use and waits for it
+  auto read_k = [&](int kb, bf16x8_t (&f)[8]) {
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) f[kk] = lds_read_b128(kl, kb * 32 * 256 + (koff ^ (kk << 5)));
+  };
+  auto read_v = [&](int kb, int cc, s16x8_t (&v)[4]) {       // the 16 keys of chunk cc, all 128 dimensions
+#pragma unroll
+    for (int db = 0; db < 4; ++db) {
+      const int off = voff + (((kb * 8 + cc * 4) * 4 + db) << 8);
+      const s16x4_t v0 = lds_read_tr16(vl, off);
+      const s16x4_t v1 = lds_read_tr16(vl, off + (2 * 4 << 8));
+      v[db] = (s16x8_t){v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+    }
+  };
+  auto scores = [&](const bf16x8_t (&f)[8]) {
+    f32x16_t s = (f32x16_t){0};
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[kk], qf[kk], s, 0, 0, 0);
+    return s;
+  };
+  auto hide = [&](int kb, f32x16_t& s) {                     // scores of keys this lane's row does not see
+    if (hidden) {
+      const int last = last_row - 4 * hi;                    // (seen from this lane's rows)
+      const unsigned have = (unsigned)((~hole_bits >> (4 * hi)) >> ((kb & 1) * 32));
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int row = (e & 3) + 8 * (e >> 2);
+        s[e] = kb * 32 + row <= last && ((have >> row) & 1) ? s[e] : -INFINITY;
+      }
+    }
+  };
+  auto largest = [&](const f32x16_t& s) {
+    float mx = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
+    return xhalf_max(mx);
+  };
+  auto outgrown = [&](float mx) { return !__all((mx - m_run) * c <= 8.0f); };       // the reference moves only when a row outgrows it by 2^8
+  auto move_reference = [&](float mx) {
+    const float m_new = fmaxf(m_run, mx);
+    const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * c);
+    m_run = m_new;
+    l_run *= alpha;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
+    return alpha;
+  };
+  auto exponentials = [&](const f32x16_t& s, u32x4_t (&pf)[2], u32x4_t (&pr)[2]) {
+    const float mc = m_run * c;
+    float rs = 0.f;
+#pragma unroll
+    for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cc * 8 + 2 * e], c, -mc));
+        const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cc * 8 + 2 * e + 1], c, -mc));
+        rs += p0 + p1;
+        unsigned h, l;
+        split_pair(p0, p1, h, l);
+        pf[cc][e] = h; pr[cc][e] = l;
+      }
+    return rs;                                               // (this half's keys)
+  };
+  auto product = [&](int i, const s16x8_t (&va)[4], const s16x8_t (&vb)[4], const u32x4_t (&pf)[2], const u32x4_t (&pr)[2]) {       // i-th of a block's 16
+    const int db = i & 3;
+    const s16x8_t v = i < 8 ? va[db] : vb[db];
+    const u32x4_t pp = ((i >> 2) & 1 ? pr : pf)[i >> 3];
+    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, pp), o[db], 0, 0, 0);
+  };
+  // exponentials() dealt among MFMAS matrix instructions, mfma(0) ... mfma(MFMAS - 1): a wave issues in order, so what is to run beside a matrix
+  // instruction has to stand behind it, and the fences keep it there (left to itself hipcc puts all of one kind first)
+  auto exponentials_beside = [&](auto mfmas, auto&& mfma, const f32x16_t& s, u32x4_t (&pf)[2], u32x4_t (&pr)[2]) {
+    constexpr int N = decltype(mfmas)::value, EACH = 16 / N;
+    const float mc = m_run * c;
+    float rs = 0.f, pe[16];
+    auto pack = [&](int q) {                                 // the q-th pair
+      rs += pe[2 * q] + pe[2 * q + 1];
+      unsigned h, l;
+      split_pair(pe[2 * q], pe[2 * q + 1], h, l);
+      pf[q >> 2][q & 3] = h; pr[q >> 2][q & 3] = l;
+    };
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      mfma(i);
+#pragma unroll
+      for (int u = 0; u < EACH; ++u) pe[i * EACH + u] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i * EACH + u], c, -mc));
+      if (i * EACH >= 2 && (i * EACH) % 2 == 0) pack(i * EACH / 2 - 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    pack(7);
+    asm volatile("" : "+v"(pf[0]), "+v"(pf[1]), "+v"(pr[0]), "+v"(pr[1]));      // (made here, not sunk to their use)
+    return rs;
+  };
+  if constexpr (!kBeside) {
+#pragma unroll
+  for (int n = 0; n < KB; ++n) {
+    const int kb = kb0 + n;
+    bf16x8_t kf[8];
+    s16x8_t va[4], vb[4];
+    u32x4_t pf[2], pr[2];
+    read_k(kb, kf);
+    QP_BATCH_FENCE();
+    f32x16_t s = scores(kf);
+    read_v(kb, 0, va);
+    QP_BATCH_FENCE();
+    hide(kb, s);
+    const float mx = largest(s);
+    if (outgrown(mx)) move_reference(mx);
+    l_run += xhalf_sum(exponentials(s, pf, pr));
+    QP_BATCH_FENCE();
+    read_v(kb, 1, vb);
+    QP_BATCH_FENCE();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) product(i, va, vb, pf, pr);
+    QP_BATCH_FENCE();
+  }
+  } else {
+    // Both blocks' scores, then the first one's products beside the second one's exponentials.
+    const int kb = kb0;
+    s16x8_t va[4], vb[4];
+    u32x4_t pf0[2], pr0[2], pf1[2], pr1[2];
+    f32x16_t s0, s1;
+    {
+      bf16x8_t f[8];
+      read_k(kb, f);
+      QP_BATCH_FENCE();
+      s0 = scores(f);
+    }
+    QP_BATCH_FENCE();
+    {
+      bf16x8_t f[8];
+      read_k(kb + 1, f);
+      QP_BATCH_FENCE();
+      hide(kb, s0);
+      s1 = scores(f);
+    }
+    QP_BATCH_FENCE();
+    read_v(kb, 0, va);
+    QP_BATCH_FENCE();
+    hide(kb + 1, s1);
+    float mx = fmaxf(largest(s0), largest(s1));
+    if (outgrown(mx)) move_reference(mx);
+    float rs = exponentials(s0, pf0, pr0);
+    QP_BATCH_FENCE();
+    rs += exponentials_beside(std::integral_constant<int, 16>(), [&](int i) { if (i == 4) read_v(kb, 1, vb); product(i, va, vb, pf0, pr0); }, s1, pf1, pr1);
+    read_v(kb + 1, 0, va);
+    read_v(kb + 1, 1, vb);
+    QP_BATCH_FENCE();
+    l_run += xhalf_sum(rs);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) product(i, va, vb, pf1, pr1);
+  }
+}
+
 template <int WR, int WK, bool kPaged>
 __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int b, int64_t r, bool row_live, bool wave_live, const bf16x8_t (&qf)[8], int k0,
                                           int k1, unsigned char* lds, Shared& sh, Rows& st) {
   using S = Shape<WR, WK>;
   constexpr int NT = S::NT, PT = S::PT, KB = S::KB, TILE = S::TILE;
-  constexpr bool kAhead = !kPaged;                             // (the paged form would spill; pages are short)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = lane >> 5, l31 = lane & 31;
   const int wk = wave / WR;
   unsigned char* kl = lds;
@@ -268,9 +432,8 @@ __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int
   f32x16_t (&o)[4] = st.o;
   float m_run = st.m, l_run = st.l;
   int par = 0;
-  if (kAhead && k0 < k1) load(k0);
   for (int t0 = k0; t0 < k1; t0 += TILE, par ^= 1) {
-    if (!kAhead) load(t0);
+    load(t0);
     __syncthreads();                                           // everyone has read the previous tile
     const bool masked = kPaged && t0 + TILE > seen_by_all;    // some row of the sequence does not see some key of this tile
     u16x2_t top = {0, 0};
@@ -292,165 +455,67 @@ __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int
     const int word = wk * KB / 2;                              // this wave's keys lie in one 64-key word of the mask
     const unsigned long long hole_bits = kPaged ? sh.holes[par][word] : 0;
     if (kPaged && tid < 4) sh.holes[par ^ 1][tid] = 0;         // last read before the barrier above, next written behind the next one
-    if (kAhead && t0 + TILE < k1) load(t0 + TILE);
     if (!wave_live) continue;
-    int ko = koff;
-    asm volatile("" : "+v"(ko));                             // (eight addresses derived again in each tile, not kept in eight registers)
-    // LDS reads run ahead of the products that need them: hipcc left to itself reads each fragment just before its use and waits for it
-    auto read_k = [&](int kb, bf16x8_t (&f)[8]) {
+    take_tile<KB, false>(p.c, kl, vl, koff, voff, wk * KB, qf, t0 + TILE > k1 || masked || hole_bits, (limit < k1 ? limit : k1 - 1) - t0, hole_bits, hi, m_run,
+                         l_run, o);
+  }
+  st.m = m_run; st.l = l_run;
+}
+
+// The prefix's keys k0 .. k1 - 1 without a look at the values: tiles go from memory straight into LDS (buffer_load ... lds: 1 KB, four rows, per wave and
+// instruction, lane i's 16 B at 16 i; the images are made by what each lane reads), kBuffers of them, so that the next ones are under way while one is
+// computed, with one barrier a tile.  Rows behind k1 read as zero (the buffer's bound).  The loads are asm, each with its own wait before the barrier:
+// hipcc would otherwise wait for all of them at the first LDS read.
+__device__ __forceinline__ void load_to_lds(unsigned lds_at, int voff, u32x4_t rsrc) {       // (the wait states: rsrc may come from a vector instruction)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds_at), "v"(voff), "s"(rsrc) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
+
+template <int WR, int WK>
+__device__ __forceinline__ void walk_prefix(const BatchAttnParams& p, int kvh, bool wave_live, bf16x8_t (&qf)[8], int k0, int k1, unsigned char* lds, Rows& st) {
+  using S = Shape<WR, WK>;
+  constexpr int KB = S::KB, TILE = S::TILE, NW = WR * WK, NB = S::kBuffers, PIECES = TILE / 4 / NW;      // 1-KB pieces a wave loads of K and of V
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, l31 = lane & 31, wk = wave / WR;
+  const int koff = l31 * 256 + ((hi ^ (l31 & 15)) << 4);
+  const int voff = (((lane & 15) >> 2) << 6) + (((lane >> 4) & 1) << 5) + ((lane & 3) << 3) + (hi << 10);
+  const int krow = wave * 4 + (lane >> 4), ksrc = krow * 256 + (((lane & 15) ^ (krow & 15)) << 4);       // piece j: + j * NW * 1024 (NW * 4 rows, a multiple of 16)
+  const int vsrc = (wave * 4 + ((lane >> 2) & 3)) * 256 + ((lane >> 4) << 6) + ((lane & 3) << 4);
+  static_assert(NW * 4 % 16 == 0, "the swizzle repeats every 16 rows");
+  const unsigned lds32 = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char*)lds + wave * 1024;
+  const unsigned char* kbase = reinterpret_cast<const unsigned char*>(p.k_pre + (int64_t)kvh * p.pre_hs16);
+  const unsigned char* vbase = reinterpret_cast<const unsigned char*>(p.v_pre + (int64_t)kvh * p.pre_hs16);
+  auto rsrc_of = [&](const unsigned char* base, int t0) {
+    const size_t at = (size_t)(base + (int64_t)t0 * 256);
+    const int rows = k1 - t0 < TILE ? k1 - t0 : TILE;
+    return (u32x4_t){(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)at), (unsigned)__builtin_amdgcn_readfirstlane((int)((unsigned)(at >> 32) & 0xffffu)),
+                     (unsigned)__builtin_amdgcn_readfirstlane(rows * 256), 0x00020000u};
+  };
+  auto load = [&](int t0, int buf) {
+    const u32x4_t rk = rsrc_of(kbase, t0), rv = rsrc_of(vbase, t0);
+    const unsigned at = lds32 + buf * (TILE * 512);
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk) f[kk] = lds_read_b128(kl, kb * 32 * 256 + (ko ^ (kk << 5)));
-    };
-    auto read_v = [&](int kb, int cc, s16x8_t (&v)[4]) {       // the 16 keys of chunk cc, all 128 dimensions
+    for (int j = 0; j < PIECES; ++j) load_to_lds(at + j * (NW * 1024), ksrc + j * (NW * 1024), rk);
 #pragma unroll
-      for (int db = 0; db < 4; ++db) {
-        const int off = voff + (((kb * 8 + cc * 4) * 4 + db) << 8);
-        const s16x4_t v0 = lds_read_tr16(vl, off);
-        const s16x4_t v1 = lds_read_tr16(vl, off + (2 * 4 << 8));
-        v[db] = (s16x8_t){v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-      }
-    };
-    auto scores = [&](const bf16x8_t (&f)[8]) {
-      f32x16_t s = (f32x16_t){0};
+    for (int j = 0; j < PIECES; ++j) load_to_lds(at + TILE * 256 + j * (NW * 1024), vsrc + j * (NW * 1024), rv);
+  };
+  float m_run = st.m, l_run = st.l;
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[kk], qf[kk], s, 0, 0, 0);
-      return s;
-    };
-    auto hide = [&](int kb, f32x16_t& s) {                     // scores of keys this lane's row does not see
-      if (t0 + TILE > k1 || masked || hole_bits) {
-        const int last = (limit < k1 ? limit : k1 - 1) - t0 - 4 * hi;              // last visible row of the tile, seen from this lane's rows
-        const unsigned have = (unsigned)((~hole_bits >> (4 * hi)) >> ((kb & 1) * 32));
+  for (int i = 0; i < NB - 1; ++i)
+    if (k0 + i * TILE < k1) load(k0 + i * TILE, i);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int row = (e & 3) + 8 * (e >> 2);
-          s[e] = kb * 32 + row <= last && ((have >> row) & 1) ? s[e] : -INFINITY;
-        }
-      }
-    };
-    auto largest = [&](const f32x16_t& s) {
-      float mx = s[0];
-#pragma unroll
-      for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
-      return xhalf_max(mx);
-    };
-    auto outgrown = [&](float mx) { return !__all((mx - m_run) * p.c <= 8.0f); };       // the reference moves only when a row outgrows it by 2^8
-    auto move_reference = [&](float mx) {
-      const float m_new = fmaxf(m_run, mx);
-      const float alpha = __builtin_amdgcn_exp2f((m_run - m_new) * p.c);
-      m_run = m_new;
-      l_run *= alpha;
-#pragma unroll
-      for (int db = 0; db < 4; ++db)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
-      return alpha;
-    };
-    auto exponentials = [&](const f32x16_t& s, u32x4_t (&pf)[2], u32x4_t (&pr)[2]) {
-      const float mc = m_run * p.c;
-      float rs = 0.f;
-#pragma unroll
-      for (int cc = 0; cc < 2; ++cc)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cc * 8 + 2 * e], p.c, -mc));
-          const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[cc * 8 + 2 * e + 1], p.c, -mc));
-          rs += p0 + p1;
-          unsigned h, l;
-          split_pair(p0, p1, h, l);
-          pf[cc][e] = h; pr[cc][e] = l;
-        }
-      return rs;                                               // (this half's keys)
-    };
-    auto product = [&](int i, const s16x8_t (&va)[4], const s16x8_t (&vb)[4], const u32x4_t (&pf)[2], const u32x4_t (&pr)[2]) {       // i-th of a block's 16
-      const int db = i & 3;
-      const s16x8_t v = i < 8 ? va[db] : vb[db];
-      const u32x4_t pp = ((i >> 2) & 1 ? pr : pf)[i >> 3];
-      o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, pp), o[db], 0, 0, 0);
-    };
-    // exponentials() dealt among MFMAS matrix instructions, mfma(0) ... mfma(MFMAS - 1): a wave issues in order, so what is to run beside a matrix
-    // instruction has to stand behind it, and the fences keep it there (left to itself hipcc puts all of one kind first)
-    auto exponentials_beside = [&](auto mfmas, auto&& mfma, const f32x16_t& s, u32x4_t (&pf)[2], u32x4_t (&pr)[2]) {
-      constexpr int N = decltype(mfmas)::value, EACH = 16 / N;
-      const float mc = m_run * p.c;
-      float rs = 0.f, pe[16];
-      auto pack = [&](int q) {                                 // the q-th pair
-        rs += pe[2 * q] + pe[2 * q + 1];
-        unsigned h, l;
-        split_pair(pe[2 * q], pe[2 * q + 1], h, l);
-        pf[q >> 2][q & 3] = h; pr[q >> 2][q & 3] = l;
-      };
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        mfma(i);
-#pragma unroll
-        for (int u = 0; u < EACH; ++u) pe[i * EACH + u] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i * EACH + u], p.c, -mc));
-        if (i * EACH >= 2 && (i * EACH) % 2 == 0) pack(i * EACH / 2 - 1);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      pack(7);
-      asm volatile("" : "+v"(pf[0]), "+v"(pf[1]), "+v"(pr[0]), "+v"(pr[1]));      // (made here, not sunk to their use)
-      return rs;
-    };
-#define QP_BATCH_FENCE() __builtin_amdgcn_sched_barrier(0)
-    if constexpr (KB == 1 || kPaged) {
-#pragma unroll
-    for (int n = 0; n < KB; ++n) {
-      const int kb = wk * KB + n;
-      bf16x8_t kf[8];
-      s16x8_t va[4], vb[4];
-      u32x4_t pf[2], pr[2];
-      read_k(kb, kf);
-      QP_BATCH_FENCE();
-      f32x16_t s = scores(kf);
-      read_v(kb, 0, va);
-      QP_BATCH_FENCE();
-      hide(kb, s);
-      const float mx = largest(s);
-      if (outgrown(mx)) move_reference(mx);
-      l_run += xhalf_sum(exponentials(s, pf, pr));
-      QP_BATCH_FENCE();
-      read_v(kb, 1, vb);
-      QP_BATCH_FENCE();
-#pragma unroll
-      for (int i = 0; i < 16; ++i) product(i, va, vb, pf, pr);
-      QP_BATCH_FENCE();
+  for (int kk = 0; kk < 8; ++kk) asm volatile("" : "+v"(qf[kk]));      // hipcc waits for the queries here, not in the loop, where its wait would be for the tiles too
+  int buf = 0;
+  for (int t0 = k0; t0 < k1; t0 += TILE) {
+    if (NB > 2 && t0 + TILE < k1) wait_loads<(NB - 2) * 2 * PIECES>(); else wait_loads<0>();             // this wave's part of the tile is there
+    __syncthreads();                                           // everyone's, and everyone has read the tile before, whose place is loaded next
+    const int ahead = t0 + (NB - 1) * TILE, to = buf + NB - 1 >= NB ? buf - 1 : buf + NB - 1;
+    if (ahead < k1) load(ahead, to);
+    if (wave_live) {
+      const unsigned char* kl = lds + buf * (TILE * 512);
+      take_tile<KB, KB == 2>(p.c, kl, kl + TILE * 256, koff, voff, wk * KB, qf, t0 + TILE > k1, k1 - 1 - t0, 0, hi, m_run, l_run, st.o);
     }
-    } else {
-      // Both blocks' scores, then the first one's products beside the second one's exponentials.
-      const int kb = wk * KB;
-      s16x8_t va[4], vb[4];
-      u32x4_t pf0[2], pr0[2], pf1[2], pr1[2];
-      f32x16_t s0, s1;
-      {
-        bf16x8_t f[8];
-        read_k(kb, f);
-        QP_BATCH_FENCE();
-        s0 = scores(f);
-      }
-      QP_BATCH_FENCE();
-      {
-        bf16x8_t f[8];
-        read_k(kb + 1, f);
-        QP_BATCH_FENCE();
-        hide(kb, s0);
-        s1 = scores(f);
-      }
-      QP_BATCH_FENCE();
-      read_v(kb, 0, va);
-      QP_BATCH_FENCE();
-      hide(kb + 1, s1);
-      float mx = fmaxf(largest(s0), largest(s1));
-      if (outgrown(mx)) move_reference(mx);
-      float rs = exponentials(s0, pf0, pr0);
-      QP_BATCH_FENCE();
-      rs += exponentials_beside(std::integral_constant<int, 16>(), [&](int i) { if (i == 4) read_v(kb, 1, vb); product(i, va, vb, pf0, pr0); }, s1, pf1, pr1);
-      read_v(kb + 1, 0, va);
-      read_v(kb + 1, 1, vb);
-      QP_BATCH_FENCE();
-      l_run += xhalf_sum(rs);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) product(i, va, vb, pf1, pr1);
-    }
+    buf = buf + 1 == NB ? 0 : buf + 1;
   }
   st.m = m_run; st.l = l_run;
 }
@@ -509,7 +574,7 @@ __device__ __forceinline__ void walk_alone(const BatchAttnParams& p, int kvh, in
   int t0 = k0 + first * 32;
   if (kAhead && t0 < k1) load(t0);
   for (; t0 < k1; t0 += 32 * WK) {
-    if (!kAhead) load(t0);
+    load(t0);
     u16x2_t top = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = __builtin_elementwise_max(top, magnitude(vx[i]));
@@ -673,7 +738,24 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
     walk_alone<WK, kPaged>(p, kvh, b, r, row_live, qf, k0, k1, wave, lds, sh, st);
     __syncthreads();                                           // the blocks are read: their LDS joins the rows
   } else {
-    walk_keys<WR, WK, kPaged>(p, kvh, b, r, row_live, wave_live, qf, k0, k1, lds, sh, st);
+    if (!kPaged) {
+      walk_prefix<WR, WK>(p, kvh, wave_live, qf, k0, k1, lds, st);
+      float z = st.l * 0.f;                                    // a value that is not finite left its mark in every row: 0 * it is NaN
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z = __builtin_fmaf(st.o[db][e], 0.f, z);
+      if (row_live && z != 0.f) sh.odd = 1;
+      __syncthreads();
+    }
+    if (kPaged || sh.odd) {
+      if (!kPaged) {                                           // the rare case: once more, with such values left out
+#pragma unroll
+        for (int db = 0; db < 4; ++db) st.o[db] = (f32x16_t){0};
+        st.m = -1e30f; st.l = 0.f;
+      }
+      walk_keys<WR, WK, kPaged>(p, kvh, b, r, row_live, wave_live, qf, k0, k1, lds, sh, st);
+    }
   }
   if (WR == 1) {
     float* obuf = reinterpret_cast<float*>(lds);
@@ -769,7 +851,7 @@ __device__ __forceinline__ int stored_rows(const Pages& pg, int b, int n_new) {
 // they run on the same XCD (workgroups go to the 8 XCDs in turn) and share its L2.
 template <int WR, int WK>
 constexpr int lds_of() {
-  constexpr int tiles = 2 * Shape<WR, WK>::TILE * 256, join = WR == 1 ? join_bytes<WK>() : (WK == 1 ? WR / 2 : WR) * 32 * kJoinRow * 4;      // (WK = 1: of the narrow form)
+  constexpr int tiles = (WR == 1 ? 1 : Shape<WR, WK>::kBuffers) * 2 * Shape<WR, WK>::TILE * 256, join = WR == 1 ? join_bytes<WK>() : (WK == 1 ? WR / 2 : WR) * 32 * kJoinRow * 4;      // (WK = 1: of the narrow form)
   return join > tiles ? join : tiles;
 }
 template <int WR, int WK>
