@@ -99,10 +99,11 @@ struct BatchAttnParams {
   Pages pg;
   int batch, t_max, hq, hkv, G; float c;
   int64_t R;
-  // prefix: `prefix_wgs` workgroups share (row blocks of the batch's live rows) x (key ranges, ns_max at most) as split_prefix() says
-  unsigned prefix_wgs; int ns_max; bool compact;
+  // prefix: at most `prefix_wgs` workgroups share (row blocks of the batch's live rows) x (key ranges); see key_ranges()
+  unsigned prefix_wgs, once, slots; int ns_max; bool compact;
+  int ns;                         // without `compact`: the ranges, 0 = no prefix
   float* pre_o; float2* pre_ml;   // [hkv][ns][live rows] rows of 128 floats / (max, sum)
-  int* starts;                    // with `compact`: [batch + 1] live tokens before a sequence, left for the joining kernel
+  int* starts;                    // with `compact`: [batch + 1] live tokens before a sequence, then the ranges, left for the joining kernel
   // pages: ns2 key ranges, nrb2 row blocks per sequence and kv head
   int ns2, nrb2; unsigned page_wgs;
   float* part_o; float2* part_ml; // [hkv][ns2][R]
@@ -113,14 +114,25 @@ struct BatchAttnParams {
 // A padded batch (n_new given) is computed without its padding: the live tokens are numbered through, row = (live token) * G + g, and the workgroups are
 // dealt over as many row blocks as that makes, so that with few live rows every block's keys are cut into more ranges.
 constexpr int kMaxCompact = 512;  // sequences whose counts fit in LDS (a larger padded batch is computed with its padding)
-struct Split { int64_t rows; int nrb, ns; };
-__host__ __device__ inline Split split_prefix(int64_t tokens, int G, int block_rows, unsigned wgs, int hkv, int ns_max) {
-  Split s;
-  s.rows = tokens * G;
-  s.nrb = (int)((s.rows + block_rows - 1) / block_rows);
-  const int ns = s.nrb ? (int)(wgs / (unsigned)s.nrb / 8 * 8) / hkv : 1;       // 8: see the mapping of workgroups to XCDs
-  s.ns = ns < 1 ? 1 : (ns < ns_max ? ns : ns_max);
-  return s;
+struct Blocks { int64_t rows; unsigned nrb; };
+__host__ __device__ inline Blocks row_blocks(int64_t tokens, int G, int block_rows) {
+  const unsigned rows = (unsigned)tokens * (unsigned)G;        // (batch * t_max * hq <= 2^26)
+  return {(int64_t)rows, (rows + block_rows - 1) / (unsigned)block_rows};
+}
+// Few row blocks: ranges so many that `once` workgroups, one for each place on the card, are busy (multiples of 8: see the mapping to XCDs).
+constexpr unsigned kFewBlocks = 4;
+__host__ __device__ inline int ranges_of_few(unsigned nrb, unsigned once, int hkv, int ns_max) {
+  const int ns = (int)(once / nrb / 8 * 8 / (unsigned)hkv);
+  return ns < 1 ? 1 : (ns < ns_max ? ns : ns_max);
+}
+// Many row blocks do not divide the card so neatly: the number of ranges, up to 64, that costs least, in tiles of one workgroup - rounds over an XCD's
+// places x (tiles of a range + about 3 for its start and end) + writing and reading its partial results.  14 blocks of 256 rows over 32785 keys and 4
+// heads: 548 us with the two ranges of the rule above, 340 with the four found here.
+__host__ __device__ inline float ranges_cost(unsigned ns, unsigned nrb, unsigned prefix_wgs, unsigned slots, int hkv, int ns_max, unsigned block_rows, unsigned tiles) {
+  const unsigned on_xcd = (hkv * ns + 7) / 8 * nrb;
+  if (ns > 1 && (ns > (unsigned)ns_max || on_xcd * 8 > prefix_wgs)) return 3e38f;
+  const unsigned rounds = (on_xcd + slots / 8 - 1) / (slots / 8);
+  return (float)rounds * (float)((tiles + ns - 1) / ns + 3) + (float)nrb * (float)(block_rows * ns * hkv) * (1.0f / 10240.0f);
 }
 // live token -> b * t_max + t
 __device__ __forceinline__ int64_t token_place(const BatchAttnParams& p, const int* starts, int64_t tok) {
@@ -859,10 +871,11 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnPa
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];          // lds_of<WR, WK>()
   __shared__ float lds_ml[WR == 1 ? WK * 64 : WR * 64];
   __shared__ Shared sh;
-  __shared__ int starts[kMaxCompact + 1];
+  __shared__ int starts[kMaxCompact + 2];
   if (blockIdx.x >= p.page_wgs) {
     const unsigned w = blockIdx.x - p.page_wgs;
-    int64_t tokens = (int64_t)p.batch * p.t_max;
+    Blocks rows = row_blocks((int64_t)p.batch * p.t_max, p.G, 32 * WR);
+    int ns = p.ns;
     if (p.compact) {
       if (threadIdx.x < 64) {                                  // running sum of the counts
         int carry = 0;
@@ -877,23 +890,37 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnPa
           if (b < p.batch) starts[b] = carry + incl - v;
           carry += __shfl(incl, 63, 64);
         }
-        if (threadIdx.x == 0) starts[p.batch] = carry;
+        rows = row_blocks(carry, p.G, 32 * WR);
+        int best = 1;
+        if (rows.nrb > kFewBlocks) {                           // each lane a number of ranges
+          float cost = ranges_cost(threadIdx.x + 1, rows.nrb, p.prefix_wgs, p.slots, p.hkv, p.ns_max, 32 * WR, (unsigned)((p.P + 63) >> 6));
+          best = threadIdx.x + 1;
+#pragma unroll
+          for (int k = 32; k > 0; k >>= 1) {
+            const float c2 = __shfl_xor(cost, k, 64);
+            const int b2 = __shfl_xor(best, k, 64);
+            if (c2 < cost || (c2 == cost && b2 < best)) { cost = c2; best = b2; }
+          }
+        } else if (rows.nrb) {
+          best = ranges_of_few(rows.nrb, p.once, p.hkv, p.ns_max);
+        }
+        if (threadIdx.x == 0) { starts[p.batch] = carry; starts[p.batch + 1] = best; }
       }
       __syncthreads();
-      tokens = starts[p.batch];
+      rows = row_blocks(starts[p.batch], p.G, 32 * WR);
+      ns = starts[p.batch + 1];
       if (w == 0)
-        for (int b = threadIdx.x; b <= p.batch; b += 64 * WR * WK) p.starts[b] = starts[b];
+        for (int b = threadIdx.x; b <= p.batch + 1; b += 64 * WR * WK) p.starts[b] = starts[b];
     }
-    const Split sp = split_prefix(tokens, p.G, 32 * WR, p.prefix_wgs, p.hkv, p.ns_max);
-    if (sp.nrb == 0) return;
-    const unsigned turn = 8u * sp.nrb;
+    if (rows.nrb == 0) return;
+    const unsigned turn = 8u * rows.nrb;
     const int item = (int)(w / turn) * 8 + (int)(w % 8), rb = (int)(w % turn) / 8;
-    if (item >= p.hkv * sp.ns) return;
-    const int kvh = item / sp.ns, split = item - kvh * sp.ns;
+    if (item >= p.hkv * ns) return;
+    const int kvh = item / ns, split = item - kvh * ns;
     int k0, k1;
-    key_range((int)p.P, sp.ns, split, k0, k1);
-    const int64_t slot = ((int64_t)kvh * sp.ns + split) * sp.rows;
-    batch_attn_block<WR, WK, false>(p, kvh, 0, (int64_t)rb * 32 * WR, sp.rows, k0, k1, p.pre_o + slot * 128, p.pre_ml + slot, starts, lds, lds_ml, sh);
+    key_range((int)p.P, ns, split, k0, k1);
+    const int64_t slot = ((int64_t)kvh * ns + split) * rows.rows;
+    batch_attn_block<WR, WK, false>(p, kvh, 0, (int64_t)rb * 32 * WR, rows.rows, k0, k1, p.pre_o + slot * 128, p.pre_ml + slot, starts, lds, lds_ml, sh);
     return;
   }
   const int w = (int)blockIdx.x;
@@ -987,14 +1014,14 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
   const int g = (int)(r - bt * p.G), b = (int)(bt / p.t_max), t = (int)(bt % p.t_max);
   if (t >= rows_new(p.pg, b, p.t_max)) return;                 // rows behind a sequence's last token stay as they are
   // parts 0 .. ns - 1: the prefix, row `live`; parts ns ...: the pages, row r
-  int64_t tokens = (int64_t)p.batch * p.t_max, live = r;
-  if (p.compact) { tokens = p.starts[p.batch]; live = (int64_t)(p.starts[b] + t) * p.G + g; }
-  const Split sp = p.ns_max ? split_prefix(tokens, p.G, p.wide_rows, p.prefix_wgs, p.hkv, p.ns_max) : Split{0, 0, 0};
-  const int np = sp.ns + p.ns2;
-  const float2 *ml0 = p.pre_ml + (int64_t)kvh * sp.ns * sp.rows + live, *ml1 = p.part_ml + (int64_t)kvh * p.ns2 * p.R + r;
-  const float *po0 = p.pre_o + ((int64_t)kvh * sp.ns * sp.rows + live) * 128 + lane32 * 4, *po1 = p.part_o + ((int64_t)kvh * p.ns2 * p.R + r) * 128 + lane32 * 4;
-  auto ml = [&](int i) { return i < sp.ns ? ml0[(int64_t)i * sp.rows] : ml1[(int64_t)(i - sp.ns) * p.R]; };
-  auto po = [&](int i) { return *reinterpret_cast<const float4*>(i < sp.ns ? po0 + (int64_t)i * sp.rows * 128 : po1 + (int64_t)(i - sp.ns) * p.R * 128); };
+  int64_t pre_rows = p.R, live = r;
+  int ns = p.ns;
+  if (p.compact) { pre_rows = (int64_t)p.starts[p.batch] * p.G; live = (int64_t)(p.starts[b] + t) * p.G + g; ns = p.starts[p.batch + 1]; }
+  const int np = ns + p.ns2;
+  const float2 *ml0 = p.pre_ml + (int64_t)kvh * ns * pre_rows + live, *ml1 = p.part_ml + (int64_t)kvh * p.ns2 * p.R + r;
+  const float *po0 = p.pre_o + ((int64_t)kvh * ns * pre_rows + live) * 128 + lane32 * 4, *po1 = p.part_o + ((int64_t)kvh * p.ns2 * p.R + r) * 128 + lane32 * 4;
+  auto ml = [&](int i) { return i < ns ? ml0[(int64_t)i * pre_rows] : ml1[(int64_t)(i - ns) * p.R]; };
+  auto po = [&](int i) { return *reinterpret_cast<const float4*>(i < ns ? po0 + (int64_t)i * pre_rows * 128 : po1 + (int64_t)(i - ns) * p.R * 128); };
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
   if (kWide) {
@@ -1135,13 +1162,20 @@ __global__ __launch_bounds__(64) void batch_combine_wide_kernel(BatchAttnParams 
 
 struct Plan {
   enum { kDirect, kWide, kRanges } form;
-  int wr, ns2, nrb2, ns_max, wide_rows, wide_nqb, wide_ns;
+  int wr, ns2, nrb2, ns_max, ns, wide_rows, wide_nqb, wide_ns;
   int64_t R;
-  unsigned prefix_wgs;
+  unsigned prefix_wgs, once, slots;
   bool compact, many_parts;
 };
 
-constexpr int64_t kDirectKeys = 1536, kWideTokens = 96;
+// kDirectKeys: one launch against two, us, one sequence (sixteen), 28 query and 4 kv heads: 400 + 112 keys 10.5 against 11.5 (10.9, 13.4), 800 + 112
+// keys 13.6 against 11.6 (14.3, 14.2), 2400 keys 26 against 12.
+// kWideWork, tokens x prefix keys from which the prefill kernel wins, ranges against it, us: 96 tokens, 768 keys 27 against 30, 32785 keys 83 against 81;
+// 244 tokens, 1952 keys 35 against 44, 32785 keys 179 against 138; 512 tokens, 2048 keys 54 against 60, 4096 keys 87 against 73.
+// kShort, keys x heads below which a workgroup has a tile or two: see the table at make_plan().
+// kFewRows: a workgroup to join a row against a wave: 28 rows x 4 heads 17.5 against 20.8 us in all, 56 x 4 over an hour 186 against 192, 224 x 4 equal,
+// 1008 x 4 131 against 126, 3584 x 4 364 against 348.
+constexpr int64_t kDirectKeys = 640, kWideTokens = 96, kWideWork = 1 << 21, kShort = 65536, kFewRows = 1024;
 
 // ranges of a sequence's pages: `keys` each, fewer ranges where sequences fill the card
 int page_ranges(int64_t wgs, int64_t seqs, int64_t suffix_cap, int most, int64_t keys = 256) {
@@ -1164,7 +1198,7 @@ Plan make_plan(const qp_ctx* ctx, int batch, int t_max, bool padded, int64_t P, 
   }
   // Tokens enough to fill row blocks of the prefill kernel head by head, all of them there, and a prefix long enough that its masked tiles (one per 64
   // tokens: it takes the last prefix row for a new one) do not count.  Its probabilities are rounded to bf16 once, as in every prefill of this library.
-  if (!padded && tokens >= kWideTokens && P >= 4 * tokens && P < (1 << 23)) {
+  if (!padded && tokens >= kWideTokens && P >= 4 * tokens && P * tokens >= kWideWork && P < (1 << 23)) {
     pl.form = Plan::kWide;
     const int64_t by128 = (tokens + 127) / 128 * 128, by256 = (tokens + 255) / 256 * 256;
     pl.wide_rows = by128 < by256 ? 128 : 256;
@@ -1180,9 +1214,21 @@ Plan make_plan(const qp_ctx* ctx, int batch, int t_max, bool padded, int64_t P, 
     pl.ns2 = page_ranges(2LL * ctx->cus, (int64_t)hkv * batch * pl.nrb2, suffix_cap, 16);
     return pl;
   }
-  // Row blocks as wide as the batch's rows (up to 256), key ranges so many that every CU is busy once.
+  // Key ranges times row blocks.  Wide row blocks read the keys less often, narrow ones waste less on rows that are not there (the pages' workgroups
+  // hold one sequence each) and start faster.  us with row blocks of 32 / 64 / 128 / 256 rows, 28 query and 4 kv heads:
+  //                                    4100 keys                      32785 keys
+  //     4 x 1 token,   28 rows         12.7 / 14.4 / 14.8 / 14.0      23.2 / 21.3 / 22.0 / 22.6
+  //    16 x 1,        112 rows         16.5 / 18.1 / 23.0 / 18.5      33.9 / 28.9 / 32.1 / 29.7
+  //    64 x 1,        448 rows         28.6 / 28.2 / 32.7 / 34.4      84.6 / 62.8 / 68.5 / 67.5
+  //    32 x 4,        896 rows         37.2 / 36.4 / 35.2 / 40.0     155.2 / 112  / 106  / 107
+  //     8 x 64 padded, 1925 rows       61.0 / 50.8 / 53.5 / 56.6     299   / 212  / 201  / 196
+  //    16 x 24,      2688 rows         85.7 / 63.1 / 57.8 / 58.2     433   / 280  / 258  / 274
+  //     8 x 128,     7168 rows          188 / 135  / 121  / 121     1022   / 762  / 690  / 653
+  // (72 live rows of 144 over 30737 keys of 8 heads: 49.9 / 44.4 / 52.2 / 39.5; 56 rows over 504015: 217 / 187 / 186 / 192.)
   pl.form = Plan::kRanges;
-  pl.wr = pl.R <= 32 ? 1 : (pl.R <= 64 ? 2 : (pl.R <= 128 ? 4 : 8));
+  pl.compact = padded && t_max > 1 && batch <= kMaxCompact && P > 0;
+  if (P * hkv < kShort) pl.wr = pl.R <= 32 || (!pl.compact && pl.R <= 128) ? 1 : (pl.R <= 2048 ? 2 : 4);
+  else pl.wr = pl.R <= 64 || (!pl.compact && pl.R <= 512) ? 2 : 8;
   const int rows = 32 * pl.wr, per_cu = pl.wr == 8 ? 1 : 2;     // resident workgroups (registers: two waves per SIMD)
   const int64_t nrb = (pl.R + rows - 1) / rows, slots = (int64_t)per_cu * ctx->cus;
   pl.nrb2 = (int)(((int64_t)t_max * G + rows - 1) / rows);
@@ -1190,14 +1236,21 @@ Plan make_plan(const qp_ctx* ctx, int batch, int t_max, bool padded, int64_t P, 
   // A page's key costs about twice a prefix's (two loads one behind the other, no tile ahead): no workgroup of the pages runs longer than one of the prefix.
   const int64_t even = P * hkv * nrb / slots / 2;
   pl.ns2 = page_ranges(slots / 4, seqs, suffix_cap, 32, even > 256 ? even : 256);
-  pl.compact = padded && t_max > 1 && batch <= kMaxCompact && P > 0;
   if (P > 0) {
-    const int64_t page_wgs = seqs * pl.ns2, left = page_wgs * 2 < slots ? slots - page_wgs : slots, once = (hkv + 7) / 8 * 8 * nrb;
-    pl.prefix_wgs = (unsigned)(left > once ? left : once);
-    const int64_t least = pl.wr == 1 ? 128 : 64, most = (P + least - 1) / least;   // a tile per range at least
-    pl.many_parts = pl.R * hkv <= 4096;                        // few rows: a workgroup each joins any number of parts; many: a wave each, 64 parts at most
+    const int64_t page_wgs = seqs * pl.ns2, left = page_wgs * 2 < slots ? slots - page_wgs : slots, least = pl.wr == 1 ? 128 : 64;
+    const int64_t most = (P + least - 1) / least, all = (hkv + 7) / 8 * 8 * nrb, places = nrb > kFewBlocks ? 3 * slots : left;
+    pl.once = (unsigned)left;
+    pl.slots = (unsigned)slots;
+    pl.prefix_wgs = (unsigned)(places > all ? places : all);
+    pl.many_parts = pl.R * hkv <= kFewRows;                    // a workgroup joins any number of parts, a wave 64 at most
     const int cap = pl.many_parts ? kMaxParts - 32 : 64 - pl.ns2;
     pl.ns_max = (int)(most < cap ? most : cap);
+    pl.ns = nrb > kFewBlocks ? 1 : ranges_of_few((unsigned)nrb, pl.once, hkv, pl.ns_max);
+    if (nrb > kFewBlocks) {
+      auto cost = [&](unsigned ns) { return ranges_cost(ns, (unsigned)nrb, pl.prefix_wgs, pl.slots, hkv, pl.ns_max, (unsigned)rows, (unsigned)((P + 63) / 64)); };
+      for (int ns = 2; ns <= 64; ++ns)
+        if (cost(ns) < cost(pl.ns)) pl.ns = ns;
+    }
   }
   return pl;
 }
@@ -1211,7 +1264,7 @@ Layout layout_of(const Plan& pl, int batch, int hq, int hkv) {
   const size_t pages = (size_t)hkv * pl.ns2 * pl.R, prefix = (size_t)pl.prefix_wgs * 32 * pl.wr;       // hkv * ns * live rows <= workgroups * block rows
   l.pre_o = take(prefix * 512); l.pre_ml = take(prefix * sizeof(float2));
   l.part_o = take(pages * 512); l.part_ml = take(pages * sizeof(float2));
-  l.starts = take(pl.compact ? ((size_t)batch + 1) * sizeof(int) : 0);
+  l.starts = take(pl.compact ? ((size_t)batch + 2) * sizeof(int) : 0);
   l.wide = take(pl.form == Plan::kWide ? (size_t)hq * pl.wide_nqb * pl.wide_ns * qpattn::partial_floats(pl.wide_rows) * sizeof(float) : 0);
   l.end = at;
   return l;
@@ -1268,7 +1321,7 @@ int qp_launch_batch_attn(const qp_ctx* ctx, const void* q, const void* k_prefix,
   p.k_pages = (const uint4*)k_pages; p.v_pages = (const uint4*)v_pages;
   p.pg = pages_of(table, seq_len, n_new, max_pages, n_pages, page_size, page_stride);
   p.batch = batch; p.t_max = t_max; p.hq = hq; p.hkv = hkv; p.G = hq / hkv; p.c = scale * 1.4426950408889634f;
-  p.R = pl.R; p.prefix_wgs = pl.prefix_wgs; p.ns_max = pl.ns_max; p.compact = pl.compact;
+  p.R = pl.R; p.prefix_wgs = pl.prefix_wgs; p.once = pl.once; p.slots = pl.slots; p.ns_max = pl.ns_max; p.ns = pl.ns; p.compact = pl.compact;
   p.pre_o = (float*)(ws + l.pre_o); p.pre_ml = (float2*)(ws + l.pre_ml);
   p.part_o = (float*)(ws + l.part_o); p.part_ml = (float2*)(ws + l.part_ml);
   p.starts = (int*)(ws + l.starts);
