@@ -742,3 +742,47 @@ def test_two_streams_at_once(ops):
     torch.cuda.synchronize()
     for s, w in zip(sets, want):
         assert torch.equal(s[-1], w)
+
+
+# --------------------------------------------------------------------------------------------- every form and shape of the attention, by its size
+@pytest.mark.parametrize("hq,hkv,P,ps,seq,T", [
+    (2, 1, 8200, 16, [3, 0], 130), (12, 2, 21900, 24, [5], 96), (16, 1, 4100, 16, [7, 0], 512), (4, 4, 16500, 16, [40, 0, 9, 100], 32),
+])
+def test_attn_prefill_form(ops, hq, hkv, P, ps, seq, T):
+    """n_new None and tokens x prefix of two million or more: the prefill kernel, head by head; with the counts given, the same rows by key ranges."""
+    bt = Batch(hkv, ps, seq, [T] * len(seq), T, seed=P)
+    bt.fill([s + T for s in seq])
+    kpre, vpre = prefix_of(bt, P)
+    q = bt.randn(bt.B, T, hq, D, scale=1.3)
+    ref, tol = attn_ref(q, kpre, vpre, P, bt, hq, D ** -0.5)
+    check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5, n_new=None), ref, tol)
+    check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5), ref, tol)
+
+
+@pytest.mark.parametrize("n_new", ["given", None])
+@pytest.mark.parametrize("hq,hkv,P,B,T", [
+    (16, 1, 4133, 6, 40), (16, 1, 67001, 8, 12), (28, 4, 17000, 5, 8), (28, 4, 16400, 3, 12), (28, 4, 4000, 20, 1), (28, 4, 16500, 9, 1), (32, 2, 33000, 40, 1),
+    (12, 12, 700, 3, 60), (32, 2, 40, 16, 64),
+])
+def test_attn_many_row_blocks(ops, hq, hkv, P, B, T, n_new):
+    """Row blocks of 32, 64, 128 and 256 rows, full, half full and nearly empty; more of them than the card takes at once."""
+    rs = np.random.RandomState(P)
+    new = rs.randint(0, T + 1, B) if n_new == "given" else np.full(B, T)
+    bt = Batch(hkv, 16, rs.randint(0, 40, B).tolist(), new.tolist(), T, seed=B)
+    bt.fill([s + n for s, n in zip(bt.seq, bt.new)])
+    kpre, vpre = prefix_of(bt, P)
+    q = bt.randn(B, T, hq, D, scale=1.3)
+    ref, tol = attn_ref(q, kpre, vpre, P, bt, hq, D ** -0.5)
+    check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5, n_new=n_new), ref, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,P,B,T", [(16, 1, 66000, 3, 6), (16, 1, 66000, 3, 12), (28, 4, 16500, 2, 4), (28, 4, 4000, 8, 12), (16, 1, 4000, 8, 20)])
+def test_attn_infinite_values_by_shape(ops, hq, hkv, P, B, T):
+    """The prefix's tiles go into LDS unseen; a range that meets a value that is not finite is computed again: in the first, a middle and the last tile."""
+    bt = Batch(hkv, 16, [5] * B, [T] * (B - 1) + [T // 2], T, seed=T)
+    bt.fill([5 + n for n in bt.new])
+    kpre, vpre = prefix_of(bt, P)
+    vpre[0, 1, 3] = float("inf"); vpre[0, P // 2, 100] = float("-inf"); vpre[0, P - 1, 7] = float("nan")
+    q = bt.randn(B, T, hq, D)
+    ref, tol = attn_ref(q, kpre, vpre, P, bt, hq, D ** -0.5)
+    check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5), ref, tol)
