@@ -53,6 +53,7 @@ class BatchDecoder:
             need = [eng.ops.batch_attn_workspace(batch, max_step, p, self.width * ps, eng.hq, eng.hkv) for p in set(self.prefix)]
             self.ws = max(need, key=lambda t: t.numel())
         self._ws_rows = {max_step: self.ws}
+        self._step: Optional[List[int]] = None                         # counts of the step whose rows keep() has not been told about
 
     # ------------------------------------------------------------------------------------------------------------- pages
     def _upload(self):
@@ -68,10 +69,11 @@ class BatchDecoder:
     def _reserve(self, counts: Sequence[int]) -> bool:
         """Pages for `counts[b]` more rows of every sequence; True when the table changed."""
         grown = False
-        for b, c in enumerate(counts):
-            need = -(-(self.length[b] + c) // self.PAGE)
+        needs = [-(-(n + c) // self.PAGE) for n, c in zip(self.length, counts)]
+        for b, need in enumerate(needs):                               # (before any page is taken: a refused step changes nothing)
             if need > self.width:
                 raise RuntimeError(f"sequence {b} is full ({self.length[b]} of {self.width * self.PAGE} rows)")
+        for b, need in enumerate(needs):
             while len(self.owned[b]) < need:
                 page = self.free.pop()
                 self.users[page] = 1
@@ -84,6 +86,8 @@ class BatchDecoder:
         children is copied for all but the first of them, because each child stores into it."""
         if len(parents) != self.B or not all(0 <= p < self.B for p in parents):
             raise ValueError(f"parents {list(parents)} for {self.B} sequences")
+        if self._step is not None:
+            raise RuntimeError("reorder() between step() and keep(): say first how many of the step's rows stay")
         if list(parents) == list(range(self.B)):
             return
         ps = self.PAGE
@@ -139,6 +143,7 @@ class BatchDecoder:
         h.copy_(eng.embed_tokens(tokens.reshape(-1)))
         pos = (self.seq_len.long()[:, None] + torch.arange(self.pos0, self.pos0 + T, device=eng.device)).reshape(1, n).expand(3, n).contiguous()
         cos, sin = ops.mrope_table(pos, s.mrope_section, s.rope_theta, D)
+        self._step = counts
         delta = None
         for l, lw in enumerate(eng.w.layers):
             kp, vp = self.pages[l, 0], self.pages[l, 1]
@@ -157,7 +162,11 @@ class BatchDecoder:
 
     def keep(self, counts: Sequence[int]):
         """counts[b] of the last step's tokens of sequence b stay; the rows behind them are overwritten by the next step."""
-        self.length = [n + int(c) for n, c in zip(self.length, counts)]
+        counts = [int(c) for c in counts]
+        if self._step is None or len(counts) != self.B or not all(0 <= c <= n for c, n in zip(counts, self._step)):
+            raise ValueError(f"keep({counts}): the last step stored {self._step} rows")
+        self._step = None
+        self.length = [n + c for n, c in zip(self.length, counts)]
         self.seq_len.copy_(torch.tensor(self.length, dtype=torch.int32))
 
 

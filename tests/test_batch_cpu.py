@@ -215,3 +215,42 @@ def test_generate_through_the_public_interface():
     obj.config.do_top_k_for_query = True
     with pytest.raises(ValueError, match="do_top_k_for_query"):
         run(num_beams=2, batched_beams=True)
+
+
+def test_keep_and_reorder_refuse_what_the_last_step_did_not_store():
+    eng, _ = engine()
+    dec = BatchDecoder(eng, 0, 2, 40, max_step=3)
+    with pytest.raises(ValueError, match="keep"):
+        dec.keep([0, 0])                                               # no step yet
+    dec.step(torch.tensor([[1, 2, 3], [4, 5, 6]]), [3, 1])
+    with pytest.raises(RuntimeError, match="keep"):
+        dec.reorder([1, 0])
+    for bad in ([3, 2], [-1, 1], [3], [3, 1, 0]):
+        with pytest.raises(ValueError, match="keep"):
+            dec.keep(bad)
+    dec.keep([3, 1])
+    assert dec.length == [3, 1]
+    with pytest.raises(ValueError, match="keep"):
+        dec.keep([1, 1])                                               # the same step twice
+    dec.reorder([1, 0])
+    assert dec.length == [1, 3]
+
+
+def test_a_refused_step_changes_nothing():
+    """Sequence 1 is full, sequence 0 needs a new page: the step is refused before a page is taken, and sequence 0 goes on alone."""
+    eng, _ = engine()
+    dec = BatchDecoder(eng, 0, 2, 31, max_step=1)
+    seq = []
+    for i in range(32):
+        dec.step(torch.tensor([[i % 7], [i % 5]]), [int(i < 16), 1])
+        dec.keep([int(i < 16), 1])
+        if i < 16:
+            seq.append(i % 7)
+    assert dec.length == [16, 32]
+    owned = [list(o) for o in dec.owned]
+    with pytest.raises(RuntimeError, match="full"):
+        dec.step(torch.tensor([[9], [9]]))
+    assert dec.owned == owned
+    logits = dec.step(torch.tensor([[9], [0]]), [1, 0])
+    dec.keep([1, 0])
+    assert near(logits[0], alone(eng, seq + [9])[-1:])
