@@ -64,6 +64,7 @@ bool pages(Args& A, int k, int64_t batch, int64_t n_kv, int64_t D, PageArgs& o, 
   A.shape(o.table, {batch, o.width});
   A.shape(o.seq_len, {batch});
   A.shape(o.n_new, {batch});
+  if (o.n_pages > INT32_MAX || o.size > INT32_MAX || o.width > INT32_MAX) A.ok = false;
   if (!A.ok || !o.k->strides().equals(o.v->strides()) || o.k->stride(1) != o.size * D || o.k->stride(2) != D || o.k->stride(3) != 1) return A.ok = false;
   o.stride = o.n_pages > 1 ? o.k->stride(0) : n_kv * o.size * D;
   return true;
@@ -102,7 +103,7 @@ PyObject* batch_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor *q = A.t(4, at::kBFloat16), *out = A.t(18, at::kBFloat16), *kp = nullptr, *vp = nullptr;
   if (!THPVariable_Check(args[19])) return refused();
   const at::Tensor& ws = THPVariable_Unpack(args[19]);
-  if (!A.ok || q->dim() != 4 || ws.get_device() != A.dev || !ws.is_contiguous()) return refused();
+  if (!A.ok || q->dim() != 4 || ws.layout() != at::kStrided || ws.get_device() != A.dev || !ws.is_contiguous()) return refused();
   const int64_t B = q->size(0), T = q->size(1);
   A.shape(q, {B, T, hq, D});
   A.shape(out, {B, T, hq, D});
@@ -112,7 +113,7 @@ PyObject* batch_attn(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!A.ok || P > (1LL << 40) || stride < 0 || stride > (1LL << 50)) return refused();
     const int64_t elements = (hkv - 1) * stride + P * D;
     for (const at::Tensor* x : {kp, vp})
-      if ((int64_t)(x->storage().nbytes() / 2) - x->storage_offset() < elements) return refused();
+      if (!x->has_storage() || (int64_t)(x->storage().nbytes() / 2) - x->storage_offset() < elements) return refused();
   }
   PageArgs pg;
   if (!A.ok || B * T > INT32_MAX || !pages(A, 9, B, hkv, D, pg, 11, 12, 13)) return refused();
@@ -131,7 +132,7 @@ PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor &lg = THPVariable_Unpack(args[4]), &ws = THPVariable_Unpack(args[12]);
   const bool f32 = lg.scalar_type() == at::kFloat;
   if ((!f32 && lg.scalar_type() != at::kBFloat16) || lg.layout() != at::kStrided || lg.get_device() != A.dev || lg.dim() != 3 || lg.size(1) < 1 ||
-      ws.get_device() != A.dev || !ws.is_contiguous())
+      ws.layout() != at::kStrided || ws.get_device() != A.dev || !ws.is_contiguous())
     return refused();
   const int64_t B = lg.size(0), T = lg.size(1) - 1, V = lg.size(2);
   const at::Tensor *drafts = A.t(5, at::kLong), *nd = A.t(6, at::kInt, true, true), *pr = T ? A.t(7, at::kFloat, false, true) : nullptr,
@@ -148,10 +149,21 @@ PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
                             (float)temperature, (int32_t*)out_ptr(acc), (int64_t*)out_ptr(tok), ws.data_ptr(), ws.nbytes(), A.stream));
 }
 
+// no C++ exception (a tensor without memory of its own, say) leaves through the C entry
+template <PyObject* (*kCall)(PyObject*, PyObject* const*, Py_ssize_t)>
+PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  try {
+    return kCall(self, args, n);
+  } catch (const std::exception& e) {
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
 PyMethodDef kMethods[] = {
-    {"batch_rope_append", (PyCFunction)(void (*)(void))batch_rope_append, METH_FASTCALL, nullptr},
-    {"batch_attn", (PyCFunction)(void (*)(void))batch_attn, METH_FASTCALL, nullptr},
-    {"verify_drafts", (PyCFunction)(void (*)(void))verify_drafts, METH_FASTCALL, nullptr},
+    {"batch_rope_append", (PyCFunction)(void (*)(void))guarded<batch_rope_append>, METH_FASTCALL, nullptr},
+    {"batch_attn", (PyCFunction)(void (*)(void))guarded<batch_attn>, METH_FASTCALL, nullptr},
+    {"verify_drafts", (PyCFunction)(void (*)(void))guarded<verify_drafts>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_qp_torch", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

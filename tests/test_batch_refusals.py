@@ -181,3 +181,21 @@ def test_missing_face_fails_loudly(monkeypatch):
     monkeypatch.delattr("quickvideo_amd._qp_torch", raising=False)
     with pytest.raises(native.QuickPrefillUnavailable, match="_qp_torch"):
         native.load_face()
+
+
+def test_tensors_without_plain_memory_are_refused(ops):
+    """A sparse tensor's is_contiguous() throws in C++: it must come back as a Python error, not end the process."""
+    kw = batch_tensors()
+    B, T, hq, hkv = 2, 3, 4, 2
+    q, kp = torch.zeros(B, T, hq, 128, dtype=torch.bfloat16), torch.zeros(hkv, 10, 128, dtype=torch.bfloat16)
+    sparse = torch.zeros(8, 8).to_sparse()
+    attn = [q, kp, kp, 1280, 10, kw["k_pages"], kw["v_pages"], kw["table"], kw["seq_len"], kw["n_new"], hq, hkv, 128, 0.1, q.clone(), torch.zeros(1 << 16, dtype=torch.uint8)]
+    for at in (0, 1, 5, 7, 15):
+        bad = sparse if at == 15 else attn[at].to_sparse()
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.batch_attn(*[bad if i == at else v for i, v in enumerate(attn)])
+    with pytest.raises((ValueError, RuntimeError)):
+        ops.verify_drafts(torch.zeros(2, 3, 7), torch.zeros(2, 2, dtype=torch.int64), None, None, torch.zeros(2, 3), 1.0, torch.zeros(2, dtype=torch.int32),
+                          torch.zeros(2, 3, dtype=torch.int64), sparse)
+    with pytest.raises((ValueError, RuntimeError)):
+        ops.batch_rope_append(*(kw | {"qkv": kw["qkv"].to_sparse()}).values())
