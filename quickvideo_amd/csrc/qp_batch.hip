@@ -7,7 +7,8 @@
 //   batch_rope_append_kernel   rotates the step's q and k rows and stores k / v into the pages
 //   batch_attn_kernel          attention of (batch x t_max) query rows over (shared prefix, own pages): partial results per key range
 //   batch_combine_kernel       joins the partial results of a row
-#include <type_traits>
+//   batch_attn_direct_kernel   both in one launch, for few keys
+//   batch_combine_wide_kernel  joins the pages' partial results with those the prefill kernel left of the prefix, for many tokens
 #include "qp_attn.h"
 
 namespace {
@@ -192,19 +193,25 @@ __device__ __forceinline__ void add_odd_values(const BatchAttnParams& p, int kvh
   }
 }
 
-// A workgroup of WR x WK waves takes a block of 32 * WR rows over one key range, kTile keys at a time: the tile goes through registers into LDS
-// (K row-major with XOR-swizzled 16-B slots; V as [key / 4][d / 32][key % 4][32] for the transposing LDS reads), the next tile's loads are in
-// flight while this one is computed.  Wave (wr, wk) owns rows [32 wr, 32 wr + 32) and, for WK = 2, half of the tile's keys:
-// S^T = K.Q^T (rows are the columns of v_mfma_f32_32x32x16_bf16: a lane owns one row), online softmax, O^T += V^T.P, all sums in fp32.
-// A value that is not finite would spoil rows that do not see it (0 * infinity is NaN) and the sum of the two products below, so it goes into
-// LDS as zero; a range that holds one ends with add_odd_values.
+// A workgroup of WR x WK waves takes a block of 32 * WR rows over one key range, a tile of 64 keys at a time, staged in LDS (K row-major with
+// XOR-swizzled 16-B slots; V as [key / 4][d / 32][key % 4][32] for the transposing LDS reads).  Wave (wr, wk) owns rows [32 wr, 32 wr + 32) and, for
+// WK = 2, half of the tile's keys: S^T = K.Q^T (rows are the columns of v_mfma_f32_32x32x16_bf16: a lane owns one row), online softmax,
+// O^T += V^T.P, all sums in fp32.  The prefix goes straight into LDS (walk_prefix), the pages, whose rows lie apart, through registers (walk_keys).
+// A value that is not finite would spoil rows that do not see it (0 * infinity is NaN) and the sum of the two products below.  walk_keys puts zero in
+// its place, and the range ends with add_odd_values; walk_prefix does not look, but such a value leaves no result of its range finite, which is then
+// computed again with walk_keys.
+// What bounds it: two waves a SIMD (200 registers each) whose matrix instructions are 60 % of a tile's time with all eight row tiles filled (3072 of
+// 5164 clocks: 448 rows over 32785 keys, 62 us), the rest is the barrier and the loads' issue; with fewer rows the bytes: 56 rows over 504015 keys
+// 187 us, 5.5 TB/s.  Tried and slower: staging the prefix through registers, one tile ahead (448 rows 64.5 us, 72 rows over 30737 keys 44.4 against
+// 39.5); the loads issued between the products (64.1, 40.6); two tiles of 64 keys in LDS instead of three for 8 waves (61.8, 41.6); four (63.0, 40.5);
+// wave priorities (no effect).
 // P goes into the product as TWO bf16 numbers, bf16(p) and bf16(p - bf16(p)): 2^-17 of p is lost instead of 2^-9.  Rounded once, as the prefill and
 // decode kernels do it, the result's error against 64 bits is 0.0021 - 0.0027 of it, with two terms 0.0017, which is its own rounding; the second
 // product reuses the V fragments, and a step that waits for the prefix's bytes has the matrix pipe free.
 template <int WR, int WK>
 struct Shape {
   static constexpr int NT = 64 * WR * WK, KB = WK == 1 ? 2 : 1, TILE = 32 * WK * KB, PT = TILE * 16 / NT;   // PT: 16-B pieces a thread stages of K and of V
-  static constexpr int kBuffers = NT == 512 ? 3 : 2;
+  static constexpr int kBuffers = NT == 512 ? 3 : 2;           // of the prefix: one workgroup of 8 waves fits on a CU, two of 4
 };
 struct Rows {                      // what a lane keeps of its row (both halves of a wave: the same row, other keys)
   f32x16_t o[4];                   // [d / 32], unscaled
@@ -221,7 +228,7 @@ __device__ __forceinline__ void split_pair(float a, float b, unsigned& hi, unsig
 typedef unsigned u32x4_t __attribute__((ext_vector_type(4)));
 
 struct Shared {                    // LDS besides the tile
-  unsigned long long holes[3][4];  // by number of the tile: its rows without a page
+  unsigned long long holes[2];     // by parity of the tile: its rows without a page
   int odd;                         // a value that is not finite was met
 };
 
@@ -280,7 +287,6 @@ __device__ __forceinline__ void take_tile(float c, const unsigned char* kl, cons
     for (int db = 0; db < 4; ++db)
 #pragma unroll
       for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
-    return alpha;
   };
   auto exponentials = [&](const f32x16_t& s, u32x4_t (&pf)[2], u32x4_t (&pr)[2]) {
     const float mc = m_run * c;
@@ -304,25 +310,23 @@ __device__ __forceinline__ void take_tile(float c, const unsigned char* kl, cons
     const u32x4_t pp = ((i >> 2) & 1 ? pr : pf)[i >> 3];
     o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, pp), o[db], 0, 0, 0);
   };
-  // exponentials() dealt among MFMAS matrix instructions, mfma(0) ... mfma(MFMAS - 1): a wave issues in order, so what is to run beside a matrix
-  // instruction has to stand behind it, and the fences keep it there (left to itself hipcc puts all of one kind first)
-  auto exponentials_beside = [&](auto mfmas, auto&& mfma, const f32x16_t& s, u32x4_t (&pf)[2], u32x4_t (&pr)[2]) {
-    constexpr int N = decltype(mfmas)::value, EACH = 16 / N;
+  // exponentials() dealt among the 16 matrix instructions mfma(0) ... mfma(15): a wave issues in order, so what is to run beside a matrix instruction
+  // has to stand behind it, and the fences keep it there (left to itself hipcc puts all of one kind first)
+  auto exponentials_beside = [&](auto&& mfma, const f32x16_t& s, u32x4_t (&pf)[2], u32x4_t (&pr)[2]) {
     const float mc = m_run * c;
     float rs = 0.f, pe[16];
-    auto pack = [&](int q) {                                 // the q-th pair
+    auto pack = [&](int q) {                                   // the q-th pair
       rs += pe[2 * q] + pe[2 * q + 1];
       unsigned h, l;
       split_pair(pe[2 * q], pe[2 * q + 1], h, l);
       pf[q >> 2][q & 3] = h; pr[q >> 2][q & 3] = l;
     };
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < 16; ++i) {
       mfma(i);
-#pragma unroll
-      for (int u = 0; u < EACH; ++u) pe[i * EACH + u] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i * EACH + u], c, -mc));
-      if (i * EACH >= 2 && (i * EACH) % 2 == 0) pack(i * EACH / 2 - 1);
-      __builtin_amdgcn_sched_barrier(0);
+      pe[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, -mc));
+      if (i >= 2 && i % 2 == 0) pack(i / 2 - 1);
+      QP_BATCH_FENCE();
     }
     pack(7);
     asm volatile("" : "+v"(pf[0]), "+v"(pf[1]), "+v"(pr[0]), "+v"(pr[1]));      // (made here, not sunk to their use)
@@ -330,27 +334,27 @@ __device__ __forceinline__ void take_tile(float c, const unsigned char* kl, cons
   };
   if constexpr (!kBeside) {
 #pragma unroll
-  for (int n = 0; n < KB; ++n) {
-    const int kb = kb0 + n;
-    bf16x8_t kf[8];
-    s16x8_t va[4], vb[4];
-    u32x4_t pf[2], pr[2];
-    read_k(kb, kf);
-    QP_BATCH_FENCE();
-    f32x16_t s = scores(kf);
-    read_v(kb, 0, va);
-    QP_BATCH_FENCE();
-    hide(kb, s);
-    const float mx = largest(s);
-    if (outgrown(mx)) move_reference(mx);
-    l_run += xhalf_sum(exponentials(s, pf, pr));
-    QP_BATCH_FENCE();
-    read_v(kb, 1, vb);
-    QP_BATCH_FENCE();
+    for (int n = 0; n < KB; ++n) {
+      const int kb = kb0 + n;
+      bf16x8_t kf[8];
+      s16x8_t va[4], vb[4];
+      u32x4_t pf[2], pr[2];
+      read_k(kb, kf);
+      QP_BATCH_FENCE();
+      f32x16_t s = scores(kf);
+      read_v(kb, 0, va);
+      QP_BATCH_FENCE();
+      hide(kb, s);
+      const float mx = largest(s);
+      if (outgrown(mx)) move_reference(mx);
+      l_run += xhalf_sum(exponentials(s, pf, pr));
+      QP_BATCH_FENCE();
+      read_v(kb, 1, vb);
+      QP_BATCH_FENCE();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) product(i, va, vb, pf, pr);
-    QP_BATCH_FENCE();
-  }
+      for (int i = 0; i < 16; ++i) product(i, va, vb, pf, pr);
+      QP_BATCH_FENCE();
+    }
   } else {
     // Both blocks' scores, then the first one's products beside the second one's exponentials.
     const int kb = kb0;
@@ -379,7 +383,7 @@ __device__ __forceinline__ void take_tile(float c, const unsigned char* kl, cons
     if (outgrown(mx)) move_reference(mx);
     float rs = exponentials(s0, pf0, pr0);
     QP_BATCH_FENCE();
-    rs += exponentials_beside(std::integral_constant<int, 16>(), [&](int i) { if (i == 4) read_v(kb, 1, vb); product(i, va, vb, pf0, pr0); }, s1, pf1, pr1);
+    rs += exponentials_beside([&](int i) { if (i == 4) read_v(kb, 1, vb); product(i, va, vb, pf0, pr0); }, s1, pf1, pr1);
     read_v(kb + 1, 0, va);
     read_v(kb + 1, 1, vb);
     QP_BATCH_FENCE();
@@ -459,14 +463,13 @@ __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int
 #pragma unroll
     for (int i = 0; i < PT; ++i) {
       const int row = srow + i * (NT / 16);
-      if (kPaged && ((holes >> i) & 1) && slot16 == 0) atomicOr(&sh.holes[par][row >> 6], 1ull << (row & 63));
+      if (kPaged && ((holes >> i) & 1) && slot16 == 0) atomicOr(&sh.holes[par], 1ull << row);
       *reinterpret_cast<uint4*>(kl + row * 256 + ((slot16 ^ (row & 15)) << 4)) = kx[i];
       *reinterpret_cast<uint4*>(vl + (((row >> 2) * 4 + (slot16 >> 2)) << 8) + ((row & 3) << 6) + ((slot16 & 3) << 4)) = vx[i];
     }
     __syncthreads();
-    const int word = wk * KB / 2;                              // this wave's keys lie in one 64-key word of the mask
-    const unsigned long long hole_bits = kPaged ? sh.holes[par][word] : 0;
-    if (kPaged && tid < 4) sh.holes[par ^ 1][tid] = 0;         // last read before the barrier above, next written behind the next one
+    const unsigned long long hole_bits = kPaged ? sh.holes[par] : 0;
+    if (kPaged && tid == 0) sh.holes[par ^ 1] = 0;            // last read before the barrier above, next written behind the next one
     if (!wave_live) continue;
     take_tile<KB, false>(p.c, kl, vl, koff, voff, wk * KB, qf, t0 + TILE > k1 || masked || hole_bits, (limit < k1 ? limit : k1 - 1) - t0, hole_bits, hi, m_run,
                          l_run, o);
@@ -675,7 +678,7 @@ __device__ __forceinline__ void walk_alone(const BatchAttnParams& p, int kvh, in
   st.m = m_run; st.l = l_run;
 }
 
-// Q fragments of the lane's row, an empty running state and cleared flags (the first barrier of walk_keys orders the flags)
+// Q fragments of the lane's row, an empty running state and cleared flags (ordered by the first barrier behind it)
 __device__ __forceinline__ void begin_rows(const BatchAttnParams& p, int kvh, int64_t bt, int g, bool row_live, bf16x8_t (&qf)[8], Shared& sh, Rows& st) {
   const int tid = threadIdx.x, hi = (tid >> 5) & 1;
   const uint4* src = p.q + ((bt * p.hq) + (int64_t)kvh * p.G + g) * 16;
@@ -688,7 +691,7 @@ __device__ __forceinline__ void begin_rows(const BatchAttnParams& p, int kvh, in
 #pragma unroll
   for (int db = 0; db < 4; ++db) st.o[db] = (f32x16_t){0};
   st.m = -1e30f; st.l = 0.f;
-  if (tid < 12) sh.holes[tid >> 2][tid & 3] = 0;
+  if (tid < 2) sh.holes[tid] = 0;
   if (tid == 0) sh.odd = 0;
 }
 
@@ -765,6 +768,8 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
 #pragma unroll
         for (int db = 0; db < 4; ++db) st.o[db] = (f32x16_t){0};
         st.m = -1e30f; st.l = 0.f;
+        __syncthreads();
+        if (tid == 0) sh.odd = 0;                              // (it may have been a query or a key: walk_keys finds the values)
       }
       walk_keys<WR, WK, kPaged>(p, kvh, b, r, row_live, wave_live, qf, k0, k1, lds, sh, st);
     }
@@ -781,48 +786,48 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
       if (d4 == 0) part_ml[row0 + row] = make_float2(m, l);
     }
   } else {
-  f32x16_t (&o)[4] = st.o;
-  float m_run = st.m, l_run = st.l;
-  if (WK == 2) {                                               // join the two key halves of a row (the tile's LDS is free)
-    __syncthreads();
-    float* obuf = reinterpret_cast<float*>(lds);               // [WR][32 rows][kJoinRow]
-    if (wk == 1) {
-      if (hi == 0) { lds_ml[(wr * 32 + l31) * 2] = m_run; lds_ml[(wr * 32 + l31) * 2 + 1] = l_run; }
+    f32x16_t (&o)[4] = st.o;
+    float m_run = st.m, l_run = st.l;
+    if (WK == 2) {                                               // join the two key halves of a row (the tile's LDS is free)
+      __syncthreads();
+      float* obuf = reinterpret_cast<float*>(lds);               // [WR][32 rows][kJoinRow]
+      if (wk == 1) {
+        if (hi == 0) { lds_ml[(wr * 32 + l31) * 2] = m_run; lds_ml[(wr * 32 + l31) * 2 + 1] = l_run; }
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4)
+            *reinterpret_cast<float4*>(obuf + (wr * 32 + l31) * kJoinRow + db * 32 + 8 * q4 + 4 * hi) =
+                make_float4(o[db][q4 * 4 + 0], o[db][q4 * 4 + 1], o[db][q4 * 4 + 2], o[db][q4 * 4 + 3]);
+      }
+      __syncthreads();
+      if (wk == 0) {
+        const float m1 = lds_ml[(wr * 32 + l31) * 2], l1 = lds_ml[(wr * 32 + l31) * 2 + 1];
+        const float m = fmaxf(m_run, m1);
+        const float a0 = __builtin_amdgcn_exp2f((m_run - m) * p.c), a1 = __builtin_amdgcn_exp2f((m1 - m) * p.c);
+        m_run = m;
+        l_run = l_run * a0 + l1 * a1;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            const float4 other = *reinterpret_cast<const float4*>(obuf + (wr * 32 + l31) * kJoinRow + db * 32 + 8 * q4 + 4 * hi);
+            o[db][q4 * 4 + 0] = o[db][q4 * 4 + 0] * a0 + other.x * a1;
+            o[db][q4 * 4 + 1] = o[db][q4 * 4 + 1] * a0 + other.y * a1;
+            o[db][q4 * 4 + 2] = o[db][q4 * 4 + 2] * a0 + other.z * a1;
+            o[db][q4 * 4 + 3] = o[db][q4 * 4 + 3] * a0 + other.w * a1;
+          }
+      }
+    }
+    if (row_live && wk == 0) {
+      if (hi == 0) part_ml[r] = make_float2(m_run, l_run);
 #pragma unroll
       for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int q4 = 0; q4 < 4; ++q4)
-          *reinterpret_cast<float4*>(obuf + (wr * 32 + l31) * kJoinRow + db * 32 + 8 * q4 + 4 * hi) =
+          *reinterpret_cast<float4*>(part_o + r * 128 + db * 32 + 8 * q4 + 4 * hi) =
               make_float4(o[db][q4 * 4 + 0], o[db][q4 * 4 + 1], o[db][q4 * 4 + 2], o[db][q4 * 4 + 3]);
     }
-    __syncthreads();
-    if (wk == 0) {
-    const float m1 = lds_ml[(wr * 32 + l31) * 2], l1 = lds_ml[(wr * 32 + l31) * 2 + 1];
-    const float m = fmaxf(m_run, m1);
-    const float a0 = __builtin_amdgcn_exp2f((m_run - m) * p.c), a1 = __builtin_amdgcn_exp2f((m1 - m) * p.c);
-    m_run = m;
-    l_run = l_run * a0 + l1 * a1;
-#pragma unroll
-    for (int db = 0; db < 4; ++db)
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const float4 other = *reinterpret_cast<const float4*>(obuf + (wr * 32 + l31) * kJoinRow + db * 32 + 8 * q4 + 4 * hi);
-        o[db][q4 * 4 + 0] = o[db][q4 * 4 + 0] * a0 + other.x * a1;
-        o[db][q4 * 4 + 1] = o[db][q4 * 4 + 1] * a0 + other.y * a1;
-        o[db][q4 * 4 + 2] = o[db][q4 * 4 + 2] * a0 + other.z * a1;
-        o[db][q4 * 4 + 3] = o[db][q4 * 4 + 3] * a0 + other.w * a1;
-      }
-    }
-  }
-  if (row_live && wk == 0) {
-    if (hi == 0) part_ml[r] = make_float2(m_run, l_run);
-#pragma unroll
-    for (int db = 0; db < 4; ++db)
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4)
-        *reinterpret_cast<float4*>(part_o + r * 128 + db * 32 + 8 * q4 + 4 * hi) =
-            make_float4(o[db][q4 * 4 + 0], o[db][q4 * 4 + 1], o[db][q4 * 4 + 2], o[db][q4 * 4 + 3]);
-  }
   }
   if (k0 < k1 && sh.odd) {                                  // (read behind the loop's barriers)
     __threadfence_block();

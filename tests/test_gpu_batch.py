@@ -786,3 +786,20 @@ def test_attn_infinite_values_by_shape(ops, hq, hkv, P, B, T):
     q = bt.randn(B, T, hq, D)
     ref, tol = attn_ref(q, kpre, vpre, P, bt, hq, D ** -0.5)
     check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5), ref, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,P,B,T", [(8, 2, 200, 2, 2), (28, 4, 4000, 3, 1), (28, 4, 16500, 8, 1), (16, 1, 66000, 3, 6), (16, 1, 66000, 3, 12)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_attn_a_query_that_is_not_finite_spoils_its_own_rows_only(ops, hq, hkv, P, B, T, value):
+    bt = Batch(hkv, 16, [5] * B, [T] * B, T, seed=T)
+    bt.fill([5 + T] * B)
+    kpre, vpre = prefix_of(bt, P)
+    q = bt.randn(B, T, hq, D)
+    ref, tol = attn_ref(q, kpre, vpre, P, bt, hq, D ** -0.5)
+    bad = q.clone()
+    bad[B - 1, T - 1, 3, 17] = value
+    bad[0, 0, hq - 1] = value
+    got = run_attn(ops, bad.cuda(), kpre, vpre, P, bt, hq, D ** -0.5)
+    got[B - 1, T - 1, 3], got[0, 0, hq - 1] = 0.0, 0.0                  # (those rows may be anything)
+    ref[B - 1, T - 1, 3], ref[0, 0, hq - 1] = 0.0, 0.0
+    check(got, ref, tol)
