@@ -106,12 +106,15 @@ struct Chunk {
 // with the 32-bit exponential instead.  More or fewer workgroups on a CU, or several chunks per workgroup with the next one's loads ahead, gained nothing.
 template <bool kF32>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyParams p) {
-  __shared__ double red[4];
+  __shared__ double red[4], red_o[4];
   __shared__ float red_m[4];
   __shared__ int red_i[4];
-  const int ch = blockIdx.x, t = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int ch = blockIdx.x, t = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, wave = tid >> 6;
   if (t > drafts_of(p, b)) return;
   const int64_t row = (int64_t)b * p.seq_stride + (int64_t)t * p.row_stride, v0 = (int64_t)ch * kChunk;
+  // a certain draft: the sum without it as well, which may be next to nothing of the whole
+  const bool certain = p.scale != 0.0 && !p.probs && t < p.T;
+  const int64_t draft = certain ? p.drafts[(int64_t)b * p.T + t] : -1;
   Chunk<kF32> c;
   c.load(p, row, v0);
   float m = -INFINITY;
@@ -121,46 +124,54 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyParams p) 
     if (!(c.x[i] == c.x[i])) c.x[i] = -INFINITY;
     if (c.x[i] > m) { m = c.x[i]; arg = (int)v0 + c.place(i); }
   }
+  // Every wave against its own maximum; they meet once, at the end.
+  double s = 0.0, o = 0.0;
+  if (p.scale == 0.0) {
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    const float om = __shfl_xor(m, d, 64);
-    const int oa = __shfl_xor(arg, d, 64);
-    if (om > m || (om == m && oa < arg)) { m = om; arg = oa; }
+    for (int d = 32; d > 0; d >>= 1) {
+      const float om = __shfl_xor(m, d, 64);
+      const int oa = __shfl_xor(arg, d, 64);
+      if (om > m || (om == m && oa < arg)) { m = om; arg = oa; }
+    }
+  } else {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    if (m != -INFINITY) {
+      bool holds = false;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) s += weight(c.x[i], m, p.scale);
+      o = s;
+      if (draft >= v0 && draft < v0 + kChunk) {                // (uniform)
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) holds |= v0 + c.place(i) == draft;
+        if (holds) {                                           // one thread sums again
+          o = 0.0;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) o += v0 + c.place(i) == draft ? 0.0 : weight(c.x[i], m, p.scale);
+        }
+        o = wave_sum_f64(o);
+      }
+      s = wave_sum_f64(s);
+    }
   }
-  if ((tid & 63) == 0) { red_m[tid >> 6] = m; red_i[tid >> 6] = arg; }
+  if ((tid & 63) == 0) { red_m[wave] = m; red_i[wave] = arg; red[wave] = s; red_o[wave] = o; }
   __syncthreads();
+  if (tid != 0) return;
   m = red_m[0]; arg = red_i[0];
 #pragma unroll
   for (int w = 1; w < 4; ++w)
     if (red_m[w] > m || (red_m[w] == m && red_i[w] < arg)) { m = red_m[w]; arg = red_i[w]; }
-  const bool sums = p.scale != 0.0 && m != -INFINITY;
-  double s = 0.0;
-  if (sums) {
+  s = o = 0.0;
+  if (p.scale != 0.0 && m != -INFINITY) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) s += weight(c.x[i], m, p.scale);
-  }
-  const double mine = s;
-  s = block_sum_f64(s, red);
-  if (!p.probs && t < p.T && sums) {                           // a certain draft: its chunk's sum without it, which may be next to nothing of the whole
-    const int64_t draft = p.drafts[(int64_t)b * p.T + t];
-    if (draft >= v0 && draft < v0 + kChunk) {                  // (uniform)
-      double o = mine;
-      bool holds = false;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) holds |= v0 + c.place(i) == draft;
-      if (holds) {                                             // one thread sums again
-        o = 0.0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) o += v0 + c.place(i) == draft ? 0.0 : weight(c.x[i], m, p.scale);
-      }
-      o = block_sum_f64(o, red);
-      if (tid == 0) p.others[(int64_t)b * p.T + t] = o;
+    for (int w = 0; w < 4; ++w) {
+      const double f = weight(red_m[w], m, p.scale);
+      s += red[w] * f; o += red_o[w] * f;
     }
+    if (draft >= v0 && draft < v0 + kChunk) p.others[(int64_t)b * p.T + t] = o;
   }
-  if (tid == 0) {
-    const int64_t at = ((int64_t)b * (p.T + 1) + t) * p.nc + ch;
-    p.sum[at] = s; p.top[at] = m; p.arg[at] = arg;
-  }
+  const int64_t at = ((int64_t)b * (p.T + 1) + t) * p.nc + ch;
+  p.sum[at] = s; p.top[at] = m; p.arg[at] = arg;
 }
 
 // Which drafts stand: every workgroup that asks finds it again from the chunks' statistics (a few KB) instead of waiting for another launch.
