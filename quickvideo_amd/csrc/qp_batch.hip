@@ -1175,12 +1175,14 @@ struct Plan {
 
 // kDirectKeys: one launch against two, us, one sequence (sixteen), 28 query and 4 kv heads: 400 + 112 keys 10.5 against 11.5 (10.9, 13.4), 800 + 112
 // keys 13.6 against 11.6 (14.3, 14.2), 2400 keys 26 against 12.
-// kWideWork, tokens x prefix keys from which the prefill kernel wins, ranges against it, us: 96 tokens, 768 keys 27 against 30, 32785 keys 83 against 81;
+// kWideWork, tokens x prefix keys from which the prefill kernel wins, ranges against it, us: 96 tokens, 768 keys 16 against 30, 32785 keys 83 against 81;
 // 244 tokens, 1952 keys 35 against 44, 32785 keys 179 against 138; 512 tokens, 2048 keys 54 against 60, 4096 keys 87 against 73.
 // kShort, keys x heads below which a workgroup has a tile or two: see the table at make_plan().
+// kLeastKeys of a range, 64 / 128 / 192 / 256 / 384 / 512, us: 28 rows over 11535 keys - / 17.0 / 16.0 / 15.5 / 15.9 / 17.2, 231 padded rows over 4100 keys
+// 23.0 / 23.1 / 21.6 / 20.6, 672 rows over 768 keys 19.4 / 19.4 / 17.3 / 16.0: fewer parts to join.
 // kFewRows: a workgroup to join a row against a wave: 28 rows x 4 heads 17.5 against 20.8 us in all, 56 x 4 over an hour 186 against 192, 224 x 4 equal,
 // 1008 x 4 131 against 126, 3584 x 4 364 against 348.
-constexpr int64_t kDirectKeys = 640, kWideTokens = 96, kWideWork = 1 << 21, kShort = 65536, kFewRows = 1024;
+constexpr int64_t kDirectKeys = 640, kWideTokens = 96, kWideWork = 1 << 21, kShort = 65536, kFewRows = 1024, kLeastKeys = 256;
 
 // ranges of a sequence's pages: `keys` each, fewer ranges where sequences fill the card
 int page_ranges(int64_t wgs, int64_t seqs, int64_t suffix_cap, int most, int64_t keys = 256) {
@@ -1242,8 +1244,8 @@ Plan make_plan(const qp_ctx* ctx, int batch, int t_max, bool padded, int64_t P, 
   const int64_t even = P * hkv * nrb / slots / 2;
   pl.ns2 = page_ranges(slots / 4, seqs, suffix_cap, 32, even > 256 ? even : 256);
   if (P > 0) {
-    const int64_t page_wgs = seqs * pl.ns2, left = page_wgs * 2 < slots ? slots - page_wgs : slots, least = pl.wr == 1 ? 128 : 64;
-    const int64_t most = (P + least - 1) / least, all = (hkv + 7) / 8 * 8 * nrb, places = nrb > kFewBlocks ? 3 * slots : left;
+    const int64_t page_wgs = seqs * pl.ns2, left = page_wgs * 2 < slots ? slots - page_wgs : slots;
+    const int64_t most = (P + kLeastKeys - 1) / kLeastKeys, all = (hkv + 7) / 8 * 8 * nrb, places = nrb > kFewBlocks ? 3 * slots : left;
     pl.once = (unsigned)left;
     pl.slots = (unsigned)slots;
     pl.prefix_wgs = (unsigned)(places > all ? places : all);
