@@ -200,7 +200,7 @@ __device__ __forceinline__ void add_odd_values(const BatchAttnParams& p, int kvh
 // A value that is not finite would spoil rows that do not see it (0 * infinity is NaN) and the sum of the two products below.  walk_keys puts zero in
 // its place, and the range ends with add_odd_values; walk_prefix does not look, but such a value leaves no result of its range finite, which is then
 // computed again with walk_keys.
-// What bounds it: two waves a SIMD (200 registers each) whose matrix instructions are 60 % of a tile's time with all eight row tiles filled (3072 of
+// What bounds it: two waves a SIMD (200 registers each) whose matrix instructions are 60 % of a tile's time with all eight row tiles filled (3100 of
 // 5164 clocks: 448 rows over 32785 keys, 62 us), the rest is the barrier and the loads' issue; with fewer rows the bytes: 56 rows over 504015 keys
 // 187 us, 5.5 TB/s.  Tried and slower: staging the prefix through registers, one tile ahead (448 rows 64.5 us, 72 rows over 30737 keys 44.4 against
 // 39.5); the loads issued between the products (64.1, 40.6); two tiles of 64 keys in LDS instead of three for 8 waves (61.8, 41.6); four (63.0, 40.5);
@@ -760,7 +760,10 @@ __device__ __forceinline__ void batch_attn_range(const BatchAttnParams& p, int k
       for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int e = 0; e < 16; ++e) z = __builtin_fmaf(st.o[db][e], 0.f, z);
-      if (row_live && z != 0.f) sh.odd = 1;
+      if (row_live && z != 0.f) {                              // (what the query of a token that is not there holds does not count)
+        const unsigned tok = (unsigned)r / (unsigned)p.G, seq = tok / (unsigned)p.t_max;
+        if (p.compact || (int)(tok - seq * p.t_max) < rows_new(p.pg, (int)seq, p.t_max)) sh.odd = 1;
+      }
       __syncthreads();
     }
     if (kPaged || sh.odd) {

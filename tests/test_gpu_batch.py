@@ -803,3 +803,77 @@ def test_attn_a_query_that_is_not_finite_spoils_its_own_rows_only(ops, hq, hkv, 
     got[B - 1, T - 1, 3], got[0, 0, hq - 1] = 0.0, 0.0                  # (those rows may be anything)
     ref[B - 1, T - 1, 3], ref[0, 0, hq - 1] = 0.0, 0.0
     check(got, ref, tol)
+
+
+@pytest.mark.parametrize("hq,hkv,P,B,T", [(28, 4, 4000, 20, 1), (28, 4, 20000, 12, 1), (8, 2, 20000, 600, 2), (32, 2, 40000, 48, 1)])
+def test_attn_idle_places_may_hold_anything(ops, hq, hkv, P, B, T):
+    """Places without a token, in batches that are computed with them: NaN in their queries reaches nothing, their outputs stay as they were."""
+    new = [0 if b % 3 else T for b in range(B)]
+    bt = Batch(hkv, 16, [b % 7 for b in range(B)], new, T, seed=B)
+    bt.fill([s + n for s, n in zip(bt.seq, bt.new)])
+    kpre, vpre = prefix_of(bt, P)
+    q = torch.full((B, T, hq, D), float("nan"), dtype=torch.bfloat16)
+    for b in range(B):
+        q[b, :new[b]] = bt.randn(new[b], hq, D)
+    ref, tol = attn_ref(q, kpre, vpre, P, bt, hq, D ** -0.5)
+    check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5), ref, tol)
+
+
+def test_attn_two_shapes_in_one_workspace_and_captured(ops):
+    """A large call and a small one share the larger one's workspace, one behind the other; captured together they replay with other lengths and tokens."""
+    hq, hkv, P = 28, 4, 9000
+    big, small = Batch(hkv, 16, [30, 0, 9], [20, 7, 20], 20, seed=1), Batch(hkv, 16, [3, 40], [1, 1], 1, seed=2)
+    big.fill([52, 22, 31]); small.fill([5, 43])
+    kpre, vpre = prefix_of(big, P)
+    ws = max((ops.batch_attn_workspace(b.B, b.T, P, b.width * b.ps, hq, hkv) for b in (big, small)), key=lambda t: t.numel())
+    calls = []
+    for b in (big, small):
+        kp, vp, table, sl, nn = b.cuda()
+        q = b.randn(b.B, b.T, hq, D)
+        calls.append((b, q, q.cuda(), kp, vp, table, sl, nn, torch.full((b.B, b.T, hq, D), float("nan"), dtype=torch.bfloat16, device="cuda")))
+
+    def go():
+        for b, _, qd, kp, vp, table, sl, nn, out in calls:
+            ops.batch_attn(qd, kpre, vpre, kpre.stride(0), P, kp, vp, table, sl, nn, hq, hkv, D, D ** -0.5, out, ws)
+
+    def compare():
+        for b, q, *_, out in calls:
+            ref, tol = attn_ref(q, kpre, vpre, P, b, hq, D ** -0.5)
+            check(out, ref, tol)
+
+    go(); go()
+    torch.cuda.synchronize()
+    compare()
+    g = torch.cuda.CUDAGraph()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        go()
+        with torch.cuda.graph(g, stream=s):
+            go()
+    torch.cuda.current_stream().wait_stream(s)
+    for step in range(3):
+        big.seq, big.new = [30 + step, step, 9], [20 - step, 7, 1 + step]
+        small.seq = [3 + step // 2, 40 + step]
+        for (b, q, qd, kp, vp, table, sl, nn, out) in calls:
+            sl.copy_(i32(b.seq)); nn.copy_(i32(b.new)); out.fill_(float("nan"))
+            q.copy_(b.randn(*q.shape)); qd.copy_(q)
+        g.replay()
+        torch.cuda.synchronize()
+        compare()
+        eager = [c[-1].clone() for c in calls]
+        go()
+        torch.cuda.synchronize()
+        for c, e in zip(calls, eager):
+            assert np.array_equal(f64(c[-1]), f64(e), equal_nan=True)
+
+
+def test_attn_infinite_values_in_the_prefill_form(ops):
+    hq, hkv, P, T = 4, 2, 8200, 130
+    bt = Batch(hkv, 16, [5, 0], [T, T], T, seed=9)
+    bt.fill([5 + T, T])
+    kpre, vpre = prefix_of(bt, P)
+    vpre[0, 0, 3] = float("inf"); vpre[0, P // 2, 5] = float("-inf"); vpre[1, P - 1, 100] = float("-inf"); vpre[1, P - 2, 7] = float("nan")
+    q = bt.randn(2, T, hq, D)
+    ref, tol = attn_ref(q, kpre, vpre, P, bt, hq, D ** -0.5)
+    check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5, n_new=None), ref, tol)
