@@ -104,6 +104,7 @@ struct Chunk {
 
 // What bounds it in a large batch is about half the logits' bytes and half the 64-bit exponentials: 32 x 5 rows of 152064 fp32 logits take 23 us, 14 us
 // with the 32-bit exponential instead.  More or fewer workgroups on a CU, or several chunks per workgroup with the next one's loads ahead, gained nothing.
+// A small call is a chain of latencies: maxima and sums per wave, which meet once, instead of a maximum of the whole chunk first (4 rows: 7.2 -> 5.3 us).
 template <bool kF32>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyParams p) {
   __shared__ double red[4], red_o[4];
