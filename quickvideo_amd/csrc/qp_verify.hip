@@ -56,10 +56,64 @@ __device__ __forceinline__ double exp2_neg(double y) {
 __device__ __forceinline__ double weight(float x, float top, double scale) {
   return exp2_neg(x == top ? 0.0 : ((double)x - (double)top) * scale);
 }
-__device__ __forceinline__ double wave_sum_f64(double v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+// Across the wave by vector instructions (data-parallel moves in rows of 16, then the two swaps): a step of a shuffle through LDS waits some hundred
+// clocks, and these calls are chains of such steps.  swap_lanes<0..5>: the other side of quads' pairs, quads' halves, eights' and rows' mirror images
+// (all lanes of the smaller group hold the same by then), rows, halves.
+template <int kStep>
+__device__ __forceinline__ unsigned swap_lanes(unsigned v, unsigned& own) {     // own: this side, as the swaps hand both over in two registers
+  own = v;
+  if constexpr (kStep == 0) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true);        // quad_perm 1 0 3 2
+  else if constexpr (kStep == 1) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true);   // quad_perm 2 3 0 1
+  else if constexpr (kStep == 2) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true);  // row_half_mirror
+  else if constexpr (kStep == 3) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true);  // row_mirror
+  else if constexpr (kStep == 4) { const auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false); own = x[0]; return x[1]; }
+  else { const auto x = __builtin_amdgcn_permlane32_swap(v, v, false, false); own = x[0]; return x[1]; }
+}
+template <int kStep = 0>
+__device__ __forceinline__ double wave_sum_f64(double v) {     // the same bits in every lane
+  if constexpr (kStep < 6) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+    unsigned lo, hi;
+    const unsigned olo = swap_lanes<kStep>((unsigned)b, lo), ohi = swap_lanes<kStep>((unsigned)(b >> 32), hi);
+    return wave_sum_f64<kStep + 1>(__builtin_bit_cast(double, (unsigned long long)hi << 32 | lo) + __builtin_bit_cast(double, (unsigned long long)ohi << 32 | olo));
+  } else {
+    return v;
+  }
+}
+// the largest value and, where several lanes hold it, the lowest number (kArg)
+template <bool kArg, int kStep = 0>
+__device__ __forceinline__ void wave_max(float& m, int& arg) {
+  if constexpr (kStep < 6) {
+    unsigned am, aa = 0, om, oa = 0;
+    om = swap_lanes<kStep>(__builtin_bit_cast(unsigned, m), am);
+    if (kArg) oa = swap_lanes<kStep>((unsigned)arg, aa);
+    const float a = __builtin_bit_cast(float, am), b = __builtin_bit_cast(float, om);
+    if (kArg) arg = b > a || (b == a && (int)oa < (int)aa) ? (int)oa : (int)aa;
+    m = fmaxf(a, b);
+    wave_max<kArg, kStep + 1>(m, arg);
+  }
+}
+// sum of this lane's and all lower lanes'
+template <int kCtrl, int kRows>
+__device__ __forceinline__ double from_below(double v) {       // 0 where nothing is below
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, kCtrl, kRows, 0xf, false);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), kCtrl, kRows, 0xf, false);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_scan_f64(double v) {
+  v += from_below<0x111, 0xf>(v);                              // row_shr 1, 2, 4, 8
+  v += from_below<0x112, 0xf>(v);
+  v += from_below<0x114, 0xf>(v);
+  v += from_below<0x118, 0xf>(v);
+  v += from_below<0x142, 0xa>(v);                              // the last lane of rows 0 and 2 to rows 1 and 3
+  v += from_below<0x143, 0xc>(v);                              // lane 31 to the upper half
   return v;
+}
+__device__ __forceinline__ double lane_f64(double v, int lane) {               // (lane: the same for all)
+  const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)b, lane), hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(b >> 32), lane);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
 template <int kWaves = 4>
 __device__ __forceinline__ double block_sum_f64(double v, double* red) {       // red: a double per wave; all threads get the sum
@@ -128,15 +182,9 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyParams p) 
   // Every wave against its own maximum; they meet once, at the end.
   double s = 0.0, o = 0.0;
   if (p.scale == 0.0) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-      const float om = __shfl_xor(m, d, 64);
-      const int oa = __shfl_xor(arg, d, 64);
-      if (om > m || (om == m && oa < arg)) { m = om; arg = oa; }
-    }
+    wave_max<true>(m, arg);
   } else {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    wave_max<false>(m, arg);
     if (m != -INFINITY) {
       bool holds = false;
 #pragma unroll
@@ -205,12 +253,7 @@ __device__ Decision decide(const VerifyParams& p, int b, int n) {
       if (c == lane) { cm = om; cs = p.sum[at + c]; }
       if (om > m || (om == m && oa < arg)) { m = om; arg = oa; }
     }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-      const float om = __shfl_xor(m, d, 64);
-      const int oa = __shfl_xor(arg, d, 64);
-      if (om > m || (om == m && oa < arg)) { m = om; arg = oa; }
-    }
+    wave_max<true>(m, arg);
     double z = 0.0, px = 0.0;
     if (p.scale != 0.0 && m != -INFINITY) {
       z = cs * weight(cm, m, p.scale);
@@ -316,22 +359,17 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyParams 
     int chunk = 0;                                             // the last one with a share so far
     for (int c0 = 0; c0 < p.nc; c0 += 64) {
       const double w = c0 ? share(c0 + tid) : held;
-      double incl = w;
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) {
-        const double o = __shfl_up(incl, k, 64);
-        if (tid >= k) incl += o;
-      }
+      const double incl = wave_scan_f64(w);
       const double before = run + (incl - w);
       const unsigned long long has = __ballot(w > 0.0), over = __ballot(w > 0.0 && run + incl > want);
       const unsigned long long pick = over ? (over & -over) : has;
       if (pick) {
         const int l = over ? __ffsll((long long)pick) - 1 : 63 - __clzll((long long)pick);
         chunk = c0 + l;
-        base = __shfl(before, l, 64);
+        base = lane_f64(before, __builtin_amdgcn_readfirstlane(l));
       }
       if (over) break;
-      run += __shfl(incl, 63, 64);
+      run += lane_f64(incl, 63);
     }
     if (tid == 0) { at_chunk = chunk; start = base; target = want; draw_kind = kind; draft = x; first = INT32_MAX; last = -1; }
   }
@@ -349,12 +387,7 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyParams 
   double w[kPickPer], sum = 0.0;
 #pragma unroll
   for (int i = 0; i < kPickPer; ++i) { w[i] = draw_weight(l[i], q[i], kind, d, p.scale); sum += w[i]; }
-  double incl = sum;
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) {
-    const double o = __shfl_up(incl, k, 64);
-    if ((tid & 63) >= k) incl += o;
-  }
+  const double incl = wave_scan_f64(sum);
   if ((tid & 63) == 63) red[tid >> 6] = incl;
   __syncthreads();
   double run = start + (incl - sum);
@@ -370,7 +403,8 @@ __global__ __launch_bounds__(kPickThreads) void verify_pick_kernel(VerifyParams 
     }
   }
   const unsigned long long hits = __ballot(hit != INT32_MAX), ables = __ballot(able >= 0);        // (one LDS atomic per wave: 1024 of them take 5 us)
-  const int wave_hit = __shfl(hit, hits ? __ffsll((long long)hits) - 1 : 0, 64), wave_able = __shfl(able, ables ? 63 - __clzll((long long)ables) : 0, 64);
+  const int wave_hit = __builtin_amdgcn_readlane(hit, __builtin_amdgcn_readfirstlane(hits ? __ffsll((long long)hits) - 1 : 0));
+  const int wave_able = __builtin_amdgcn_readlane(able, __builtin_amdgcn_readfirstlane(ables ? 63 - __clzll((long long)ables) : 0));
   if ((tid & 63) == 0) {
     if (hits) atomicMin(&first, wave_hit);
     if (ables) atomicMax(&last, wave_able);
