@@ -67,8 +67,8 @@ __global__ __launch_bounds__(256) void batch_rope_append_kernel(const uint4* __r
   }
   const uint4 ct = cos_t[row * 8 + (c & 7)], st = sin_t[row * 8 + (c & 7)];
   uint4 p;
-  p.x = __shfl_xor((int)x.x, 8, 16); p.y = __shfl_xor((int)x.y, 8, 16);
-  p.z = __shfl_xor((int)x.z, 8, 16); p.w = __shfl_xor((int)x.w, 8, 16);
+  auto across = [](unsigned v) { return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, true); };         // row_ror 8: lane i ^ 8 of 16
+  p.x = across(x.x); p.y = across(x.y); p.z = across(x.z); p.w = across(x.w);
   const float sign = (c < 8) ? -1.f : 1.f;
   const unsigned xw[4] = {x.x, x.y, x.z, x.w}, pw[4] = {p.x, p.y, p.z, p.w}, cw[4] = {ct.x, ct.y, ct.z, ct.w}, sw[4] = {st.x, st.y, st.z, st.w};
   unsigned o[4];
@@ -890,13 +890,14 @@ __global__ __launch_bounds__(64 * WR * WK, 2) void batch_attn_kernel(BatchAttnPa
         for (int b0 = 0; b0 < p.batch; b0 += 64) {
           const int b = b0 + (int)threadIdx.x, v = b < p.batch ? rows_new(p.pg, b, p.t_max) : 0;
           int incl = v;
-#pragma unroll
-          for (int k = 1; k < 64; k <<= 1) {
-            const int o = __shfl_up(incl, k, 64);
-            if ((int)threadIdx.x >= k) incl += o;
-          }
+          incl += __builtin_amdgcn_update_dpp(0, incl, 0x111, 0xf, 0xf, false);        // row_shr 1, 2, 4, 8; the last lanes of rows, of the lower half
+          incl += __builtin_amdgcn_update_dpp(0, incl, 0x112, 0xf, 0xf, false);
+          incl += __builtin_amdgcn_update_dpp(0, incl, 0x114, 0xf, 0xf, false);
+          incl += __builtin_amdgcn_update_dpp(0, incl, 0x118, 0xf, 0xf, false);
+          incl += __builtin_amdgcn_update_dpp(0, incl, 0x142, 0xa, 0xf, false);
+          incl += __builtin_amdgcn_update_dpp(0, incl, 0x143, 0xc, 0xf, false);
           if (b < p.batch) starts[b] = carry + incl - v;
-          carry += __shfl(incl, 63, 64);
+          carry += __builtin_amdgcn_readlane(incl, 63);
         }
         rows = row_blocks(carry, p.G, 32 * WR);
         int best = 1;
@@ -1044,8 +1045,7 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
     fetch(grp);
     float M = -1e30f;
     for (int i = tid; i < np; i += 256) M = fmaxf(M, ml(i).x);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+    M = wave_max_f32(M);
     if (lane == 0) red[wave] = M;
     __syncthreads();
     M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
@@ -1055,8 +1055,7 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
       lds_a[i] = x.y == 0.f ? 0.f : fmaxf(a, kTiny);           // an empty range left no o behind
       l = __builtin_fmaf(x.y, a, l);
     }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
+    l = wave_sum_f32(l);
     if (lane == 0) red[4 + wave] = l;
     __syncthreads();
     l = (red[4] + red[5]) + (red[6] + red[7]);
@@ -1075,13 +1074,11 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
   } else {                                                     // np <= 64: lane i holds part i
     const float2 x = lane < np ? ml(lane) : make_float2(-1e30f, 0.f);
     float M = x.x;
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+    M = wave_max_f32(M);
     float a = __builtin_amdgcn_exp2f((x.x - M) * p.c);
     l = x.y * a;
     a = x.y == 0.f ? 0.f : fmaxf(a, kTiny);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
+    l = wave_sum_f32(l);
     for (int i0 = 0; i0 < np; i0 += GROUPS * 4) {
       float4 v[4];
       float ak[4];
@@ -1100,8 +1097,7 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
       }
     }
   }
-  acc.x += __shfl_xor(acc.x, 32, 64); acc.y += __shfl_xor(acc.y, 32, 64);
-  acc.z += __shfl_xor(acc.z, 32, 64); acc.w += __shfl_xor(acc.w, 32, 64);
+  acc.x = xhalf_sum(acc.x); acc.y = xhalf_sum(acc.y); acc.z = xhalf_sum(acc.z); acc.w = xhalf_sum(acc.w);
   if (kWide) {
     if (lane < 32) lds_o[wave][lane32] = acc;
     __syncthreads();

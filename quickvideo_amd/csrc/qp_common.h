@@ -54,6 +54,39 @@ __device__ __forceinline__ float bf16_bits_to_f32(unsigned short b) { return __u
 // the RoPE / RMSNorm / SwiGLU kernels lose ~100 VALU instructions per 16-byte chunk.
 __device__ __forceinline__ unsigned short f32_to_bf16_bits(float f) { return __builtin_bit_cast(unsigned short, (__bf16)f); }
 __device__ __forceinline__ float round_bf16(float f) { return bf16_bits_to_f32(f32_to_bf16_bits(f)); }
+// Across the wave by vector instructions (data-parallel moves in rows of 16, then the two swaps): a step of a shuffle through LDS waits some hundred
+// clocks, and these calls are chains of such steps.  swap_lanes<0..5>: the other side of quads' pairs, quads' halves, eights' and rows' mirror images
+// (all lanes of the smaller group hold the same by then), rows, halves.
+template <int kStep>
+__device__ __forceinline__ unsigned swap_lanes(unsigned v, unsigned& own) {     // own: this side, as the swaps hand both over in two registers
+  own = v;
+  if constexpr (kStep == 0) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true);        // quad_perm 1 0 3 2
+  else if constexpr (kStep == 1) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true);   // quad_perm 2 3 0 1
+  else if constexpr (kStep == 2) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true);  // row_half_mirror
+  else if constexpr (kStep == 3) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true);  // row_mirror
+  else if constexpr (kStep == 4) { const auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false); own = x[0]; return x[1]; }
+  else { const auto x = __builtin_amdgcn_permlane32_swap(v, v, false, false); own = x[0]; return x[1]; }
+}
+template <int kStep = 0>
+__device__ __forceinline__ float wave_sum_f32(float v) {       // the same bits in every lane
+  if constexpr (kStep < 6) {
+    unsigned own;
+    const unsigned other = swap_lanes<kStep>(__builtin_bit_cast(unsigned, v), own);
+    return wave_sum_f32<kStep + 1>(__builtin_bit_cast(float, own) + __builtin_bit_cast(float, other));
+  } else {
+    return v;
+  }
+}
+template <int kStep = 0>
+__device__ __forceinline__ float wave_max_f32(float v) {
+  if constexpr (kStep < 6) {
+    unsigned own;
+    const unsigned other = swap_lanes<kStep>(__builtin_bit_cast(unsigned, v), own);
+    return wave_max_f32<kStep + 1>(fmaxf(__builtin_bit_cast(float, own), __builtin_bit_cast(float, other)));
+  } else {
+    return v;
+  }
+}
 // Correctly rounded fp32 square root.  hipcc's sqrtf/__fsqrt_rn can be 1 ulp off (measured: s = 262.03513 gave
 // 16.187498 instead of 16.1875, which flipped a bf16 round-to-even tie and with it a kept index); the fp64 square root
 // rounded once to fp32 is exact because sqrt of an fp32 value is never within 2^-48 of an fp32 rounding boundary.

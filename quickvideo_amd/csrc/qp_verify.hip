@@ -56,19 +56,6 @@ __device__ __forceinline__ double exp2_neg(double y) {
 __device__ __forceinline__ double weight(float x, float top, double scale) {
   return exp2_neg(x == top ? 0.0 : ((double)x - (double)top) * scale);
 }
-// Across the wave by vector instructions (data-parallel moves in rows of 16, then the two swaps): a step of a shuffle through LDS waits some hundred
-// clocks, and these calls are chains of such steps.  swap_lanes<0..5>: the other side of quads' pairs, quads' halves, eights' and rows' mirror images
-// (all lanes of the smaller group hold the same by then), rows, halves.
-template <int kStep>
-__device__ __forceinline__ unsigned swap_lanes(unsigned v, unsigned& own) {     // own: this side, as the swaps hand both over in two registers
-  own = v;
-  if constexpr (kStep == 0) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true);        // quad_perm 1 0 3 2
-  else if constexpr (kStep == 1) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true);   // quad_perm 2 3 0 1
-  else if constexpr (kStep == 2) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true);  // row_half_mirror
-  else if constexpr (kStep == 3) return (unsigned)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true);  // row_mirror
-  else if constexpr (kStep == 4) { const auto x = __builtin_amdgcn_permlane16_swap(v, v, false, false); own = x[0]; return x[1]; }
-  else { const auto x = __builtin_amdgcn_permlane32_swap(v, v, false, false); own = x[0]; return x[1]; }
-}
 template <int kStep = 0>
 __device__ __forceinline__ double wave_sum_f64(double v) {     // the same bits in every lane
   if constexpr (kStep < 6) {
