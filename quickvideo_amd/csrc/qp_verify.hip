@@ -270,7 +270,7 @@ __device__ __forceinline__ double draw_weight(float l, float q, int kind, const 
   return kind == LESS_DRAFT ? fmax(w - (double)q * d.z, 0.0) : w;
 }
 
-// (512 threads: the five rows of a four-draft sequence are joined by eight waves at once; 32 sequences 46.8 us in all, with 256 threads 49.6 - 51.5, with 1024 52.5)
+// (512 threads: the five rows of a four-draft sequence are joined by eight waves at once; then 32 sequences 46.8 us in all, with 256 threads 49.6 - 51.5, with 1024 52.5)
 constexpr int kRestThreads = 512, kRestPer = kChunk / kRestThreads, kRestWaves = kRestThreads / 64;
 template <bool kF32>
 __global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(VerifyParams p) {
