@@ -102,7 +102,7 @@ __device__ __forceinline__ double lane_f64(double v, int lane) {               /
   const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)b, lane), hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(b >> 32), lane);
   return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
-template <int kWaves = 4>
+template <int kWaves>
 __device__ __forceinline__ double block_sum_f64(double v, double* red) {       // red: a double per wave; all threads get the sum
   v = wave_sum_f64(v);
   __syncthreads();
