@@ -877,3 +877,18 @@ def test_attn_infinite_values_in_the_prefill_form(ops):
     q = bt.randn(2, T, hq, D)
     ref, tol = attn_ref(q, kpre, vpre, P, bt, hq, D ** -0.5)
     check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5, n_new=None), ref, tol)
+
+
+@pytest.mark.parametrize("B,T,n_new", [(12, 1, "given"), (8, 6, "given"), (4, 24, None)])
+def test_attn_prefix_heads_past_4_gb(ops, B, T, n_new):
+    """Heads of the prefix 2.4 GB apart: the third one's rows lie behind 2^32 bytes, in every form that stages the prefix its own way."""
+    hq, hkv, P, stride = 12, 3, 30000, 1_200_000_000
+    bt = Batch(hkv, 16, [4] * B, [T] * (B - 1) + [T if n_new is None else 0], T, seed=T)
+    bt.fill([4 + n for n in bt.new])
+    k, v = bt.randn(hkv, P, D), bt.randn(hkv, P, D)
+    far = [torch.empty((hkv - 1) * stride + P * D, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    views = [x.as_strided((hkv, P, D), (stride, D, 1)) for x in far]
+    views[0].copy_(k); views[1].copy_(v)
+    q = bt.randn(B, T, hq, D)
+    ref, tol = attn_ref(q, k, v, P, bt, hq, D ** -0.5)
+    check(run_attn(ops, q.cuda(), views[0], views[1], P, bt, hq, D ** -0.5, n_new=n_new), ref, tol)
