@@ -8,7 +8,6 @@
 //   batch_attn_kernel          attention of (batch x t_max) query rows over (shared prefix, own pages): partial results per key range
 //   batch_combine_kernel       joins the partial results of a row
 //   batch_attn_direct_kernel   both in one launch, for few keys
-//   batch_combine_wide_kernel  joins the pages' partial results with those the prefill kernel left of the prefix, for many tokens
 #include "qp_attn.h"
 
 namespace {
@@ -108,8 +107,6 @@ struct BatchAttnParams {
   // pages: ns2 key ranges, nrb2 row blocks per sequence and kv head
   int ns2, nrb2; unsigned page_wgs;
   float* part_o; float2* part_ml; // [hkv][ns2][R]
-  // many tokens: the prefix parts come from the prefill kernel (qp_attn_s6.hip) in its own layout, `wide_ns` per item of wide_rows tokens and a head
-  const float* wide; int wide_rows, wide_ns, wide_nqb;
 };
 
 // A padded batch (n_new given) is computed without its padding: the live tokens are numbered through, row = (live token) * G + g, and the workgroups are
@@ -205,9 +202,11 @@ __device__ __forceinline__ void add_odd_values(const BatchAttnParams& p, int kvh
 // 187 us, 5.5 TB/s.  Tried and slower: staging the prefix through registers, one tile ahead (448 rows 64.5 us, 72 rows over 30737 keys 44.4 against
 // 39.5); the loads issued between the products (64.1, 40.6); two tiles of 64 keys in LDS instead of three for 8 waves (61.8, 41.6); four (63.0, 40.5);
 // wave priorities (no effect).
-// P goes into the product as TWO bf16 numbers, bf16(p) and bf16(p - bf16(p)): 2^-17 of p is lost instead of 2^-9.  Rounded once, as the prefill and
-// decode kernels do it, the result's error against 64 bits is 0.0021 - 0.0027 of it, with two terms 0.0017, which is its own rounding; the second
-// product reuses the V fragments, and a step that waits for the prefix's bytes has the matrix pipe free.
+// P goes into the product as TWO bf16 numbers, bf16(p) and bf16(p - bf16(p)): 2^-16 of p is lost at most instead of 2^-8.  Rounded once, as the prefill
+// and decode kernels do it, the result's error against 64 bits is 0.0021 - 0.0027 of it, with two terms 0.0017, which is its own rounding; the second
+// product reuses the V fragments, and a step that waits for the prefix's bytes has the matrix pipe free.  Every form does so, also that of many tokens,
+// for which the prefill kernel with its one rounding is faster in part (28 and 4 heads, 4 x 61 tokens over 32785 keys 135 against 175 us, 96 x 1 76
+// against 89, 4 x 128 over 4096 keys 70 against 73, over 2048 52 both; 4 and 2 heads, 2 x 130 tokens over 8200 keys 47 against 26).
 template <int WR, int WK>
 struct Shape {
   static constexpr int NT = 64 * WR * WK, KB = WK == 1 ? 2 : 1, TILE = 32 * WK * KB, PT = TILE * 16 / NT;   // PT: 16-B pieces a thread stages of K and of V
@@ -1117,79 +1116,24 @@ __global__ __launch_bounds__(256) void batch_combine_kernel(BatchAttnParams p) {
   *reinterpret_cast<uint2*>(p.out + ((bt * p.hq) + (int64_t)kvh * p.G + g) * 128 + lane32 * 4) = y;
 }
 
-// Many tokens over a long prefix: joins, for 32 tokens of a head and 32 of the 128 dimensions, the prefill kernel's partial results (a lane reads
-// what the lane of the same number wrote: [wave][d / 8][lane][4], then (max, sum) [wave][2][lane]) and those of the pages.
-__global__ __launch_bounds__(64) void batch_combine_wide_kernel(BatchAttnParams p) {
-  const int items = p.wide_nqb * p.G, item = blockIdx.x % items, kvh = blockIdx.x / items;
-  const int qb = p.wide_nqb - 1 - item / p.G, g = item % p.G, wave = blockIdx.y, db = blockIdx.z, lane = threadIdx.x, hi = lane >> 5;
-  const int64_t rows = p.R / p.G, bt = (int64_t)qb * p.wide_rows + wave * 32 + (lane & 31);
-  if ((int64_t)qb * p.wide_rows + wave * 32 >= rows) return;
-  const int b = bt < rows ? (int)(bt / p.t_max) : 0, t = bt < rows ? (int)(bt - (int64_t)b * p.t_max) : 0;
-  const bool live = bt < rows && t < rows_new(p.pg, b, p.t_max);
-  const int pf = qpattn::partial_floats(p.wide_rows);
-  const float* base = p.wide + (int64_t)(kvh * items + item) * p.wide_ns * pf;
-  const float* ml = base + p.wide_rows * 128 + wave * 128 + lane;
-  const int64_t r = live ? bt * p.G + g : 0;
-  const float2* pml = p.part_ml + (int64_t)kvh * p.ns2 * p.R + r;
-  float M = -1e30f;
-  for (int i = 0; i < p.wide_ns; ++i) M = fmaxf(M, ml[(int64_t)i * pf]);
-  if (live)
-    for (int i = 0; i < p.ns2; ++i) M = fmaxf(M, pml[(int64_t)i * p.R].x);
-  float l = 0.f;
-  f32x4_t acc[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) acc[k] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < p.wide_ns; ++i) {
-    const float m = ml[(int64_t)i * pf], a = m == -1e30f ? 0.f : fmaxf(__builtin_amdgcn_exp2f((m - M) * p.c), kTiny);
-    l = __builtin_fmaf(ml[(int64_t)i * pf + 64], a, l);
-    const f32x4_t* o = reinterpret_cast<const f32x4_t*>(base + (int64_t)i * pf) + (wave * 16 + db * 4) * 64 + lane;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] += o[k * 64] * a;
-  }
-  if (!live) return;
-  for (int i = 0; i < p.ns2; ++i) {
-    const float2 x = pml[(int64_t)i * p.R];
-    if (x.y == 0.f) continue;                                  // an empty range left no o behind
-    const float a = fmaxf(__builtin_amdgcn_exp2f((x.x - M) * p.c), kTiny);
-    l = __builtin_fmaf(x.y, a, l);
-    const float* o = p.part_o + ((int64_t)kvh * p.ns2 * p.R + (int64_t)i * p.R + r) * 128 + db * 32 + 4 * hi;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] += *reinterpret_cast<const f32x4_t*>(o + 8 * k) * a;
-  }
-  const float inv = l != 0.f ? 1.0f / l : 0.f;                 // a row that sees no key is zero
-  uint16_t* out = p.out + ((bt * p.hq) + (int64_t)kvh * p.G + g) * 128 + db * 32 + 4 * hi;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    uint2 y = make_uint2(0, 0);
-    if (l != 0.f) {
-      y.x = (unsigned)f32_to_bf16_bits(acc[k][0] * inv) | ((unsigned)f32_to_bf16_bits(acc[k][1] * inv) << 16);
-      y.y = (unsigned)f32_to_bf16_bits(acc[k][2] * inv) | ((unsigned)f32_to_bf16_bits(acc[k][3] * inv) << 16);
-    }
-    *reinterpret_cast<uint2*>(out + 8 * k) = y;
-  }
-}
-
 struct Plan {
-  enum { kDirect, kWide, kRanges } form;
-  int wr, ns2, nrb2, ns_max, ns, wide_rows, wide_nqb, wide_ns;
+  int wr, ns2, nrb2, ns_max, ns;
   int64_t R;
   unsigned prefix_wgs, once, slots;
-  bool compact, many_parts;
+  bool direct, compact, many_parts;
 };
 
 // kDirectKeys: one launch against two, us, one sequence (sixteen), 28 query and 4 kv heads: 400 + 112 keys 10.5 against 11.5 (10.9, 13.4), 800 + 112
 // keys 13.6 against 11.6 (14.3, 14.2), 2400 keys 26 against 12.
-// kWideWork, tokens x prefix keys from which the prefill kernel wins, ranges against it, us: 96 tokens, 768 keys 16 against 30, 32785 keys 83 against 81;
-// 244 tokens, 1952 keys 35 against 44, 32785 keys 179 against 138; 512 tokens, 2048 keys 54 against 60, 4096 keys 87 against 73.
 // kShort, keys x heads below which a workgroup has a tile or two: see the table at make_plan().
 // kLeastKeys of a range, 64 / 128 / 192 / 256 / 384 / 512, us: 28 rows over 11535 keys - / 17.0 / 16.0 / 15.5 / 15.9 / 17.2, 231 padded rows over 4100 keys
 // 23.0 / 23.1 / 21.6 / 20.6, 672 rows over 768 keys 19.4 / 19.4 / 17.3 / 16.0: fewer parts to join.
 // kFewRows: a workgroup to join a row against a wave: 28 rows x 4 heads 17.5 against 20.8 us in all, 56 x 4 over an hour 186 against 192, 224 x 4 equal,
 // 1008 x 4 131 against 126, 3584 x 4 364 against 348.
-constexpr int64_t kDirectKeys = 640, kWideTokens = 96, kWideWork = 1 << 21, kShort = 65536, kFewRows = 1024, kLeastKeys = 256;
+constexpr int64_t kDirectKeys = 640, kShort = 65536, kFewRows = 1024, kLeastKeys = 256;
 
 // ranges of a sequence's pages: `keys` each, fewer ranges where sequences fill the card
-int page_ranges(int64_t wgs, int64_t seqs, int64_t suffix_cap, int most, int64_t keys = 256) {
+int page_ranges(int64_t wgs, int64_t seqs, int64_t suffix_cap, int most, int64_t keys) {
   int64_t ns2 = wgs / seqs;
   const int64_t by_keys = (suffix_cap + keys - 1) / keys;
   if (ns2 > by_keys) ns2 = by_keys;
@@ -1203,26 +1147,8 @@ Plan make_plan(const qp_ctx* ctx, int batch, int t_max, bool padded, int64_t P, 
   const int64_t tokens = (int64_t)batch * t_max;
   pl.R = tokens * G;
   if (t_max * G <= 32 && (int64_t)hkv * batch <= ctx->cus && P + suffix_cap <= kDirectKeys) {
-    pl.form = Plan::kDirect;
+    pl.direct = true;
     pl.ns2 = 1;
-    return pl;
-  }
-  // Tokens enough to fill row blocks of the prefill kernel head by head, all of them there, and a prefix long enough that its masked tiles (one per 64
-  // tokens: it takes the last prefix row for a new one) do not count.  Its probabilities are rounded to bf16 once, as in every prefill of this library.
-  if (!padded && tokens >= kWideTokens && P >= 4 * tokens && P * tokens >= kWideWork && P < (1 << 23)) {
-    pl.form = Plan::kWide;
-    const int64_t by128 = (tokens + 127) / 128 * 128, by256 = (tokens + 255) / 256 * 256;
-    pl.wide_rows = by128 < by256 ? 128 : 256;
-    pl.wide_nqb = (int)((tokens + pl.wide_rows - 1) / pl.wide_rows);
-    const int64_t items = (int64_t)hkv * G * pl.wide_nqb, slots = (int64_t)ctx->cus * (pl.wide_rows == 256 ? 1 : 2), tiles = (P + 63) / 64;
-    int64_t best = 0;
-    for (int ns = 1; ns <= 32 && ns * 8 <= tiles + 8; ++ns) {  // rounds of workgroups x (their tiles + what a range costs besides, about 4 tiles)
-      const int64_t cost = (items * ns + slots - 1) / slots * ((tiles + ns - 1) / ns + 4);
-      if (best == 0 || cost < best) { best = cost; pl.wide_ns = ns; }
-    }
-    pl.wr = pl.R / batch <= 64 ? 2 : 4;                        // the pages' own launch: narrow row blocks, many workgroups
-    pl.nrb2 = (int)(((int64_t)t_max * G + 32 * pl.wr - 1) / (32 * pl.wr));
-    pl.ns2 = page_ranges(2LL * ctx->cus, (int64_t)hkv * batch * pl.nrb2, suffix_cap, 16);
     return pl;
   }
   // Key ranges times row blocks.  Wide row blocks read the keys less often, narrow ones waste less on rows that are not there (the pages' workgroups
@@ -1236,7 +1162,6 @@ Plan make_plan(const qp_ctx* ctx, int batch, int t_max, bool padded, int64_t P, 
   //    16 x 24,      2688 rows         85.7 / 63.1 / 57.8 / 58.2     433   / 280  / 258  / 274
   //     8 x 128,     7168 rows          188 / 135  / 121  / 121     1022   / 762  / 690  / 653
   // (72 live rows of 144 over 30737 keys of 8 heads: 49.9 / 44.4 / 52.2 / 39.5; 56 rows over 504015: 217 / 187 / 186 / 192.)
-  pl.form = Plan::kRanges;
   pl.compact = padded && t_max > 1 && batch <= kMaxCompact && P > 0;
   if (P * hkv < kShort) pl.wr = pl.R <= 32 || (!pl.compact && pl.R <= 128) ? 1 : (pl.R <= 2048 ? 2 : 4);
   else pl.wr = pl.R <= 64 || (!pl.compact && pl.R <= 512) ? 2 : 8;
@@ -1267,8 +1192,8 @@ Plan make_plan(const qp_ctx* ctx, int batch, int t_max, bool padded, int64_t P, 
 }
 
 // where things lie in the workspace
-struct Layout { size_t pre_o, pre_ml, part_o, part_ml, starts, wide, end; };
-Layout layout_of(const Plan& pl, int batch, int hq, int hkv) {
+struct Layout { size_t pre_o, pre_ml, part_o, part_ml, starts, end; };
+Layout layout_of(const Plan& pl, int batch, int hkv) {
   Layout l;
   size_t at = 0;
   auto take = [&](size_t bytes) { const size_t a = at; at += (bytes + 255) & ~(size_t)255; return a; };
@@ -1276,7 +1201,6 @@ Layout layout_of(const Plan& pl, int batch, int hq, int hkv) {
   l.pre_o = take(prefix * 512); l.pre_ml = take(prefix * sizeof(float2));
   l.part_o = take(pages * 512); l.part_ml = take(pages * sizeof(float2));
   l.starts = take(pl.compact ? ((size_t)batch + 2) * sizeof(int) : 0);
-  l.wide = take(pl.form == Plan::kWide ? (size_t)hq * pl.wide_nqb * pl.wide_ns * qpattn::partial_floats(pl.wide_rows) * sizeof(float) : 0);
   l.end = at;
   return l;
 }
@@ -1314,8 +1238,8 @@ int qp_launch_batch_rope_append(const void* qkv, const void* cos, const void* si
 }
 
 size_t qp_batch_attn_workspace_bytes_impl(const qp_ctx* ctx, int batch, int t_max, int64_t P, int64_t suffix_cap, int hq, int hkv) {
-  const size_t a = layout_of(make_plan(ctx, batch, t_max, false, P, suffix_cap, hq, hkv), batch, hq, hkv).end;
-  const size_t b = layout_of(make_plan(ctx, batch, t_max, true, P, suffix_cap, hq, hkv), batch, hq, hkv).end;
+  const size_t a = layout_of(make_plan(ctx, batch, t_max, false, P, suffix_cap, hq, hkv), batch, hkv).end;
+  const size_t b = layout_of(make_plan(ctx, batch, t_max, true, P, suffix_cap, hq, hkv), batch, hkv).end;
   return a > b ? a : b;
 }
 
@@ -1324,7 +1248,7 @@ int qp_launch_batch_attn(const qp_ctx* ctx, const void* q, const void* k_prefix,
                          const int32_t* seq_len, const int32_t* n_new, int batch, int t_max, int hq, int hkv, float scale, void* out, void* workspace,
                          hipStream_t s) {
   const Plan pl = make_plan(ctx, batch, t_max, n_new != nullptr, P, (int64_t)max_pages * page_size, hq, hkv);
-  const Layout l = layout_of(pl, batch, hq, hkv);
+  const Layout l = layout_of(pl, batch, hkv);
   char* ws = (char*)workspace;
   BatchAttnParams p = {};
   p.q = (const uint4*)q; p.out = (uint16_t*)out;
@@ -1339,30 +1263,12 @@ int qp_launch_batch_attn(const qp_ctx* ctx, const void* q, const void* k_prefix,
   p.ns2 = pl.ns2; p.nrb2 = pl.nrb2;
   p.page_wgs = (unsigned)((int64_t)hkv * batch * pl.nrb2 * pl.ns2);
   int rc;
-  if (pl.form == Plan::kDirect) {
+  if (pl.direct) {
     static std::atomic<unsigned long long> opted{0};
     if ((rc = qp_opt_in_lds(opted, (const void*)batch_attn_direct_kernel, kDirectLds, "batch_attn_direct"))) return rc;
     batch_attn_direct_kernel<<<(unsigned)(hkv * batch), 64 * kDirectWaves, kDirectLds, s>>>(p);
     return qp_check_launch("batch_attn(direct)");
   }
-  if (pl.form == Plan::kWide) {
-    if ((rc = pl.wr == 2 ? launch_ranges<2, 2>(p, p.page_wgs, s) : launch_ranges<4, 1>(p, p.page_wgs, s))) return rc;
-    qpattn::AttnParams a = {};
-    a.q = (const uint4*)q; a.kp = p.k_pre; a.vp = p.v_pre; a.pre_hs16 = p.pre_hs16; a.P = P - 1;
-    a.kn = p.k_pre + (P - 1) * 16; a.vn = p.v_pre + (P - 1) * 16; a.new_hs16 = p.pre_hs16; a.n = 1;       // token i sees new rows 0 .. i: the one there is
-    a.hq = hq; a.group = p.G; a.c = p.c; a.nqb = pl.wide_nqb; a.hkv = hkv; a.items = pl.wide_nqb * p.G;
-    a.n_whole = 0; a.nsplit = pl.wide_ns; a.ws = (float*)(ws + l.wide);          // every item leaves partial results
-    a.heads_per_seq = hkv; a.kv_row_bytes = 256;
-    a.nq = batch * t_max; a.qb_rows = pl.wide_rows;
-    const qp_dev_switches& dev = qp_dev();
-    a.prio_mode = (dev.s6_prio.load(std::memory_order_relaxed) & 3) | ((dev.s6_early_out.load(std::memory_order_relaxed) & 3) << 2);
-    qp_launch_attn_s6(a, hkv <= 8 && 8 % hkv == 0, (unsigned)(a.items * a.nsplit), s);
-    if ((rc = qp_check_launch("batch_attn(wide)"))) return rc;
-    p.wide = a.ws; p.wide_rows = pl.wide_rows; p.wide_ns = pl.wide_ns; p.wide_nqb = pl.wide_nqb;
-    batch_combine_wide_kernel<<<dim3((unsigned)(hkv * a.items), (unsigned)(pl.wide_rows / 32), 4), 64, 0, s>>>(p);
-    return qp_check_launch("batch_attn(wide combine)");
-  }
-  p.wide_rows = 32 * pl.wr;                                    // (the joining kernel needs the block's rows)
   const unsigned grid = p.page_wgs + pl.prefix_wgs;
   switch (pl.wr) {
     case 1: rc = launch_ranges<1, 4>(p, grid, s); break;

@@ -892,3 +892,33 @@ def test_attn_prefix_heads_past_4_gb(ops, B, T, n_new):
     q = bt.randn(B, T, hq, D)
     ref, tol = attn_ref(q, k, v, P, bt, hq, D ** -0.5)
     check(run_attn(ops, q.cuda(), views[0], views[1], P, bt, hq, D ** -0.5, n_new=n_new), ref, tol)
+
+
+@pytest.mark.parametrize("T,n_new", [(1, "given"), (128, "given"), (128, None)])
+def test_attn_probabilities_go_into_the_product_as_two_terms(ops, T, n_new):
+    """Two keys have all the weight (the others' e^-350 is 0 in 32 bits), and in column t of row t their values balance: a probability rounded to bf16 once, off by
+    up to 2^-8 of it, shows there.  Of two terms 2^-16 is lost; besides that the exponent (products and scores are exact here: 2^-22 max |s|), the exponential
+    (2^-21), both again in the normaliser, four fp32 roundings, and the result's own: 2^-8 |o| + (2^-16 + 2 d + 2^-22) sum w |v|.  The same whatever the number
+    of tokens, with the counts given and without them."""
+    P, scale = 16384, D ** -0.5
+    bt = Batch(1, 16, [0], [T], T, seed=3)
+    bt.fill([T])
+    kpre = torch.zeros(1, P, D, dtype=torch.bfloat16)
+    kpre[:, 2:, 1] = -1.0
+    kpre[:, 0, 0] = 1.0
+    for j in range(T):
+        bt.row(bt.k_pool, 0, j).zero_()[:, 1] = -1.0
+    q = torch.zeros(1, T, 1, D, dtype=torch.bfloat16)
+    q[0, :, 0, 0] = torch.linspace(-9.0, 9.0, T) if T > 1 else 5.0
+    q[..., 1] = 4000.0
+    s = torch.stack([q[0, :, 0, 0].double() * scale, torch.zeros(T, dtype=torch.float64)], 1)
+    vpre = bt.randn(1, P, D)
+    vpre[:, 0], vpre[:, 1] = 1.0, 0.5
+    vpre[0, 1, :T] = -torch.exp(s[:, 0]).to(torch.bfloat16)
+    w = torch.softmax(s, 1)
+    ref, size = w @ vpre[0, :2].double(), w @ vpre[0, :2].double().abs()
+    d = 2.0 ** -22 * s.abs().amax(1, keepdim=True) + 2.0 ** -21
+    tol = 2.0 ** -8 * ref.abs() + (2.0 ** -16 + 2 * d + 2.0 ** -22) * size
+    got = run_attn(ops, q.cuda(), kpre.cuda(), vpre.cuda(), P, bt, 1, scale, n_new=n_new)
+    off = (got[0, :, 0].double().cpu() - ref).abs() - tol
+    assert (off <= 0).all(), off.max().item()
