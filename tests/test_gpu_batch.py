@@ -922,3 +922,23 @@ def test_attn_probabilities_go_into_the_product_as_two_terms(ops, T, n_new):
     got = run_attn(ops, q.cuda(), kpre.cuda(), vpre.cuda(), P, bt, 1, scale, n_new=n_new)
     off = (got[0, :, 0].double().cpu() - ref).abs() - tol
     assert (off <= 0).all(), off.max().item()
+
+
+# ------------------------------------------------------------------------------------------------------------- values near the type's largest
+@pytest.mark.parametrize("hq,hkv,P,B,T,n_new", [(8, 2, 300, 2, 2, "given"), (28, 4, 4000, 3, 1, "given"), (28, 4, 4000, 40, 1, "given"), (28, 4, 4000, 40, 1, None),
+                                                (16, 1, 66000, 3, 6, "given"), (28, 4, 16500, 2, 4, "given"), (4, 2, 8200, 2, 130, None)])
+def test_attn_large_finite_values_far_below_the_maximum(ops, hq, hkv, P, B, T, n_new):
+    """The last half of the prefix scores 360 below its first key (e^-360 is 0 in 32 bits) and holds one finite value row of 1e38: it adds nothing, in whichever
+    range it lies; the sequences' own rows score in between and hold one as well."""
+    bt = Batch(hkv, 16, [5] * B, [T] * B, T, seed=T)
+    bt.fill([5 + T] * B, scale=0.05)
+    kpre, vpre = prefix_of(bt, P, scale=0.05)
+    kpre[:, 0] = 4.0
+    kpre[:, P // 2:P] = -4.0
+    vpre[:, P - 2, ::3] = 1.0e38
+    for b in range(B):
+        bt.row(bt.v_pool, b, 3)[:, 1::3] = -1.0e38
+    q = (4.0 + 0.02 * torch.randn(B, T, hq, D, generator=bt.g)).to(torch.bfloat16)
+    ref, tol = attn_ref(q, kpre, vpre, P, bt, hq, D ** -0.5)
+    assert np.isfinite(ref).all() and np.abs(ref).max() < 100
+    check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5, n_new=n_new), ref, tol)
