@@ -204,8 +204,8 @@ __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyParams p) 
       const double f = weight(red_m[w], m, p.scale);
       s += red[w] * f; o += red_o[w] * f;
     }
-    if (draft >= v0 && draft < v0 + kChunk) p.others[(int64_t)b * p.T + t] = o;
   }
+  if (draft >= v0 && draft < v0 + kChunk) p.others[(int64_t)b * p.T + t] = o;              // (0 of a chunk that offers nothing)
   const int64_t at = ((int64_t)b * (p.T + 1) + t) * p.nc + ch;
   p.sum[at] = s; p.top[at] = m; p.arg[at] = arg;
 }

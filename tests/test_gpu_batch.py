@@ -942,3 +942,21 @@ def test_attn_large_finite_values_far_below_the_maximum(ops, hq, hkv, P, B, T, n
     ref, tol = attn_ref(q, kpre, vpre, P, bt, hq, D ** -0.5)
     assert np.isfinite(ref).all() and np.abs(ref).max() < 100
     check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5, n_new=n_new), ref, tol)
+
+
+def test_verify_a_certain_draft_in_a_chunk_that_is_filtered_out(ops):
+    """Top-k filters whole chunks of 4096 logits away; the refused draft lies in one of them.  The chunk's sum without the draft is 0, not what the workspace held."""
+    B, T, V = 3, 2, 3 * 4096
+    x, drafts, _, u = verify_case(B, T, V, torch.float32, False, seed=11)
+    x[:, :, 4096:8192] = float("-inf")
+    drafts[:] = 5000
+    want = verify_ref(x, drafts, None, None, u, 0.8)
+    ws = ops.verify_drafts_workspace(B, T, V)
+    for stale in (0xff, 0x7f):                                           # NaN; a number of 1e306
+        ws.fill_(stale)
+        acc, tok = torch.zeros(B, dtype=torch.int32, device="cuda"), torch.zeros(B, T + 1, dtype=torch.int64, device="cuda")
+        ops.verify_drafts(x.cuda(), drafts.cuda(), None, None, u.cuda(), 0.8, acc, tok, ws)
+        assert np.array_equal(acc.cpu().numpy(), want[0]) and np.array_equal(tok.cpu().numpy(), want[1])
+        chunks = 3
+        at = (B * (T + 1) * chunks + B * chunks) * 8                     # behind the sums of the rows' chunks and those of the refused rows
+        assert ws[at:at + B * T * 8].view(torch.float64).tolist() == [0.0] * (B * T)
