@@ -288,7 +288,9 @@ int qp_decode_advance(qp_ctx* ctx, int64_t* state, int64_t n_values, void* strea
  *                t >= n_new[b] is not read, not stored, and its outputs are left as they were.
  * Lengths and tables are read on the device: a captured step replays with new ones.  A page number outside [0, n_pages), a row behind
  * max_pages * page_size or a negative seq_len is never followed: such a row is not stored, and not attended.
- * batch * t_max <= 65536, prefix_len and max_pages * page_size <= 2^30; the context's device need not be the current one, `stream` must be the context device's.                    */
+ * batch * t_max <= 65536, prefix_len and max_pages * page_size <= 2^30.  qp_batch_attn refuses a batch whose launch would have 2^32 threads, and its workspace
+ * query gives 0 for it; batch * t_max * n_q_heads < 2^26 with batch * n_kv_heads < 2^22 is always within that.
+ * The context's device need not be the current one, `stream` must be the context device's. */
 /* Rotates the step's queries and keys and stores keys and values into the pages.  qkv bf16 [batch][t_max][(n_q + 2 n_kv) * 128]; cos /
  * sin bf16 [batch][t_max][64] (qp_mrope_table over batch * t_max positions); q_out bf16 [batch][t_max][n_q][128], not overlapping qkv.
  * Rotate-half as in qp_rope_append, in fp32 with ONE rounding to bf16 (qp_rope_append rounds after each step). */

@@ -769,6 +769,8 @@ int qp_batch_attn(qp_ctx* ctx, const void* q, const void* k_prefix, const void* 
   QP_REQUIRE(scale > 0.f && scale <= 3.0e38f, QP_ERR_INVALID, "%s: scale=%g must be positive and finite", who, (double)scale);
   QP_REQUIRE(aligned16(q) && aligned16(k_prefix) && aligned16(v_prefix) && aligned16(out) && aligned16(workspace), QP_ERR_INVALID, "%s: alignment", who);
   const size_t need = qp_batch_attn_workspace_bytes_impl(ctx, batch, t_max, prefix_len, (int64_t)max_pages * page_size, n_q_heads, n_kv_heads);
+  QP_REQUIRE(need > 0, QP_ERR_UNSUPPORTED, "%s: batch=%d x t_max=%d rows of %d / %d heads make a launch of 2^32 threads or more", who, batch, t_max, n_q_heads,
+             n_kv_heads);
   if (workspace_bytes < need) return qp_fail(QP_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", who, workspace_bytes, need);
   DeviceScope dev(ctx->device);
   return qp_launch_batch_attn(ctx, q, k_prefix, v_prefix, prefix_head_stride, prefix_len, k_pages, v_pages, page_stride, n_pages, page_size, page_table,

@@ -1217,6 +1217,13 @@ Layout layout_of(const Plan& pl, int batch, int hkv) {
   return l;
 }
 
+// grids x threads below 2^32, as a launch takes them (the direct form has a workgroup per CU at most)
+bool launches(const Plan& pl, int batch, int hkv) {
+  if (pl.direct) return true;
+  const int64_t threads = pl.wr == 8 ? 512 : 256, pages = (int64_t)hkv * batch * pl.nrb2 * pl.ns2, join = pl.many_parts ? pl.R * hkv : (pl.R * hkv + 3) / 4;
+  return (pages + pl.prefix_wgs) * threads < (1LL << 32) && join * 256 < (1LL << 32);
+}
+
 Pages pages_of(const int32_t* table, const int32_t* seq_len, const int32_t* n_new, int max_pages, int n_pages, int page_size, int64_t page_stride) {
   Pages pg;
   pg.table = table; pg.seq_len = seq_len; pg.n_new = n_new;
@@ -1249,10 +1256,16 @@ int qp_launch_batch_rope_append(const void* qkv, const void* cos, const void* si
   return qp_check_launch("batch_rope_append");
 }
 
+// 0: a launch would have 2^32 threads or more
 size_t qp_batch_attn_workspace_bytes_impl(const qp_ctx* ctx, int batch, int t_max, int64_t P, int64_t suffix_cap, int hq, int hkv) {
-  const size_t a = layout_of(make_plan(ctx, batch, t_max, false, P, suffix_cap, hq, hkv), batch, hkv).end;
-  const size_t b = layout_of(make_plan(ctx, batch, t_max, true, P, suffix_cap, hq, hkv), batch, hkv).end;
-  return a > b ? a : b;
+  size_t most = 0;
+  for (bool padded : {false, true}) {
+    const Plan pl = make_plan(ctx, batch, t_max, padded, P, suffix_cap, hq, hkv);
+    if (!launches(pl, batch, hkv)) return 0;
+    const size_t bytes = layout_of(pl, batch, hkv).end;
+    if (bytes > most) most = bytes;
+  }
+  return most;
 }
 
 int qp_launch_batch_attn(const qp_ctx* ctx, const void* q, const void* k_prefix, const void* v_prefix, int64_t prefix_head_stride, int64_t P,

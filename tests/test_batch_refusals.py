@@ -199,3 +199,20 @@ def test_tensors_without_plain_memory_are_refused(ops):
                           torch.zeros(2, 3, dtype=torch.int64), sparse)
     with pytest.raises((ValueError, RuntimeError)):
         ops.batch_rope_append(*(kw | {"qkv": kw["qkv"].to_sparse()}).values())
+
+
+@pytest.mark.parametrize("batch,t_max,n_q,n_kv,prefix,fits", [
+    (65536, 1, 1024, 1024, 200, False), (32768, 2, 1024, 1024, 200, False), (65536, 1, 128, 128, 200, True), (65536, 1, 128, 128, 1000, False),
+    (65536, 1, 64, 64, 200, True), (65536, 1, 64, 64, 1000, True), (65536, 1, 28, 4, 200, True), (16, 4096, 64, 8, 200, True), (1, 65536, 64, 64, 1000, True),
+])
+def test_batches_that_no_launch_takes_are_refused(lib, ctx, batch, t_max, n_q, n_kv, prefix, fits):
+    """grid x threads of a launch stay below 2^32: larger batches are refused before the first launch, and the workspace query says so.  65536 one-token
+    sequences x 128 key heads are 2^23 workgroups of the pages: of 256 threads over a short prefix, of 512 over a longer one."""
+    need = lib.qp_batch_attn_workspace_bytes(ctx[0], batch, t_max, prefix, 64, n_q, n_kv)
+    assert (need > 0) == fits
+    change = dict(batch=batch, t_max=t_max, n_q=n_q, n_kv=n_kv, prefix_len=prefix, stride=prefix * 128, page_stride=n_kv * 16 * 128)
+    if fits:
+        assert call(lib.qp_batch_attn, ctx, ATTN, **change, ws_bytes=need - 1) == -4
+    else:
+        assert call(lib.qp_batch_attn, ctx, ATTN, **change, ws_bytes=1 << 60) == -2
+        assert "2^32" in lib.qp_last_error().decode()
