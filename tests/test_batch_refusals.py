@@ -216,3 +216,10 @@ def test_batches_that_no_launch_takes_are_refused(lib, ctx, batch, t_max, n_q, n
     else:
         assert call(lib.qp_batch_attn, ctx, ATTN, **change, ws_bytes=1 << 60) == -2
         assert "2^32" in lib.qp_last_error().decode()
+
+
+@pytest.mark.parametrize("scale,good", [(1e8, True), (1.01e8, False), (1e9, False), (3e38, False), (1e-30, True)])
+def test_scales_that_leave_an_empty_range_finite(lib, ctx, scale, good):
+    """The running maximum of a row that has seen nothing is -1e30; a scale that makes -1e30 * scale * log2(e) infinite turned such a range into NaN."""
+    assert call(lib.qp_batch_attn, ctx, ATTN, scale=scale, ws_bytes=1000) == (-4 if good else -1)
+    assert ("workspace" if good else "scale") in lib.qp_last_error().decode()
