@@ -299,7 +299,7 @@ int qp_batch_rope_append(qp_ctx* ctx, const void* qkv, const void* cos, const vo
                          int64_t page_stride, int n_pages, int page_size, const int32_t* page_table, int max_pages, void* stream);
 /* Query (b, t) attends the prefix rows [0, prefix_len) and its sequence's rows j <= seq_len[b] + t (the step's rows must have been
  * appended).  The prefix is read once for the whole batch.  GQA native, any n_q / n_kv ratio.  q, out bf16 [batch][t_max][n_q][128] (out
- * may be q).  0 < scale <= 1e8; products q.k within +-1e30 before the scale.  A row that sees no key is zero; what a masked row holds (infinities, NaN) does not reach the result.  prefix tensors may
+ * may be q itself, not a part of it).  0 < scale <= 1e8; products q.k within +-1e30 before the scale.  A row that sees no key is zero; what a masked row holds (infinities, NaN) does not reach the result.  prefix tensors may
  * be NULL when prefix_len is 0.  workspace: qp_batch_attn_workspace_bytes with suffix_capacity = max_pages * page_size; a caller with
  * two of these calls in flight at once (two streams, two captured graphs) gives each its own. */
 size_t qp_batch_attn_workspace_bytes(const qp_ctx* ctx, int batch, int t_max, int64_t prefix_len, int64_t suffix_capacity, int n_q_heads,

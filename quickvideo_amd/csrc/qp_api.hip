@@ -769,6 +769,8 @@ int qp_batch_attn(qp_ctx* ctx, const void* q, const void* k_prefix, const void* 
   // (the kernels' empty running maximum is -1e30: times scale * log2(e) it has to stay finite, or a range of which a row sees nothing makes it NaN)
   QP_REQUIRE(scale > 0.f && scale <= 1.0e8f, QP_ERR_INVALID, "%s: scale=%g must be positive and at most 1e8", who, (double)scale);
   QP_REQUIRE(aligned16(q) && aligned16(k_prefix) && aligned16(v_prefix) && aligned16(out) && aligned16(workspace), QP_ERR_INVALID, "%s: alignment", who);
+  const size_t q_bytes = (size_t)batch * t_max * n_q_heads * 256;
+  QP_REQUIRE(out == q || !overlap(q, q_bytes, out, q_bytes), QP_ERR_INVALID, "%s: out overlaps q (it may be q itself)", who);
   const size_t need = qp_batch_attn_workspace_bytes_impl(ctx, batch, t_max, prefix_len, (int64_t)max_pages * page_size, n_q_heads, n_kv_heads);
   QP_REQUIRE(need > 0, QP_ERR_UNSUPPORTED, "%s: batch=%d x t_max=%d rows of %d / %d heads make a launch of 2^32 threads or more", who, batch, t_max, n_q_heads,
              n_kv_heads);

@@ -223,3 +223,9 @@ def test_scales_that_leave_an_empty_range_finite(lib, ctx, scale, good):
     """The running maximum of a row that has seen nothing is -1e30; a scale that makes -1e30 * scale * log2(e) infinite turned such a range into NaN."""
     assert call(lib.qp_batch_attn, ctx, ATTN, scale=scale, ws_bytes=1000) == (-4 if good else -1)
     assert ("workspace" if good else "scale") in lib.qp_last_error().decode()
+
+
+@pytest.mark.parametrize("shift,good", [(0, True), (16, False), (-16, False), (2 * 3 * 28 * 256 - 16, False), (2 * 3 * 28 * 256, True), (-2 * 3 * 28 * 256, True)])
+def test_out_is_q_or_apart_from_it(lib, ctx, shift, good):
+    assert call(lib.qp_batch_attn, ctx, ATTN, out=A + shift, ws_bytes=1000) == (-4 if good else -1)
+    assert ("workspace" if good else "overlaps") in lib.qp_last_error().decode()
