@@ -488,9 +488,13 @@ __device__ __forceinline__ void walk_keys(const BatchAttnParams& p, int kvh, int
 // instruction, lane i's 16 B at 16 i; the images are made by what each lane reads), kBuffers of them, so that the next ones are under way while one is
 // computed, with one barrier a tile.  Rows behind k1 read as zero (the buffer's bound).  The loads are asm, each with its own wait before the barrier:
 // hipcc would otherwise wait for all of them at the first LDS read.
+// m0 is written by name, so it is declared; hipcc warns that it is a reserved register (it keeps no variable there, but has uses of its own).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_to_lds(unsigned lds_at, int voff, u32x4_t rsrc) {       // (the wait states: rsrc may come from a vector instruction)
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds_at), "v"(voff), "s"(rsrc) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds_at), "v"(voff), "s"(rsrc) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 template <int N>
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory"); }
 
