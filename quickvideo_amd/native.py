@@ -151,7 +151,7 @@ def load_face():
     try:
         from . import _qp_torch
     except ImportError as e:
-        raise QuickPrefillUnavailable(f"quickvideo_amd/_qp_torch.so cannot be loaded ({e}): build it with `python -c 'import __graft_entry__ as g; g.build()'`") from e
+        raise QuickPrefillUnavailable(f"quickvideo_amd/_qp_torch.so cannot be loaded ({e}): build it with `python -c 'import __graft_entry__ as g; g.build()'` (or `make -C quickvideo_amd/csrc face`)") from e
     return _qp_torch
 
 
@@ -187,7 +187,6 @@ class QuickPrefillOps:
         # lock-releasing handle of the same .so: the producer thread, RCCL/gloo progress and Ctrl-C keep running meanwhile
         self.lib_blocking = load_library(hold_gil=False)
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        self._bind_face()
         h = _vp()
         self._check(self.lib.qp_create(ctypes.byref(h), self.device.index or 0))
         self.ctx = h
@@ -428,11 +427,15 @@ class QuickPrefillOps:
     # -- a batch of sequences over one prefilled video (include/quickprefill.h; batch.py drives them)
     # These run once per layer and token, so the module _qp_torch (csrc/qp_torch.cpp) reads the tensors and makes the call; it returns REFUSED, without a
     # call, when a tensor is not what the kernels take, and the _why_* functions here say what is wrong with it.
+    # It is loaded with the first of these calls, so that the other operators need the library alone.
+    _face = None
+
     def _bind_face(self):
         self._face = load_face()
         self._dev = self.device.index or 0
         self._stream_of = torch._C._cuda_getCurrentRawStream      # torch.cuda.current_stream(dev).cuda_stream without making a Stream object
         self._fns = {n: ctypes.cast(getattr(self.lib, n), _vp).value for n in ("qp_batch_rope_append", "qp_batch_attn", "qp_verify_drafts")}
+        return self._face
 
     def _after(self, status, why, *args):
         if status == self._face.REFUSED:
@@ -477,8 +480,9 @@ class QuickPrefillOps:
         """qkv [B, T, (n_q + 2 n_kv) * D] -> q_out [B, T, n_q, D] rotated; rotated keys and values into the sequences' pages
         [n_pages, n_kv, page_size, D] at rows seq_len[b] ...  cos / sin: bf16 [B, T, D/2] (or the [B * T, D/2] mrope_table returns).
         seq_len int32 [B], n_new int32 [B] or None (T each), table int32 [B, max_pages]."""
-        rc = self._face.batch_rope_append(self._fns["qp_batch_rope_append"], self.ctx.value or 0, self._dev, self._stream_of(self._dev), qkv, cos, sin, seq_len, n_new,
-                                          table, k_pages, v_pages, n_q, n_kv, head_dim, q_out)
+        face = self._face or self._bind_face()
+        rc = face.batch_rope_append(self._fns["qp_batch_rope_append"], self.ctx.value or 0, self._dev, self._stream_of(self._dev), qkv, cos, sin, seq_len, n_new,
+                                    table, k_pages, v_pages, n_q, n_kv, head_dim, q_out)
         if rc:
             self._after(rc, self._why_append, qkv, cos, sin, seq_len, n_new, table, k_pages, v_pages, n_q, n_kv, head_dim, q_out)
 
@@ -505,8 +509,9 @@ class QuickPrefillOps:
                    workspace):
         """q, out [B, T, n_q, D]: attention of every row over the shared prefix rows [0, prefix_len) (k_prefix / v_prefix as in prefill_attn, None
         without a prefix) and its sequence's pages up to and including its own row."""
-        rc = self._face.batch_attn(self._fns["qp_batch_attn"], self.ctx.value or 0, self._dev, self._stream_of(self._dev), q, k_prefix, v_prefix, prefix_head_stride,
-                                   prefix_len, k_pages, v_pages, table, seq_len, n_new, n_q, n_kv, head_dim, scale, out, workspace)
+        face = self._face or self._bind_face()
+        rc = face.batch_attn(self._fns["qp_batch_attn"], self.ctx.value or 0, self._dev, self._stream_of(self._dev), q, k_prefix, v_prefix, prefix_head_stride,
+                             prefix_len, k_pages, v_pages, table, seq_len, n_new, n_q, n_kv, head_dim, scale, out, workspace)
         if rc:
             self._after(rc, self._why_attn, q, k_prefix, v_prefix, prefix_head_stride, prefix_len, k_pages, v_pages, table, seq_len, n_new, n_q, n_kv, head_dim,
                         scale, out, workspace)
@@ -538,8 +543,9 @@ class QuickPrefillOps:
     def verify_drafts(self, logits, drafts, n_draft, draft_probs, uniforms, temperature, n_accepted, tokens, workspace):
         """logits [B, T + 1, V] (bf16 or fp32, rows contiguous), drafts int64 [B, T], n_draft int32 [B] or None, draft_probs fp32 [B, T, V] or None,
         uniforms fp32 [B, T + 1] (None when temperature is 0) -> n_accepted int32 [B], tokens int64 [B, T + 1]."""
-        rc = self._face.verify_drafts(self._fns["qp_verify_drafts"], self.ctx.value or 0, self._dev, self._stream_of(self._dev), logits, drafts, n_draft, draft_probs,
-                                      uniforms, temperature, n_accepted, tokens, workspace)
+        face = self._face or self._bind_face()
+        rc = face.verify_drafts(self._fns["qp_verify_drafts"], self.ctx.value or 0, self._dev, self._stream_of(self._dev), logits, drafts, n_draft, draft_probs,
+                                uniforms, temperature, n_accepted, tokens, workspace)
         if rc:
             self._after(rc, self._why_verify, logits, drafts, n_draft, draft_probs, uniforms, temperature, n_accepted, tokens, workspace)
 

@@ -229,3 +229,34 @@ def test_scales_that_leave_an_empty_range_finite(lib, ctx, scale, good):
 def test_out_is_q_or_apart_from_it(lib, ctx, shift, good):
     assert call(lib.qp_batch_attn, ctx, ATTN, out=A + shift, ws_bytes=1000) == (-4 if good else -1)
     assert ("workspace" if good else "overlaps") in lib.qp_last_error().decode()
+
+
+def test_the_other_operators_need_no_face(monkeypatch):
+    """An operator object comes up and works with the library alone; only a call of the batch operators asks for the module, and says how to build it."""
+    import sys
+
+    class Lib:
+        """the library's entry points that construction calls, without a device"""
+        def __getattr__(self, name):
+            return {"qp_create": lambda out, device: 0, "qp_select_workspace_bytes": lambda n: 16, "qp_destroy": lambda ctx: None,
+                    "qp_decode_advance": lambda *a: 0}[name]
+
+    monkeypatch.setitem(sys.modules, "quickvideo_amd._qp_torch", None)
+    monkeypatch.delattr("quickvideo_amd._qp_torch", raising=False)
+    monkeypatch.setattr(native, "load_library", lambda *a, **k: Lib())
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(native.QuickPrefillOps, "_stream", staticmethod(lambda: 0))
+    ops = native.QuickPrefillOps(torch.device("cpu"))
+    ops.decode_advance(torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(native.QuickPrefillUnavailable, match="make -C quickvideo_amd/csrc face"):
+        ops.batch_rope_append(*batch_tensors().values())
+
+
+def test_the_library_builds_without_torch():
+    """`make` asks neither g++ nor Python for anything (programs in C build the library alone); `make face` builds the module."""
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.abspath(native.__file__)), "csrc")
+    plan = lambda *goal: subprocess.run(["make", "-Bn", "-C", csrc, "PYTHON=echo no-python", *goal], capture_output=True, text=True, check=True).stdout   # noqa: E731
+    assert "libquickprefill.so" in plan() and "g++" not in plan() and "no-python" not in plan() and "_qp_torch" not in plan()
+    assert "g++" in plan("face") and "_qp_torch.so" in plan("face")
