@@ -542,7 +542,8 @@ class PrefillPipeline:
         """generation kwargs as the reference hands them to HF `generate` (qwen25_lvu.py:744-761); unset ones fall back to the
         checkpoint's generation_config.json (`model.generation_defaults`), then to greedy.  `num_beams > 1`: beam search with HF's
         semantics (`length_penalty`, `early_stopping`, with `do_sample` beam-search multinomial sampling; beam.py); `batched_beams`: the
-        beams of a step go through the model together and read the video's cache once (batch.py; one GPU).  `lookup_tokens`: up to that many
+        beams of a step go through the model together and read the video's cache once (batch.py; one GPU; with `num_beams` 1 there is one row a step
+        either way and the call is the one without it).  `lookup_tokens`: up to that many
         tokens a step are drafted from the prompt and the answer so far and verified in one pass over the cache (HF's prompt lookup, batch.py; one
         GPU, one beam).  Both are refused where they cannot work; neither changes what a call without them computes.
         `question`: the user's text, or the reference's `messages` list (chat(); qwen25_lvu.py:546-548) when the processor can

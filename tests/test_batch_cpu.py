@@ -254,3 +254,13 @@ def test_a_refused_step_changes_nothing():
     logits = dec.step(torch.tensor([[9], [0]]), [1, 0])
     dec.keep([1, 0])
     assert near(logits[0], alone(eng, seq + [9])[-1:])
+
+
+def test_batched_beams_with_one_beam_is_the_call_without_it():
+    import lvu
+    from quickvideo_amd.lvu import load_native_model
+    obj = lvu.LVU(lvu.LVUConfig("synthetic:tiny", top_p=0.5, video_group_size=4, num_frames=8), model=load_native_model("synthetic:tiny", device="cpu"))
+    obj._ops = BatchOracleOps()
+    run = lambda **kw: obj.generate("What happens?", "synthetic://?frames=16&h=56&w=84&fps=2&seed=3", max_new_tokens=6, eos_token_id=None, **kw)[0]      # noqa: E731
+    assert run(num_beams=1, batched_beams=True) == run(batched_beams=True) == run()
+    assert run(batched_beams=True, lookup_tokens=2) == run()
