@@ -548,6 +548,9 @@ __device__ __forceinline__ void walk_prefix(const BatchAttnParams& p, int kvh, b
 
 // The same for ONE row tile (WR = 1): nothing is shared, so every wave stages and computes 32-key blocks of its own (block first, first + WK, ... of the
 // range) in its own 16 KB of LDS, without a barrier; waves drift apart and hide each other's waiting.
+// A block is asked for when the one before is done.  Asking for the next one ahead costs 30 registers and does not pay, because a wave has two blocks here,
+// rarely more (us without and with it: one launch, 12 and 2 heads, 417 keys 9.5, 10.0; 28 and 4 heads, 7 rows, 300 keys 9.7, 9.6, 400 10.4, 10.8, 500 11.9,
+// 11.7; ranges of 256 keys, 7 rows over 4100 11.3, 11.1, 28 over 4100 11.95, 12.1, over 11535 13.45, 13.45, 64 rows of 8 heads over 2000 12.6, 12.7).
 template <int WK, bool kPaged>
 __device__ __forceinline__ void walk_alone(const BatchAttnParams& p, int kvh, int b, int64_t r, bool row_live, const bf16x8_t (&qf)[8], int k0, int k1, int first,
                                            unsigned char* lds, Shared& sh, Rows& st) {
@@ -596,10 +599,7 @@ __device__ __forceinline__ void walk_alone(const BatchAttnParams& p, int kvh, in
   const int voff = (((lane & 15) >> 2) << 6) + (((lane >> 4) & 1) << 5) + ((lane & 3) << 3) + (hi << 10);
   f32x16_t (&o)[4] = st.o;
   float m_run = st.m, l_run = st.l;
-  constexpr bool kAhead = !kPaged;                             // (the paged form would spill)
-  int t0 = k0 + first * 32;
-  if (kAhead && t0 < k1) load(t0);
-  for (; t0 < k1; t0 += 32 * WK) {
+  for (int t0 = k0 + first * 32; t0 < k1; t0 += 32 * WK) {
     load(t0);
     u16x2_t top = {0, 0};
 #pragma unroll
@@ -627,7 +627,6 @@ __device__ __forceinline__ void walk_alone(const BatchAttnParams& p, int kvh, in
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    if (kAhead && t0 + 32 * WK < k1) load(t0 + 32 * WK);
     f32x16_t s = (f32x16_t){0};
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk) {
@@ -1139,14 +1138,21 @@ struct Plan {
   bool direct, compact, many_parts;
 };
 
-// kDirectKeys: one launch against two, us, one sequence (sixteen), 28 query and 4 kv heads: 400 + 112 keys 10.5 against 11.5 (10.9, 13.4), 800 + 112
-// keys 13.6 against 11.6 (14.3, 14.2), 2400 keys 26 against 12.
-// kShort, keys x heads below which a workgroup has a tile or two: see the table at make_plan().
-// kLeastKeys of a range, 64 / 128 / 192 / 256 / 384 / 512, us: 28 rows over 11535 keys - / 17.0 / 16.0 / 15.5 / 15.9 / 17.2, 231 padded rows over 4100 keys
-// 23.0 / 23.1 / 21.6 / 20.6, 672 rows over 768 keys 19.4 / 19.4 / 17.3 / 16.0: fewer parts to join.
+// kDirectKeys: one launch against two, us, one sequence (sixteen), 28 query and 4 kv heads, up to 96 keys of the pages: 300 keys 9.8 against 11.0 (10.1,
+// 11.5), 400 10.5 against 11.0 (10.9, 11.8), 500 11.9 against 11.0 (12.0, 11.9), 600 11.7 against 11.1 (12.7, 12.0), 1000 15.0 against 11.0; 64 and 8
+// heads, 3 x 4 padded tokens, 500 keys 12.0 against 13.4, 800 14.9 against 13.2.
+// kOneTile, keys x heads x 32-row tiles of the batch below which blocks of one tile win: about a workgroup for each CU and 256 keys.  us with one tile and two:
+// 28 rows over 8000 keys of 4 heads 12.6, 12.9, over 11535 13.55, 13.35, over 16000 16.4, 14.6; 56 rows over 4100 12.5, 13.6, over 11535 15.9, 14.8; 448 rows
+// over 1000 14.7, 15.6, over 1500 21.3, 16.2; 32 rows over 24000 of 2 heads 14.6 both, over 32000 16.5, 15.3; 64 rows over 3000 of 8 13.3, 14.4, over 6000
+// 16.7, 15.6.  Not beyond kOneTileRows: 672 rows over 700 18.6, 16.5, 1400 over 100 26.8, 21.8.  Where a sequence has more rows than a tile its pages are read
+// several times, kOneTilePages keys x tiles at most: 3 x 6 padded tokens with 40 keys of their own over 2000 keys 13.0, 14.2, 8 x 6 with 1000 over 700 39.5, 24.4.
+// kShort, keys x heads below which a workgroup of many rows has few tiles: see the table at make_plan().
+// kLeastKeys of a range, 64 / 128 / 192 / 256 / 384 / 512, us: 28 rows over 11535 keys 16.1 / 15.4 / 13.4 / 13.7 / 14.5 / 16.8, over 4100 14.0 / 12.0 / 11.7 /
+// 12.0 / 13.5 / 15.0, 8 x 8 padded tokens over 4100 22.5 / 21.8 / 19.2 / 17.4 / 17.7 / 19.2, 672 rows over 768 keys 20.2 / 20.3 / 18.0 / 17.6 / 19.4 / 19.4:
+// fewer parts to join.
 // kFewRows: a workgroup to join a row against a wave: 28 rows x 4 heads 17.5 against 20.8 us in all, 56 x 4 over an hour 186 against 192, 224 x 4 equal,
 // 1008 x 4 131 against 126, 3584 x 4 364 against 348.
-constexpr int64_t kDirectKeys = 640, kShort = 65536, kFewRows = 1024, kLeastKeys = 256;
+constexpr int64_t kDirectKeys = 640, kOneTile = 60 << 10, kOneTileRows = 512, kOneTilePages = 24 << 10, kShort = 65536, kFewRows = 1024, kLeastKeys = 256;
 
 // ranges of a sequence's pages: `keys` each, fewer ranges where sequences fill the card
 int page_ranges(int64_t wgs, int64_t seqs, int64_t suffix_cap, int most, int64_t keys) {
@@ -1170,16 +1176,19 @@ Plan make_plan(const qp_ctx* ctx, int batch, int t_max, bool padded, int64_t P, 
   // Key ranges times row blocks.  Wide row blocks read the keys less often, narrow ones waste less on rows that are not there (the pages' workgroups
   // hold one sequence each) and start faster.  us with row blocks of 32 / 64 / 128 / 256 rows, 28 query and 4 kv heads:
   //                                    4100 keys                      32785 keys
-  //     4 x 1 token,   28 rows         12.7 / 14.4 / 14.8 / 14.0      23.2 / 21.3 / 22.0 / 22.6
-  //    16 x 1,        112 rows         16.5 / 18.1 / 23.0 / 18.5      33.9 / 28.9 / 32.1 / 29.7
-  //    64 x 1,        448 rows         28.6 / 28.2 / 32.7 / 34.4      84.6 / 62.8 / 68.5 / 67.5
-  //    32 x 4,        896 rows         37.2 / 36.4 / 35.2 / 40.0     155.2 / 112  / 106  / 107
-  //     8 x 64 padded, 1925 rows       61.0 / 50.8 / 53.5 / 56.6     299   / 212  / 201  / 196
-  //    16 x 24,      2688 rows         85.7 / 63.1 / 57.8 / 58.2     433   / 280  / 258  / 274
-  //     8 x 128,     7168 rows          188 / 135  / 121  / 121     1022   / 762  / 690  / 653
-  // (72 live rows of 144 over 30737 keys of 8 heads: 49.9 / 44.4 / 52.2 / 39.5; 56 rows over 504015: 217 / 187 / 186 / 192.)
+  //     4 x 1 token,   28 rows         12.0 / 12.4 / 12.5 / 14.0      21.9 / 20.3 / 20.3 / 21.9
+  //    16 x 1,        112 rows         15.1 / 14.8 / 16.9 / 18.1      33.0 / 28.7 / 31.3 / 28.6
+  //    64 x 1,        448 rows         28.1 / 27.0 / 27.1 / 34.4      83.6 / 60.4 / 62.9 / 64.2
+  //    32 x 4,        896 rows         38.9 / 34.9 / 33.6 / 38.0     155   / 111  / 101  / 102
+  //     8 x 64 padded, 1701, 2135      59.1 / 47.6 / 51.3 / 53.9     373   / 246  / 225  / 221
+  //    16 x 24,      2688 rows         86.0 / 62.6 / 57.4 / 56.6     431   / 281  / 259  / 273
+  //     8 x 128,     7168 rows          187 / 135  / 119  / 119     1039   / 762  / 697  / 652
+  // (77 live rows of 144 over 30737 keys of 8 heads: 43.6 / 39.2 / 40.3 / 36.1; 56 rows over 504015: 219 / 186 / 188 / 198.)
   pl.compact = padded && t_max > 1 && batch <= kMaxCompact && P > 0;
-  if (P * hkv < kShort) pl.wr = pl.R <= 32 || (!pl.compact && pl.R <= 128) ? 1 : (pl.R <= 2048 ? 2 : 4);
+  const int64_t tiles = (pl.R + 31) / 32, seq_rows = (int64_t)t_max * G;
+  const bool one_tile = seq_rows <= 32 ? pl.R <= kOneTileRows : pl.R <= 128 && hkv * batch * ((seq_rows + 31) / 32) * suffix_cap <= kOneTilePages;
+  if (one_tile && P * hkv * tiles < kOneTile) pl.wr = 1;
+  else if (P * hkv < kShort) pl.wr = pl.R <= 2048 ? 2 : 4;
   else pl.wr = pl.R <= 64 || (!pl.compact && pl.R <= 512) ? 2 : 8;
   const int rows = 32 * pl.wr, per_cu = pl.wr == 8 ? 1 : 2;     // resident workgroups (registers: two waves per SIMD)
   const int64_t nrb = (pl.R + rows - 1) / rows, slots = (int64_t)per_cu * ctx->cus;

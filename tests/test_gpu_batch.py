@@ -960,3 +960,24 @@ def test_verify_a_certain_draft_in_a_chunk_that_is_filtered_out(ops):
         chunks = 3
         at = (B * (T + 1) * chunks + B * chunks) * 8                     # behind the sums of the rows' chunks and those of the refused rows
         assert ws[at:at + B * T * 8].view(torch.float64).tolist() == [0.0] * (B * T)
+
+
+@pytest.mark.parametrize("hq,hkv,P,B,T,suffix,n_new", [
+    (28, 4, 1000, 64, 1, 20, "given"), (28, 4, 1500, 64, 1, 20, "given"), (28, 4, 700, 73, 1, 40, None), (28, 4, 700, 74, 1, 40, None), (64, 8, 2000, 8, 1, 30, "given"),
+    (8, 1, 12000, 16, 1, 9, None), (32, 2, 8000, 2, 1, 700, "given"), (28, 4, 2000, 3, 6, 40, "given"), (28, 4, 2000, 3, 6, 1000, "given"), (28, 4, 900, 4, 4, 5, "given"),
+    (33, 1, 700, 3, 1, 100, None), (32, 1, 700, 16, 1, 100, None),
+])
+@pytest.mark.parametrize("odd", [False, True])
+def test_attn_on_both_sides_of_the_one_tile_rule(ops, hq, hkv, P, B, T, suffix, n_new, odd):
+    """Batches of up to 512 rows over prefixes of about 256 keys a CU, with few and with many keys of their own, and just beyond; with infinite and NaN values in a
+    first, a middle and a last block of 32 keys."""
+    rs = np.random.RandomState(P + B)
+    new = rs.randint(0, T + 1, B) if n_new == "given" and T > 1 else np.full(B, T)
+    bt = Batch(hkv, 16, rs.randint(suffix // 2, suffix + 1, B).tolist(), new.tolist(), T, seed=B)
+    bt.fill([s + n for s, n in zip(bt.seq, bt.new)])
+    kpre, vpre = prefix_of(bt, P)
+    if odd:
+        vpre[0, 1, 3] = float("inf"); vpre[0, P // 2, 100] = float("-inf"); vpre[hkv - 1, P - 1, 7] = float("nan")
+    q = bt.randn(B, T, hq, D, scale=1.3)
+    ref, tol = attn_ref(q, kpre, vpre, P, bt, hq, D ** -0.5)
+    check(run_attn(ops, q.cuda(), kpre, vpre, P, bt, hq, D ** -0.5, n_new=n_new), ref, tol)
