@@ -35,3 +35,29 @@ def dev_switch():
     yield set_
     for name in touched:
         lib.qp_dev_switch(name.encode(), DEV_SWITCH_DEFAULTS[name])
+
+
+def cu_mask_status(words):
+    """What the HIP runtime says to a stream with this CU mask (0: it makes one); no error stays behind for the next call."""
+    import ctypes
+    hip = ctypes.CDLL("libamdhip64.so")
+    raw = ctypes.c_void_p()
+    status = hip.hipExtStreamCreateWithCUMask(ctypes.byref(raw), len(words), (ctypes.c_uint32 * len(words))(*words))
+    if status == 0:
+        hip.hipStreamDestroy(raw)
+    else:
+        hip.hipGetLastError()
+    return status
+
+
+def pytest_runtest_setup(item):
+    """test_prune_tail_inplace_many_streams_and_cu_mask asks for a stream whose mask names CUs of one XCD only (bit i is a CU of XCD i % 8, its bits are
+    multiples of 16).  Newer runtimes refuse any mask that leaves an XCD without a CU; where this one does, the test cannot be set up, and
+    tests/test_gpu_prune_streams.py has both of its halves with two CUs of every XCD."""
+    if item.name == "test_prune_tail_inplace_many_streams_and_cu_mask":
+        import torch
+        if torch.cuda.is_available():
+            torch.zeros(1, device="cuda")
+            status = cu_mask_status([0x00010001] * 8)
+            if status:
+                pytest.skip(f"hipExtStreamCreateWithCUMask: status {status} for a mask that leaves XCDs without a CU (see test_gpu_prune_streams.py)")
