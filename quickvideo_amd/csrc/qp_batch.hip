@@ -206,8 +206,8 @@ __device__ __forceinline__ void add_odd_values(const BatchAttnParams& p, int kvh
 // its place, and the range ends with add_odd_values; walk_prefix does not look, but such a value leaves no result of its range finite, which is then
 // computed again with walk_keys.
 // What bounds it: two waves a SIMD (200 registers each) whose matrix instructions are 60 % of a tile's time with all eight row tiles filled (3100 of
-// 5164 clocks: 448 rows over 32785 keys, 62 us), the rest is the barrier and the loads' issue; with fewer rows the bytes: 56 rows over 504015 keys
-// 187 us, 5.5 TB/s.  Tried and slower: staging the prefix through registers, one tile ahead (448 rows 64.5 us, 72 rows over 30737 keys 44.4 against
+// 5164 clocks: 448 live rows of 1708 over 32785 keys, 62 us), the rest is the barrier and the loads' issue; with fewer rows the bytes: 56 rows over 504015 keys
+// 186 us, 5.5 TB/s.  Tried and slower: staging the prefix through registers, one tile ahead (448 rows 64.5 us, 72 rows over 30737 keys 44.4 against
 // 39.5); the loads issued between the products (64.1, 40.6); two tiles of 64 keys in LDS instead of three for 8 waves (61.8, 41.6); four (63.0, 40.5);
 // wave priorities (no effect).
 // P goes into the product as TWO bf16 numbers, bf16(p) and bf16(p - bf16(p)): 2^-16 of p is lost at most instead of 2^-8.  Rounded once, as the prefill
@@ -1150,8 +1150,8 @@ struct Plan {
 // kLeastKeys of a range, 64 / 128 / 192 / 256 / 384 / 512, us: 28 rows over 11535 keys 16.1 / 15.4 / 13.4 / 13.7 / 14.5 / 16.8, over 4100 14.0 / 12.0 / 11.7 /
 // 12.0 / 13.5 / 15.0, 8 x 8 padded tokens over 4100 22.5 / 21.8 / 19.2 / 17.4 / 17.7 / 19.2, 672 rows over 768 keys 20.2 / 20.3 / 18.0 / 17.6 / 19.4 / 19.4:
 // fewer parts to join.
-// kFewRows: a workgroup to join a row against a wave: 28 rows x 4 heads 17.5 against 20.8 us in all, 56 x 4 over an hour 186 against 192, 224 x 4 equal,
-// 1008 x 4 131 against 126, 3584 x 4 364 against 348.
+// kFewRows, rows x heads up to which a workgroup joins a row, against a wave, us in all: 28 x 4 over 11535 keys 13.6 against 16.6, 56 x 4 over 504015 186
+// against 195, 112 x 4 over 32785 28.3 against 30.7, 224 x 4 over 11535 24.2 against 24.7, 336 x 4 33.8 against 31.8, 1008 x 4 over 32785 126 against 119.
 constexpr int64_t kDirectKeys = 640, kOneTile = 60 << 10, kOneTileRows = 512, kOneTilePages = 24 << 10, kShort = 65536, kFewRows = 1024, kLeastKeys = 256;
 
 // ranges of a sequence's pages: `keys` each, fewer ranges where sequences fill the card

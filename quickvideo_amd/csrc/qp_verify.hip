@@ -143,8 +143,8 @@ struct Chunk {
   }
 };
 
-// What bounds it in a large batch is about half the logits' bytes and half the 64-bit exponentials: 32 x 5 rows of 152064 fp32 logits take 23 us, 14 us
-// with the 32-bit exponential instead.  More or fewer workgroups on a CU, or several chunks per workgroup with the next one's loads ahead, gained nothing.
+// What bounds it in a large batch is about half the logits' bytes and half the 64-bit exponentials: 32 x 5 rows of 152064 fp32 logits take 21 us (23 in the
+// first calls, before the clocks have risen; 14 then with the 32-bit exponential instead).  More or fewer workgroups on a CU, or several chunks per workgroup with the next one's loads ahead, gained nothing.
 // A small call is a chain of latencies: maxima and sums per wave, which meet once, instead of a maximum of the whole chunk first (4 rows: 7.2 -> 5.3 us).
 template <bool kF32>
 __global__ __launch_bounds__(kThreads) void verify_stats_kernel(VerifyParams p) {
@@ -270,7 +270,8 @@ __device__ __forceinline__ double draw_weight(float l, float q, int kind, const 
   return kind == LESS_DRAFT ? fmax(w - (double)q * d.z, 0.0) : w;
 }
 
-// (512 threads: the five rows of a four-draft sequence are joined by eight waves at once; then 32 sequences 46.8 us in all, with 256 threads 49.6 - 51.5, with 1024 52.5)
+// (512 threads: the five rows of a four-draft sequence are joined by eight waves at once; when that was chosen 32 sequences took 46.8 us in all, with 256
+// threads 49.6 - 51.5, with 1024 52.5; 43 now)
 constexpr int kRestThreads = 512, kRestPer = kChunk / kRestThreads, kRestWaves = kRestThreads / 64;
 template <bool kF32>
 __global__ __launch_bounds__(kRestThreads) void verify_rest_kernel(VerifyParams p) {
